@@ -49,6 +49,8 @@ extern "C" {
 #define OM_ACT_NONE 0
 #define OM_ACT_RELU 1
 #define OM_ACT_RELU6 2
+/* x * sigmoid(x): only in the GroupNorm entry points (omCudaGroupNormActNhwc and its backward) */
+#define OM_ACT_SILU 3
 
 /* ---------------- device, memory, streams ---------------- */
 int omCudaInit(int nDeviceId);                                         /* replaces :287 */
@@ -583,6 +585,82 @@ int omCudaDepthwiseConv2dNhwc(const void* pIn, const float* pPacked, const float
 /* elementwise NHWC residual add + activation: out = act(a + b) (nDtype) */
 int omCudaAddActNhwc(const void* pA, const void* pB, void* pOut, long long nCount, int nAct,
                      int nDtype);
+
+/* ---------------- new: channels-last attention-block operators ----------------
+ * GroupNorm with its activation, attention and dropout on the NHWC storage of the fused path,
+ * each with its backward: GroupNorm + activation -> projection (a 1x1 omCudaConv2dBnAct to
+ * 3 * heads * head dim channels) -> attention on the projection's output in place ->
+ * projection -> dropout + residual. A [N, H, W, C] map is the token matrix [N, H*W, C].
+ * Workspaces are device memory of at least the stated bytes, 16-byte aligned, that the call may
+ * overwrite; one may be shared by calls on the same stream. Results do not depend on the order
+ * in which blocks run: no atomics. */
+
+/* Bytes of pWorkspace of omCudaGroupNormActNhwc (bBackward = 0) and of its backward (1);
+ * a negative OM_ERR_* for arguments those calls refuse. */
+long long omCudaGroupNormNhwcWorkspaceBytes(int nN, int nHW, int nC, int nCs, int nGroups,
+                                            int nDtype, int bBackward);
+/* y = act(gamma_c * (x - mean) * invstd + beta_c) on [nN, nHW, nCs] maps of nC channels
+ * (nC <= nCs, nCs % 8 == 0; stored channels past nC are written as 0), mean and
+ * invstd = 1 / sqrt(var + eps) over the nHW * nC / nGroups values of each (n, group), var the
+ * biased variance. Any of pGamma, pBeta (NULL: 1, 0), pMean, pInvStd ([nN, nGroups] outputs for
+ * the backward) may be NULL. nAct: OM_ACT_NONE, RELU, RELU6 or SILU; nDtype F32, BF16 or F16;
+ * statistics and arithmetic in fp32. pOut may be pIn. */
+int omCudaGroupNormActNhwc(const void* pIn, void* pOut, const float* pGamma, const float* pBeta,
+                           float* pMean, float* pInvStd, void* pWorkspace, int nN, int nHW, int nC,
+                           int nCs, int nGroups, float fEps, int nAct, int nDtype);
+/* The gradients of that call from dY, its input and the saved mean and invstd: dX [nN, nHW, nCs]
+ * (0 past nC) and, unless NULL, pGradGamma and pGradBeta [nC], fp32. The activation's derivative
+ * is taken at the recomputed pre-activation (ReLU: 0 at 0; ReLU6: 0 at 0 and 6). pGradIn may be
+ * pGradOut. */
+int omCudaGroupNormActNhwcBackward(const void* pGradOut, const void* pIn, const float* pMean,
+                                   const float* pInvStd, const float* pGamma, const float* pBeta,
+                                   void* pGradIn, float* pGradGamma, float* pGradBeta,
+                                   void* pWorkspace, int nN, int nHW, int nC, int nCs, int nGroups,
+                                   int nAct, int nDtype);
+/* out = (pResidual ? residual : 0) + (keep_i ? x * 65536 / (65536 - T) : 0), T = round(65536 p),
+ * for nCount contiguous elements of nDtype (F32, BF16, F16), arithmetic in fp32. Element i is
+ * kept where its 16 random bits are at least T: bits 16 * (i % 2) and up of word (i % 8) / 2 of
+ * Philox4x32-10 (Salmon, Moraes, Dror, Shaw, 2011) at counter (i / 8, nOffset) and key nSeed,
+ * each 64 bits, low word first. No mask is stored: the backward is the same call on dY with the
+ * same nSeed and nOffset and no residual (the residual's gradient is dY itself). Give every
+ * call of a training run its own nOffset. p in [0, 1]; a dropped NaN or infinity gives 0. pOut
+ * may be pIn or pResidual. */
+int omCudaDropoutAdd(const void* pIn, const void* pResidual, void* pOut, long long nCount,
+                     float fProb, unsigned long long nSeed, unsigned long long nOffset,
+                     int nDtype);
+/* Bytes of pWorkspace of omCudaAttention (bBackward = 0) and omCudaAttentionBackward (1); a
+ * negative OM_ERR_* for arguments those calls refuse. */
+long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int nKvHeads, int nSq, int nSk,
+                                        int nHeadDim, int bBackward);
+/* out = softmax(fScale * Q K^T) V per batch entry and head, without storing the scores.
+ * Q, out: [nBatch, nSq, nHeads, nHeadDim]; K, V: [nBatch, nSk, nKvHeads, nHeadDim], where head h
+ * reads key/value head h / (nHeads / nKvHeads) (nKvHeads divides nHeads). pStrides is a host array
+ * of 12 element strides: (batch, token, head) of Q, of K, of V and of out; the head dimension is
+ * contiguous. So Q, K and V may be the thirds of one projection output [N, S, 3, H, D], head-major
+ * [N, H, S, D] or token-major [N, S, H, D], without a copy. Strides of dimensions longer than 1
+ * are positive; strides are multiples of 8 and pointers 16-byte aligned.
+ * pQLens, pKvLens: optional device arrays [nBatch] of the tokens in use (clamped to [0, nSq] and
+ * [0, nSk]); what tokens past them hold is not used, NaN and infinities included. bCausal: query i
+ * sees keys j <= i + kvLen - qLen. A query that sees no key, or lies past its length, gets zeros.
+ * pLse [nBatch, nHeads, nSq] fp32 (NULL when no backward follows): log(sum exp(score)) of each
+ * query, minus infinity where it sees no key. nDtype BF16 or F16, nHeadDim a multiple of 8 up to
+ * 128 (else OM_ERR_UNSUPPORTED); scores, sums and accumulators in fp32, probabilities rounded to
+ * nDtype for their product with V. */
+int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut, float* pLse,
+                    const long long* pStrides, const int* pQLens, const int* pKvLens,
+                    void* pWorkspace, int nBatch, int nHeads, int nKvHeads, int nSq, int nSk,
+                    int nHeadDim, float fScale, int bCausal, int nDtype);
+/* The gradients of that call. The probabilities are recomputed from Q, K and the forward's pLse;
+ * pOut is the forward's output. pStrides: 24 element strides, (batch, token, head) of Q, K, V,
+ * out, dOut, dQ, dK, dV. dK and dV sum over the query heads that share a key/value head. dQ of
+ * queries that see no key or lie past their length, and dK, dV of keys past theirs, are zeros.
+ * dQ, dK and dV must not overlap an input. */
+int omCudaAttentionBackward(const void* pGradOut, const void* pQ, const void* pK, const void* pV,
+                            const void* pOut, const float* pLse, void* pGradQ, void* pGradK,
+                            void* pGradV, const long long* pStrides, const int* pQLens,
+                            const int* pKvLens, void* pWorkspace, int nBatch, int nHeads,
+                            int nKvHeads, int nSq, int nSk, int nHeadDim, float fScale,
+                            int bCausal, int nDtype);
 
 #ifdef __cplusplus
 }

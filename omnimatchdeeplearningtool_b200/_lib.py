@@ -28,6 +28,7 @@ STATUS_NAMES = {
 DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 DTYPE_U8 = 3   # 8-bit image samples (value / 255), an input dtype of the stem entry points
 ACT_NONE, ACT_RELU, ACT_RELU6 = 0, 1, 2
+ACT_SILU = 3   # GroupNorm entry points only
 
 
 class OmCudaError(RuntimeError):
@@ -169,6 +170,13 @@ _SIGS = {
     "omCudaPackDepthwiseWeight": [P, P, P, P, P, F, P, P, I, I, I, I],
     "omCudaDepthwiseConv2dNhwc": [P, P, P, P, I, I, I, I, I, I, I, I, I, I],
     "omCudaAddActNhwc": [P, P, P, c_longlong, I, I],
+    # channels-last attention-block operators
+    "omCudaGroupNormActNhwc": [P, P, P, P, P, P, P, I, I, I, I, I, F, I, I],
+    "omCudaGroupNormActNhwcBackward": [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I],
+    "omCudaDropoutAdd": [P, P, P, c_longlong, F, c_ulonglong, c_ulonglong, I],
+    "omCudaAttention": [P, P, P, P, P, POINTER(c_longlong), P, P, P] + [I] * 6 + [F, I, I],
+    "omCudaAttentionBackward": [P, P, P, P, P, P, P, P, P, POINTER(c_longlong), P, P, P] + [I] * 6 +
+                               [F, I, I],
 }
 for _name, _args in _SIGS.items():
     _fn = getattr(lib, _name)
@@ -188,11 +196,17 @@ lib.omCudaConvInputSplitBytes.argtypes = [I, I, I, I, I]
 lib.omCudaConvInputSplitBytes.restype = c_longlong
 lib.omCudaStemInputSplitBytes.argtypes = [I, I, I, I, I, I, I, I]
 lib.omCudaStemInputSplitBytes.restype = c_longlong
+lib.omCudaGroupNormNhwcWorkspaceBytes.argtypes = [I, I, I, I, I, I, I]
+lib.omCudaGroupNormNhwcWorkspaceBytes.restype = c_longlong
+lib.omCudaAttentionWorkspaceBytes.argtypes = [I, I, I, I, I, I, I]
+lib.omCudaAttentionWorkspaceBytes.restype = c_longlong
 
 EXPORTED = sorted(list(_SIGS) + ["omCudaGetStream", "omCudaPackedConvWeightElems",
                                  "omCudaPackedStemWeightElems", "omCudaStemWorkspaceBytes",
                                  "omCudaStoredChannels", "omCudaConvInputSplitBytes",
-                                 "omCudaStemInputSplitBytes"])
+                                 "omCudaStemInputSplitBytes",
+                                 "omCudaGroupNormNhwcWorkspaceBytes",
+                                 "omCudaAttentionWorkspaceBytes"])
 
 
 def check(status: int, fn: str = "omCuda") -> None:

@@ -1,0 +1,134 @@
+// Dropout with the residual add from a counter-based generator (omCudaDropoutAdd): the mask is
+// a function of (seed, offset, element index), so it is never stored and the backward pass
+// draws it again.
+//
+// Element i takes 16 bits of Philox4x32-10 (Salmon, Moraes, Dror, Shaw, "Parallel random
+// numbers: as easy as 1, 2, 3", SC 2011) at counter (i / 8, offset): one generator call serves
+// the 8 elements of a 16-byte vector. 16 bits give the drop probability in steps of 2^-16; the
+// scale is 65536 / (65536 - T) for the T that is used, so the expectation stays exact.
+#include "om_common.cuh"
+
+namespace omb {
+namespace drop {
+
+__device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint32_t k0, uint32_t k1) {
+#pragma unroll
+    for (int r = 0; r < 10; ++r) {
+        const unsigned long long p0 = (unsigned long long)c.x * 0xD2511F53u;
+        const unsigned long long p1 = (unsigned long long)c.z * 0xCD9E8D57u;
+        c = make_uint4((uint32_t)(p1 >> 32) ^ c.y ^ k0, (uint32_t)p1,
+                       (uint32_t)(p0 >> 32) ^ c.w ^ k1, (uint32_t)p0);
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return c;
+}
+
+template <int DT> struct Elem { using T = float; };
+template <> struct Elem<OM_DTYPE_BF16> { using T = __nv_bfloat16; };
+template <> struct Elem<OM_DTYPE_F16> { using T = __half; };
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ void from_f(float v, float& o) { o = v; }
+__device__ __forceinline__ void from_f(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void from_f(float v, __half& o) { o = __float2half_rn(v); }
+
+struct Params {
+    const void* x;
+    const void* res;
+    void* out;
+    long long n;
+    uint32_t k0, k1, o0, o1;
+    uint32_t thr;   // T: elements whose 16 bits are below it are dropped
+    float scale;
+};
+
+// One thread per 8 elements. VEC: all pointers 16-byte aligned, so full groups move in 16-byte
+// accesses; the last group, and every group otherwise, goes element by element.
+template <int DT, bool RES, bool VEC>
+__global__ void __launch_bounds__(256) dropout_kernel(const Params p) {
+    using T = typename Elem<DT>::T;
+    const T* x = static_cast<const T*>(p.x);
+    const T* res = static_cast<const T*>(p.res);
+    T* out = static_cast<T*>(p.out);
+    const long long groups = (p.n + 7) / 8;
+    for (long long g = blockIdx.x * 256LL + threadIdx.x; g < groups; g += gridDim.x * 256LL) {
+        const uint4 w = philox4x32_10(
+            make_uint4((uint32_t)g, (uint32_t)(g >> 32), p.o0, p.o1), p.k0, p.k1);
+        const uint32_t word[4] = {w.x, w.y, w.z, w.w};
+        alignas(16) T v[8], r[8];
+        const long long i0 = g * 8;
+        const int left = p.n - i0 < 8 ? (int)(p.n - i0) : 8;
+        if (VEC && left == 8) {
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j) {
+                reinterpret_cast<uint4*>(v)[j] = reinterpret_cast<const uint4*>(x + i0)[j];
+                if (RES)
+                    reinterpret_cast<uint4*>(r)[j] = reinterpret_cast<const uint4*>(res + i0)[j];
+            }
+        } else {
+            for (int j = 0; j < 8; ++j) {
+                v[j] = j < left ? x[i0 + j] : T(0.f);
+                if (RES) r[j] = j < left ? res[i0 + j] : T(0.f);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t bits = (word[j / 2] >> (16 * (j % 2))) & 0xFFFFu;
+            float y = bits >= p.thr ? to_f(v[j]) * p.scale : 0.f;
+            if (RES) y += to_f(r[j]);
+            from_f(y, v[j]);
+        }
+        if (VEC && left == 8) {
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+                reinterpret_cast<uint4*>(out + i0)[j] = reinterpret_cast<uint4*>(v)[j];
+        } else {
+            for (int j = 0; j < left; ++j) out[i0 + j] = v[j];
+        }
+    }
+}
+
+template <int DT, bool RES>
+static void launch(DeviceCtx* c, const Params& p, bool vec) {
+    const int grid = ew_grid(c, (p.n + 7) / 8, 256);
+    if (vec)
+        dropout_kernel<DT, RES, true><<<grid, 256, 0, c->compute>>>(p);
+    else
+        dropout_kernel<DT, RES, false><<<grid, 256, 0, c->compute>>>(p);
+}
+
+}  // namespace drop
+}  // namespace omb
+
+using namespace omb;
+
+extern "C" int omCudaDropoutAdd(const void* pIn, const void* pResidual, void* pOut,
+                                long long nCount, float fProb, unsigned long long nSeed,
+                                unsigned long long nOffset, int nDtype) {
+    OMB_CTX_OR_FAIL(c);
+    if (nCount < 0 || !(fProb >= 0.f && fProb <= 1.f)) return OM_ERR_INVALID;
+    if (nDtype != OM_DTYPE_F32 && nDtype != OM_DTYPE_BF16 && nDtype != OM_DTYPE_F16)
+        return OM_ERR_UNSUPPORTED;
+    if (nCount == 0) return OM_OK;
+    const uintptr_t any = reinterpret_cast<uintptr_t>(pIn) | reinterpret_cast<uintptr_t>(pOut) |
+                          reinterpret_cast<uintptr_t>(pResidual);
+    if (!pIn || !pOut || any % (nDtype == OM_DTYPE_F32 ? 4 : 2)) return OM_ERR_INVALID;
+    drop::Params p;
+    p.x = pIn; p.res = pResidual; p.out = pOut; p.n = nCount;
+    p.k0 = (uint32_t)nSeed; p.k1 = (uint32_t)(nSeed >> 32);
+    p.o0 = (uint32_t)nOffset; p.o1 = (uint32_t)(nOffset >> 32);
+    p.thr = (uint32_t)((double)fProb * 65536.0 + 0.5);
+    p.scale = p.thr < 65536 ? (float)(65536.0 / (65536.0 - p.thr)) : 0.f;
+    const bool vec = any % 16 == 0;
+    const bool res = pResidual != nullptr;
+    if (nDtype == OM_DTYPE_F32)
+        res ? drop::launch<OM_DTYPE_F32, true>(c, p, vec) : drop::launch<OM_DTYPE_F32, false>(c, p, vec);
+    else if (nDtype == OM_DTYPE_BF16)
+        res ? drop::launch<OM_DTYPE_BF16, true>(c, p, vec) : drop::launch<OM_DTYPE_BF16, false>(c, p, vec);
+    else
+        res ? drop::launch<OM_DTYPE_F16, true>(c, p, vec) : drop::launch<OM_DTYPE_F16, false>(c, p, vec);
+    return after_launch(c);
+}
