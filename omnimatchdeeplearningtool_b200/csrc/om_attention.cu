@@ -14,7 +14,7 @@ struct View {          // a [batch, token, head, D] tensor: element strides, D c
 struct Params {
     View q, k, v, o, dout, dq, dk, dv;
     float* lse;        // [B, H, Sq]
-    float* delta;      // [B, H, Sq], the row sums of dO o O
+    float* delta;      // [B, H, Sq], scale times the row sums of dO o O
     const int *qlens, *kvlens;
     int B, H, Hkv, Sq, Sk, D, causal;
     float scale;
@@ -34,25 +34,6 @@ __device__ __forceinline__ typename Half16<DT>::T* row_out(const View& v, int b,
 __device__ __forceinline__ int len_of(const int* lens, int b, int most) {
     return lens ? min(max(lens[b], 0), most) : most;
 }
-template <int DT>
-__device__ float dot(const typename Half16<DT>::T* a, const typename Half16<DT>::T* b, int D) {
-    float s = 0.f;
-    for (int d = 0; d < D; ++d) s += Half16<DT>::to_f(a[d]) * Half16<DT>::to_f(b[d]);
-    return s;
-}
-__device__ float block_reduce(float v, float* sh, bool is_max) {
-    for (int o = 16; o; o >>= 1) {
-        const float u = __shfl_xor_sync(~0u, v, o);
-        v = is_max ? fmaxf(v, u) : v + u;
-    }
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
-    __syncthreads();
-    v = sh[0];
-    for (int w = 1; w < (int)blockDim.x / 32; ++w) v = is_max ? fmaxf(v, sh[w]) : v + sh[w];
-    return v;
-}
-
 // ---------------------------------------------------------------- tcgen05 pieces
 // D[tmem] (+)= A[tmem] * B[smem]: A holds 16-bit pairs, one row per lane, K along the columns.
 __device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
@@ -401,69 +382,313 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(128) attn_dq_kernel(const Params p) {
-    using H16 = Half16<DT>;
-    __shared__ float sp[128];
-    const int i = blockIdx.x, h = blockIdx.y % p.H, b = blockIdx.y / p.H, t = threadIdx.x;
-    const int hk = h / (p.H / p.Hkv);
-    const int ql = len_of(p.qlens, b, p.Sq), kl = len_of(p.kvlens, b, p.Sk);
-    int end = i < ql ? kl : 0;
-    if (p.causal) end = min(end, i + kl - ql + 1);
-    const long long at = ((long long)b * p.H + h) * p.Sq + i;
-    const float lse = p.lse[at];
-    const float delta = end > 0 ? dot<DT>(row<DT>(p.dout, b, i, h), row<DT>(p.o, b, i, h), p.D) : 0.f;
-    if (t == 0) p.delta[at] = delta;
-    float acc = 0.f;
-    for (int j0 = 0; j0 < end; j0 += 128) {
-        const int j = j0 + t;
-        float ds = 0.f;
-        if (j < end) {
-            const float w = expf(dot<DT>(row<DT>(p.q, b, i, h), row<DT>(p.k, b, j, hk), p.D) * p.scale - lse);
-            ds = w * (dot<DT>(row<DT>(p.dout, b, i, h), row<DT>(p.v, b, j, hk), p.D) - delta) * p.scale;
-        }
-        __syncthreads();
-        sp[t] = ds;
-        __syncthreads();
-        if (t < p.D)
-            for (int jj = 0; jj < min(128, end - j0); ++jj)
-                acc += sp[jj] * H16::to_f(row<DT>(p.k, b, j0 + jj, hk)[t]);
-    }
-    if (t < p.D) row_out<DT>(p.dq, b, i, h)[t] = H16::from_f(acc);
-}
+// ---------------------------------------------------------------- backward
+// Both backward kernels are one template. KV = false (dQ): a CTA keeps Q and dO of 128 queries
+// and streams key/value blocks; KV = true (dK, dV): it keeps K and V of 128 keys and streams Q
+// and dO blocks of every query head that shares them. With X1, X2 the kept tiles and Y1, Y2 the
+// streamed ones, per block:
+//   S = X1 Y1^T, dP = X2 Y2^T                     (the transposes of S and dP for KV)
+//   P = exp(S - lse), dS = scale * P o (dP - delta)
+//   dQ += dS Y1                                   KV: dV += P Y2, dK += dS Y1
+// The thread of a row of S has the row of P^T or dS that the next product takes as its TMEM
+// operand, so P and dS never leave TMEM and nothing is transposed: Y1 and Y2 serve as K-major
+// operands of the first products and as MN-major operands of the others. dQ and dK, dV are
+// summed in two passes that each recompute S (7 products instead of 5): every sum is kept in one
+// CTA's TMEM, so no fp32 gradient is accumulated in memory by atomics and results are repeatable.
+// Two warpgroups share the tile: warpgroup w has columns 64 w .. 64 w + 63.
+// TMEM: S at 0, dP at 128 (P and dS over the first half of each 64 columns), accumulators behind.
+template <int DP>
+struct BwdCfg {
+    static constexpr int TILE = DP / 64 * PANEL;
+    static constexpr int SLOTS = DP == 128 ? 4 : 8;
+    static constexpr int STAT_OFF = (2 + SLOTS) * TILE;      // lse and delta of a block, two buffers
+    static constexpr int BAR_OFF = STAT_OFF + 2 * 2 * 128 * 4;
+    static constexpr int SMEM = BAR_OFF + 512 + 1024;
+    static constexpr int THREADS = 256 + 64;
+    static constexpr int ACC = 256, TMEM_COLS = 512;
+};
 
-// One block per (batch, key/value head, key), after attn_dq_kernel has left delta.
-template <int DT>
-__global__ void __launch_bounds__(128) attn_dkv_kernel(const Params p) {
-    using H16 = Half16<DT>;
-    __shared__ float sp[128], sd[128];
-    const int j = blockIdx.x, hk = blockIdx.y % p.Hkv, b = blockIdx.y / p.Hkv, t = threadIdx.x;
+template <int DP, bool KV, int DT>
+__global__ void __launch_bounds__(320, 1)
+attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2,
+                const __grid_constant__ CUtensorMap my1, const __grid_constant__ CUtensorMap my2,
+                const Params p) {
+    using Cf = BwdCfg<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    float* stat = reinterpret_cast<float*>(smem + Cf::STAT_OFF);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BAR_OFF);
+    uint64_t *x_full = bars, *s_full = bars + 1, *dp_full = bars + 2, *p_ready = bars + 3, *ds_ready = bars + 4,
+             *stat_ready = bars + 5, *acc_full = bars + 6, *drain = bars + 7;
+    uint64_t* full = bars + 8;
+    uint64_t* empty = full + Cf::SLOTS;
+    uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    constexpr int W_LOAD = 8, W_MMA = 9;
+    const int rep = p.H / p.Hkv, heads = KV ? p.Hkv : p.H;
+    const int hx = blockIdx.y % heads, b = blockIdx.y / heads;   // head of the kept tiles
+    const int hy0 = KV ? hx * rep : hx / rep;                    // first head of the streamed ones
+    const int r0 = (p.causal && !KV ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * 128;
     const int ql = len_of(p.qlens, b, p.Sq), kl = len_of(p.kvlens, b, p.Sk);
-    const int first = p.causal ? max(0, j - (kl - ql)) : 0;
-    float dk = 0.f, dv = 0.f;
-    if (j < kl)
-        for (int h = hk * (p.H / p.Hkv); h < (hk + 1) * (p.H / p.Hkv); ++h)
-            for (int i0 = first; i0 < ql; i0 += 128) {
-                const int i = i0 + t;
-                float w = 0.f, ds = 0.f;
-                if (i < ql) {
-                    const long long at = ((long long)b * p.H + h) * p.Sq + i;
-                    w = expf(dot<DT>(row<DT>(p.q, b, i, h), row<DT>(p.k, b, j, hk), p.D) * p.scale - p.lse[at]);
-                    ds = w * (dot<DT>(row<DT>(p.dout, b, i, h), row<DT>(p.v, b, j, hk), p.D) - p.delta[at]) * p.scale;
-                }
-                __syncthreads();
-                sp[t] = w;
-                sd[t] = ds;
-                __syncthreads();
-                if (t < p.D)
-                    for (int ii = 0; ii < min(128, ql - i0); ++ii) {
-                        dv += sp[ii] * H16::to_f(row<DT>(p.dout, b, i0 + ii, h)[t]);
-                        dk += sd[ii] * H16::to_f(row<DT>(p.q, b, i0 + ii, h)[t]);
-                    }
+    // streamed blocks: first .. first + per of each streamed head
+    int first = 0, per = 0;
+    if (KV) {
+        if (r0 < kl) {
+            first = p.causal ? max(0, r0 - (kl - ql)) / 128 : 0;
+            per = max(0, (ql + 127) / 128 - first);
+        }
+    } else {
+        int end = r0 < ql ? kl : 0;
+        if (p.causal) end = min(end, min(r0 + 128, ql) + kl - ql);
+        per = end > 0 ? (end + 127) / 128 : 0;
+    }
+    const int nblk = KV ? per * rep : per;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 8; ++i) mbar_init(bars + i, i == 3 || i == 4 || i == 5 ? 256 : 1);
+        for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == W_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                         smem_u32(tmem_holder)), "r"(Cf::TMEM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_holder;
+    unsigned int err = 0;
+
+    if (warp == W_LOAD) {
+        if (lane == 0 && nblk > 0) {
+            mbar_expect_tx(x_full, 2 * Cf::TILE);
+            load_tile<DP>(0, smem, &mx1, x_full, r0, hx, b);
+            load_tile<DP>(Cf::TILE, smem, &mx2, x_full, r0, hx, b);
+            int i = 0;
+            for (; i < 2 * nblk; ++i) {   // Y1, Y2 of each block in turn
+                const int slot = i % Cf::SLOTS, blk = i / 2;
+                if (!mbar_wait(empty + slot, ((i / Cf::SLOTS) & 1) ^ 1, abort_flag)) { err = ERR_LOAD; break; }
+                mbar_expect_tx(full + slot, Cf::TILE);
+                load_tile<DP>((2 + slot) * Cf::TILE, smem, i & 1 ? &my2 : &my1, full + slot,
+                              (first + blk % per) * 128, hy0 + blk / per, b);
             }
-    if (t < p.D) {
-        row_out<DT>(p.dk, b, j, hk)[t] = H16::from_f(dk);
-        row_out<DT>(p.dv, b, j, hk)[t] = H16::from_f(dv);
+            if (err || *abort_flag) {     // every load issued has to land before the CTA ends
+                *abort_flag = 1;
+                if (!mbar_wait_drain(x_full, 0)) err |= ERR_DRAIN;
+                for (int j = max(0, i - Cf::SLOTS); j < i; ++j)
+                    if (!mbar_wait_drain(full + j % Cf::SLOTS, (j / Cf::SLOTS) & 1)) err |= ERR_DRAIN;
+            }
+        }
+    } else if (warp == W_MMA) {
+        if (lane == 0 && nblk > 0) {
+            const int ks = (p.D + 15) / 16;
+            const bool f16 = DT == OM_DTYPE_F16;
+            const uint32_t id_s = idesc_f16(f16, 128, false, p.neg), id_dp = idesc_f16(f16, 128, false, false);
+            const uint32_t id_acc = idesc_f16(f16, ks * 16, true, false);
+            const uint32_t x1 = smem_u32(smem), x2 = x1 + Cf::TILE, y = x1 + 2 * Cf::TILE;
+            auto tile = [&](int i) { return y + (i % Cf::SLOTS) * Cf::TILE; };
+            auto wait_y = [&](int i) { return mbar_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
+            auto score = [&](uint32_t d, uint32_t x, int i, uint32_t id, uint64_t* bar) {
+                for (int k = 0; k < ks; ++k) tc_mma(tmem + d, desc_k(x, k), desc_k(tile(i), k), id, k > 0);
+                tc_commit(bar);
+            };
+            // the 128-long product over the rows of Y: the left operand's columns 0..63 are the 32
+            // words at `a`, columns 64..127 the 32 words at `a` + 64
+            auto accumulate = [&](uint32_t d, uint32_t a, int i, bool more) {
+                for (int k = 0; k < 8; ++k)
+                    tc_mma_ts(tmem + d, tmem + a + (k / 4) * 64 + (k % 4) * 8, desc_mn(tile(i), k), id_acc, more || k > 0);
+            };
+            bool ok = mbar_wait(x_full, 0, abort_flag) && wait_y(0);
+            if (ok) { tc_fence_after(); score(0, x1, 0, id_s, s_full); ok = wait_y(1); }
+            if (ok) score(128, x2, 1, id_dp, dp_full);
+            for (int i = 0; ok && i < nblk; ++i) {
+                const bool more = i + 1 < nblk;
+                ok = mbar_wait(p_ready, i & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                if (KV) accumulate(Cf::ACC + DP, 0, 2 * i + 1, i > 0);
+                if (more) {
+                    ok = wait_y(2 * i + 2);
+                    if (!ok) break;
+                    score(0, x1, 2 * i + 2, id_s, s_full);
+                }
+                ok = mbar_wait(ds_ready, i & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                accumulate(Cf::ACC, 128, 2 * i, i > 0);
+                tc_commit(empty + (2 * i) % Cf::SLOTS);
+                tc_commit(empty + (2 * i + 1) % Cf::SLOTS);
+                if (more) {
+                    ok = wait_y(2 * i + 3);
+                    if (!ok) break;
+                    score(128, x2, 2 * i + 3, id_dp, dp_full);
+                } else {
+                    tc_commit(acc_full);
+                }
+            }
+            if (!ok) {                    // no MMA may run on when the CTA ends
+                *abort_flag = 1;
+                err = ERR_MMA;
+                tc_commit(drain);
+                if (!mbar_wait_drain(drain, 0)) err |= ERR_DRAIN;
+            }
+        }
+        __syncwarp();
+    } else {
+        const int w = warp / 4, row = (warp % 4) * 32 + lane, tid = threadIdx.x;
+        const int r = r0 + row;
+        const uint32_t lanes = (uint32_t)(warp % 4) << 21;
+        const uint32_t s_addr = tmem + lanes + w * 64, dp_addr = s_addr + 128;
+        constexpr float LOG2E = 1.4426950408889634f;
+        bool ok = true;
+        float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's lse * log2(e) and scale * delta
+        int row_lo = 0, row_hi = 0;           // the streamed rows that this row meets
+        if (KV) {
+            if (r < kl) {
+                row_lo = p.causal ? max(0, r - (kl - ql)) : 0;
+                row_hi = ql;
+            }
+        } else {
+            row_hi = r < ql ? kl : 0;
+            if (p.causal) row_hi = min(row_hi, r + kl - ql + 1);
+            float d = 0.f;
+            if (row_hi > 0) {                 // half of dO . O, 8 elements at a time
+                const auto* go = attn::row<DT>(p.dout, b, r, hx);
+                const auto* o = attn::row<DT>(p.o, b, r, hx);
+                for (int c = w; c < p.D / 8; c += 2) {
+                    const uint4 u = reinterpret_cast<const uint4*>(go)[c], v = reinterpret_cast<const uint4*>(o)[c];
+                    const auto* a2 = reinterpret_cast<const typename Half16<DT>::T2*>(&u);
+                    const auto* b2 = reinterpret_cast<const typename Half16<DT>::T2*>(&v);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const float2 f = Half16<DT>::unpack(a2[x]), g = Half16<DT>::unpack(b2[x]);
+                        d += f.x * g.x + f.y * g.y;
+                    }
+                }
+                lse2 = p.lse[((long long)b * p.H + hx) * p.Sq + r] * LOG2E;
+            }
+            stat[tid] = d;
+            mbar_arrive(stat_ready);
+            ok = __all_sync(~0u, mbar_wait(stat_ready, 0, abort_flag));
+            ds0 = (stat[row] + stat[row + 128]) * p.scale;
+            if (ok && w == 0 && r < p.Sq) p.delta[((long long)b * p.H + hx) * p.Sq + r] = ds0;
+        }
+        // KV: thread tid fetches lse (tid < 128) or delta of one query of the next block
+        auto fetch = [&](int blk) {
+            const int i = (first + blk % per) * 128 + tid % 128;
+            if (i >= ql) return 0.f;
+            const long long at = ((long long)b * p.H + hy0 + blk / per) * p.Sq + i;
+            return tid < 128 ? p.lse[at] * LOG2E : p.delta[at];
+        };
+        float next = KV && nblk > 0 ? fetch(0) : 0.f;
+        for (int i = 0; ok && i < nblk; ++i) {
+            const int y0 = (first + i % per) * 128;
+            const float *c_lse = stat + (i & 1) * 256 + w * 64, *c_ds = c_lse + 128;
+            if (KV) {
+                stat[(i & 1) * 256 + tid] = next;
+                mbar_arrive(stat_ready);
+                if (i + 1 < nblk) next = fetch(i + 1);
+                ok = __all_sync(~0u, mbar_wait(stat_ready, i & 1, abort_flag));
+                if (!ok) break;
+            }
+            ok = __all_sync(~0u, mbar_wait(s_full, i & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t pv[64];
+            tmem_ld32_issue(s_addr, pv);
+            tmem_ld32_issue(s_addr + 32, pv + 32);
+            tmem_ld_wait<64>(pv);
+            float* pr = reinterpret_cast<float*>(pv);
+            if (!KV) {                        // S may be overwritten: P stays in registers
+                tc_fence_before();
+                mbar_arrive(p_ready);
+            }
+            const int lo = row_lo - y0 - w * 64, hi = row_hi - y0 - w * 64;
+            const bool mask = __any_sync(~0u, lo > 0 || hi < 64);
+#pragma unroll
+            for (int c = 0; c < 64; ++c) pr[c] = ex2(fmaf(pr[c], p.scale2, KV ? -c_lse[c] : -lse2));
+            if (mask) {
+#pragma unroll
+                for (int c = 0; c < 64; ++c) pr[c] = c >= lo && c < hi ? pr[c] : 0.f;
+            }
+            // streamed rows past the sequence's length may hold anything
+            const int y_end = KV ? ql : kl;
+            if (y_end - y0 < 128) {
+                const int iy = 2 * i + w;
+                ok = __all_sync(~0u, mbar_wait(full + iy % Cf::SLOTS, (iy / Cf::SLOTS) & 1, abort_flag));
+                if (!ok) break;
+                zero_tail<DP>(smem + (2 + iy % Cf::SLOTS) * Cf::TILE, y_end - y0, row);
+            }
+            if (KV) {
+                uint32_t pk[32];
+#pragma unroll
+                for (int c = 0; c < 32; ++c) pk[c] = pack16<DT>(pr[2 * c], pr[2 * c + 1]);
+                tmem_st32(s_addr, pk);
+                tmem_st_wait();
+                tc_fence_before();
+                mbar_arrive(p_ready);
+            }
+            ok = __all_sync(~0u, mbar_wait(dp_full, i & 1, abort_flag));
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t dv[64], dk[32];
+            tmem_ld32_issue(dp_addr, dv);
+            tmem_ld32_issue(dp_addr + 32, dv + 32);
+            tmem_ld_wait<64>(dv);
+            float* dp = reinterpret_cast<float*>(dv);
+#pragma unroll
+            for (int c = 0; c < 64; ++c) dp[c] = pr[c] * fmaf(dp[c], p.scale, KV ? -c_ds[c] : -ds0);
+            if (mask) {                       // 0 * what a masked place holds
+#pragma unroll
+                for (int c = 0; c < 64; ++c) dp[c] = c >= lo && c < hi ? dp[c] : 0.f;
+            }
+#pragma unroll
+            for (int c = 0; c < 32; ++c) dk[c] = pack16<DT>(dp[2 * c], dp[2 * c + 1]);
+            tmem_st32(dp_addr, dk);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(ds_ready);
+        }
+        if (ok && nblk > 0) ok = __all_sync(~0u, mbar_wait(acc_full, 0, abort_flag));
+        if (!ok) {
+            *abort_flag = 1;
+            err = ERR_MATH;
+        } else {
+            tc_fence_after();
+            // dQ: the warpgroups take alternate 32 columns; KV: the first writes dK, the second dV
+            const int rows = KV ? p.Sk : p.Sq;
+            const View& view = !KV ? p.dq : w == 0 ? p.dk : p.dv;
+            auto* out = r < rows ? row_out<DT>(view, b, r, hx) : nullptr;
+            const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w * DP : 0);
+            for (int c = KV ? 0 : w * 32; c < p.D; c += KV ? 32 : 64) {
+                uint32_t o[32];
+                if (nblk > 0) {
+                    tmem_ld32_issue(acc + c, o);
+                    tmem_ld_wait<32>(o);
+                }
+                const int n8 = min(32, p.D - c) / 8;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    uint32_t v[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+                        v[q] = nblk > 0 ? pack16<DT>(__uint_as_float(o[x * 8 + 2 * q]), __uint_as_float(o[x * 8 + 2 * q + 1]))
+                                        : 0u;
+                    if (out && x < n8) reinterpret_cast<uint4*>(out + c)[x] = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+            }
+        }
+    }
+    if (err) atomicOr(p.err, err);
+    tc_fence_before();
+    __syncthreads();
+    if (warp == W_MMA) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cf::TMEM_COLS));
     }
 }
 
@@ -536,6 +761,36 @@ static int forward(DeviceCtx* c, const Params& p) {
     return p.Sq <= 128 ? launch_fwd<128, 1, DT>(c, p) : launch_fwd<128, 2, DT>(c, p);
 }
 
+template <int DP, bool KV, int DT>
+static int launch_bwd(DeviceCtx* c, const CUtensorMap (&m)[4], const Params& p) {
+    using Cf = BwdCfg<DP>;
+    auto kern = attn_bwd_kernel<DP, KV, DT>;
+    static bool attr_set[64] = {false};
+    if (!attr_set[c->device]) {
+        OMB_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::SMEM));
+        attr_set[c->device] = true;
+    }
+    const dim3 grid(((KV ? p.Sk : p.Sq) + 127) / 128, p.B * (KV ? p.Hkv : p.H));
+    if (KV)
+        kern<<<grid, Cf::THREADS, Cf::SMEM, c->compute>>>(m[1], m[2], m[0], m[3], p);
+    else
+        kern<<<grid, Cf::THREADS, Cf::SMEM, c->compute>>>(m[0], m[3], m[1], m[2], p);
+    return after_launch(c);
+}
+template <int DP, int DT>
+static int backward(DeviceCtx* c, const Params& p) {
+    CUtensorMap m[4] = {};                // Q, K, V, dO
+    int st = OM_OK;
+    if (p.Sq > 0) st = encode(&m[0], p.q, p.B, p.Sq, p.H, p.D, DT);
+    if (st == OM_OK && p.Sk > 0) st = encode(&m[1], p.k, p.B, p.Sk, p.Hkv, p.D, DT);
+    if (st == OM_OK && p.Sk > 0) st = encode(&m[2], p.v, p.B, p.Sk, p.Hkv, p.D, DT);
+    if (st == OM_OK && p.Sq > 0) st = encode(&m[3], p.dout, p.B, p.Sq, p.H, p.D, DT);
+    // dQ first: it leaves delta for dK and dV
+    if (st == OM_OK && p.Sq > 0) st = launch_bwd<DP, false, DT>(c, m, p);
+    if (st == OM_OK && p.Sk > 0) st = launch_bwd<DP, true, DT>(c, m, p);
+    return st;
+}
+
 }  // namespace attn
 }  // namespace omb
 
@@ -602,21 +857,7 @@ extern "C" int omCudaAttentionBackward(const void* pGradOut, const void* pQ, con
     p.B = nBatch; p.H = nHeads; p.Hkv = nKvHeads; p.Sq = nSq; p.Sk = nSk; p.D = nHeadDim;
     p.causal = bCausal != 0; p.err = c->err_word;
     attn::set_scale(&p, fScale);
-    if (nSq > 0) {
-        const dim3 grid(nSq, nBatch * nHeads);
-        if (nDtype == OM_DTYPE_BF16)
-            attn::attn_dq_kernel<OM_DTYPE_BF16><<<grid, 128, 0, c->compute>>>(p);
-        else
-            attn::attn_dq_kernel<OM_DTYPE_F16><<<grid, 128, 0, c->compute>>>(p);
-        if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
-    }
-    if (nSk > 0) {
-        const dim3 grid(nSk, nBatch * nKvHeads);
-        if (nDtype == OM_DTYPE_BF16)
-            attn::attn_dkv_kernel<OM_DTYPE_BF16><<<grid, 128, 0, c->compute>>>(p);
-        else
-            attn::attn_dkv_kernel<OM_DTYPE_F16><<<grid, 128, 0, c->compute>>>(p);
-        if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
-    }
-    return OM_OK;
+    if (nHeadDim <= 64)
+        return nDtype == OM_DTYPE_BF16 ? attn::backward<64, OM_DTYPE_BF16>(c, p) : attn::backward<64, OM_DTYPE_F16>(c, p);
+    return nDtype == OM_DTYPE_BF16 ? attn::backward<128, OM_DTYPE_BF16>(c, p) : attn::backward<128, OM_DTYPE_F16>(c, p);
 }
