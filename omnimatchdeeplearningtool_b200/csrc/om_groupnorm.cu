@@ -1,169 +1,740 @@
 // GroupNorm with its activation on channels-last maps, forward and backward.
+//
+// z = gamma_c (x - mean) rstd + beta_c, y = act(z), statistics over the HW x C/G values of each
+// (sample, group). Backward, with dz = dy act'(z), xh = (x - mean) rstd and t = gamma_c dz:
+//   dbeta_c = sum dz, dgamma_c = sum dz xh, dx = rstd (t - mean(t) - xh mean(t xh)),
+// where the group means follow from the per-channel sums: mean(t) = sum_c gamma_c A_c / M with
+// A_c = sum dz, mean(t xh) = sum_c gamma_c B_c / M with B_c = sum dz xh.
+//
+// Bound by memory: the floor is one read of each input and one write of the output. A unit is
+// one sample's slab of channels (whole groups, at least 64 bytes of a pixel where there are as
+// many). Where a unit fits the shared memory of a cluster of up to 8 CTAs, one kernel reads it
+// once into shared memory, exchanges the sums over the cluster's distributed shared memory and
+// writes the output from there. Larger units take three launches: partial sums per chunk of
+// pixels, their combination, and the pass that reads the input again.
+// Statistics are fp32 means and centred sums of squares, merged pairwise (Chan, Golub, LeVeque,
+// 1979), so a mean far from zero costs no precision; every merge has a fixed order.
+#include <cooperative_groups.h>
+
 #include "om_common.cuh"
 
 namespace omb {
 namespace gn {
 
-template <int DT> struct Elem { using T = float; };
-template <> struct Elem<OM_DTYPE_BF16> { using T = __nv_bfloat16; };
-template <> struct Elem<OM_DTYPE_F16> { using T = __half; };
+namespace cg = cooperative_groups;
 
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ void from_f(float v, float& o) { o = v; }
-__device__ __forceinline__ void from_f(float v, __nv_bfloat16& o) { o = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void from_f(float v, __half& o) { o = __float2half_rn(v); }
+constexpr int T = 256;                    // threads of every block
+constexpr int MAX_VC = 256;               // 8-channel vectors of a pixel that one block covers
+constexpr int MAX_CLUSTER = 8;
+constexpr int SMEM_MAX = 227 * 1024;
+constexpr int MAX_GROUPS = 40;            // of a slab: it ends with the first unit of lcm(cpg, 8)
+                                          // channels that reaches 32, so below 32 / cpg + 8
 
-__device__ __forceinline__ float act_fwd(float z, int act) {
-    if (act == OM_ACT_SILU) return z / (1.f + __expf(-z));
-    return apply_act(z, act);
+template <int DT> struct Elem { using T = float; static constexpr int V16 = 2; };
+template <> struct Elem<OM_DTYPE_BF16> { using T = __nv_bfloat16; static constexpr int V16 = 1; };
+template <> struct Elem<OM_DTYPE_F16> { using T = __half; static constexpr int V16 = 1; };
+
+// 8 channels of one pixel: V16 16-byte pieces
+template <int DT> struct Vec { uint4 q[Elem<DT>::V16]; };
+
+template <int DT>
+__device__ __forceinline__ void unpack(const Vec<DT>& v, float (&f)[8]) {
+    if constexpr (DT == OM_DTYPE_F32) {
+        const float* s = reinterpret_cast<const float*>(&v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = s[i];
+    } else {
+        const auto* s = reinterpret_cast<const typename Half16<DT>::T2*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 u = Half16<DT>::unpack(s[i]);
+            f[2 * i] = u.x;
+            f[2 * i + 1] = u.y;
+        }
+    }
+}
+template <int DT>
+__device__ __forceinline__ Vec<DT> pack(const float (&f)[8]) {
+    Vec<DT> v;
+    if constexpr (DT == OM_DTYPE_F32) {
+        float* d = reinterpret_cast<float*>(&v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = f[i];
+    } else {
+        auto* d = reinterpret_cast<typename Half16<DT>::T2*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = Half16<DT>::pack(f[2 * i], f[2 * i + 1]);
+    }
+    return v;
+}
+template <int DT>
+__device__ __forceinline__ Vec<DT> load(const void* base, long long elem) {
+    Vec<DT> v;
+    const uint4* s = reinterpret_cast<const uint4*>(static_cast<const typename Elem<DT>::T*>(base) + elem);
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::V16; ++i) v.q[i] = __ldg(s + i);
+    return v;
+}
+template <int DT>
+__device__ __forceinline__ void store(void* base, long long elem, const Vec<DT>& v) {
+    uint4* d = reinterpret_cast<uint4*>(static_cast<typename Elem<DT>::T*>(base) + elem);
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::V16; ++i) d[i] = v.q[i];
+}
+// Slot s of a thread's own shared memory, in planes of T 16-byte pieces (no bank conflicts); the
+// copy is asynchronous and only the thread that issued it reads it.
+template <int DT>
+__device__ __forceinline__ void copy_in(uint4* sm, int s, const void* base, long long elem) {
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const typename Elem<DT>::T*>(base) + elem);
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::V16; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         (uint32_t)__cvta_generic_to_shared(sm + (s * Elem<DT>::V16 + i) * T + threadIdx.x)),
+                     "l"(src + i) : "memory");
+}
+template <int DT>
+__device__ __forceinline__ Vec<DT> own(const uint4* sm, int s) {
+    Vec<DT> v;
+#pragma unroll
+    for (int i = 0; i < Elem<DT>::V16; ++i) v.q[i] = sm[(s * Elem<DT>::V16 + i) * T + threadIdx.x];
+    return v;
+}
+__device__ __forceinline__ void copies_done() {
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+}
+
+template <int ACT>
+__device__ __forceinline__ float act_fwd(float z) {
+    if (ACT == OM_ACT_SILU) return __fdividef(z, 1.f + __expf(fminf(-z, 80.f)));
+    return apply_act(z, ACT);
 }
 // dz = dy * act'(z)
-__device__ __forceinline__ float act_bwd(float dy, float z, int act) {
-    if (act == OM_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-z));
+template <int ACT>
+__device__ __forceinline__ float act_bwd(float dy, float z) {
+    if (ACT == OM_ACT_SILU) {
+        const float s = __fdividef(1.f, 1.f + __expf(fminf(-z, 80.f)));
         return dy * (s * (1.f + z * (1.f - s)));
     }
-    if (act == OM_ACT_RELU) return z > 0.f ? dy : 0.f;
-    if (act == OM_ACT_RELU6) return z > 0.f && z < 6.f ? dy : 0.f;
+    if (ACT == OM_ACT_RELU) return z > 0.f ? dy : 0.f;
+    if (ACT == OM_ACT_RELU6) return z > 0.f && z < 6.f ? dy : 0.f;
     return dy;
 }
 
 struct Params {
-    const void* x;
-    const void* dy;
+    const void *x, *dy;
     void* out;
     const float *gamma, *beta;
-    float *mean, *rstd;   // forward: written when given
+    float *mean, *rstd;       // [N, G]: written by the forward when given, read by the backward
     float *dgamma, *dbeta;
-    int N, HW, C, Cs, G, act;
+    float* ws;
+    int N, HW, C, Cs, G;
     float eps;
+    int cpg;
+    int vc;                   // vectors of a slab
+    int nslab;
+    int cluster;              // CTAs of a unit
+    int rows;                 // pixels of a CTA's part
+    int iters;                // of them per thread
+    int nchunk;               // parts of a sample (three-launch form)
 };
 
-// Sum over the block (blockDim.x a multiple of 32), the result in every thread.
+// What a thread works on: vector column cv of pixels first, first + step, ... < end
+struct Part {
+    int n, c0, nval;          // sample, first channel, channels of it that are not padding
+    int first, step, end;
+    bool active;
+    long long base;           // element of (n, pixel 0, c0)
+};
+__device__ __forceinline__ Part part_of(const Params& p, int n, int slab, int piece) {
+    Part t;
+    const int cv = threadIdx.x % p.vc, r = threadIdx.x / p.vc;
+    t.n = n;
+    t.step = T / p.vc;
+    t.c0 = (slab * p.vc + cv) * 8;
+    t.active = r < t.step && t.c0 < p.Cs;
+    t.nval = min(max(p.C - t.c0, 0), 8);
+    t.first = piece * p.rows + r;
+    t.end = t.active ? min((piece + 1) * p.rows, p.HW) : 0;
+    t.base = (long long)n * p.HW * p.Cs + t.c0;
+    return t;
+}
+__device__ __forceinline__ long long at(const Params& p, const Part& t, int pixel) {
+    return t.base + (long long)pixel * p.Cs;
+}
+
+// Two per-channel values of every thread, added over the threads of the same channel: the
+// results land in sums[2][vc * 8]. red: T * 16 floats. A fixed order; ends with a barrier.
+__device__ void reduce_channels(const Params& p, float (&a)[8], float (&b)[8], float* red, float* sums) {
+    const int R = T / p.vc, cv = threadIdx.x % p.vc, r = threadIdx.x / p.vc;
+    int rows = R;
+    if (p.vc <= 16 && (p.vc & (p.vc - 1)) == 0) {   // a warp holds 32 / vc whole rows
+        for (int o = 16; o >= p.vc; o >>= 1)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[i] += __shfl_xor_sync(~0u, a[i], o);
+                b[i] += __shfl_xor_sync(~0u, b[i], o);
+            }
+        rows = T / 32;
+        if (threadIdx.x % 32 < p.vc)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                red[(threadIdx.x / 32 * p.vc + cv) * 16 + i] = a[i];
+                red[(threadIdx.x / 32 * p.vc + cv) * 16 + 8 + i] = b[i];
+            }
+    } else if (r < R) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            red[(r * p.vc + cv) * 16 + i] = a[i];
+            red[(r * p.vc + cv) * 16 + 8 + i] = b[i];
+        }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < p.vc * 16; c += T) {   // c: vector, then a or b, then channel
+        float s = 0.f;
+        for (int k = 0; k < rows; ++k) s += red[k * p.vc * 16 + c];
+        sums[(c % 16 / 8) * p.vc * 8 + c / 16 * 8 + c % 8] = s;
+    }
+    __syncthreads();
+}
+
+// Per-thread running statistics of 8 channels: batches of up to 4 pixels are centred on their own
+// mean and merged.
+struct Stats {
+    float mean[8], m2[8], n;
+    __device__ __forceinline__ void clear() {
+        n = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mean[i] = m2[i] = 0.f;
+    }
+    template <int B>
+    __device__ __forceinline__ void add(const float (&v)[B][8]) {
+        const float w = (float)B / (n + (float)B), k = n * w;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float s = 0.f, q = 0.f;
+#pragma unroll
+            for (int j = 0; j < B; ++j) s += v[j][i];
+            const float m = s * (1.f / B);
+#pragma unroll
+            for (int j = 0; j < B; ++j) q += (v[j][i] - m) * (v[j][i] - m);
+            const float d = m - mean[i];
+            mean[i] += d * w;
+            m2[i] += q + d * d * k;
+        }
+        n += (float)B;
+    }
+};
+// The mean and centred sum of squares of each channel over the block's pixels (count of them),
+// into sums[0][c], sums[1][c].
+__device__ void block_stats(const Params& p, const Stats& st, float count, float* red, float* sums) {
+    float a[8], b[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { a[i] = st.mean[i] * st.n; b[i] = 0.f; }
+    reduce_channels(p, a, b, red, sums);
+    const int cv = threadIdx.x % p.vc;
+    float m[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        m[i] = sums[cv * 8 + i] / count;
+        const float d = st.mean[i] - m[i];
+        a[i] = 0.f;
+        b[i] = st.n > 0.f ? st.m2[i] + st.n * d * d : 0.f;
+    }
+    __syncthreads();
+    reduce_channels(p, a, b, red, sums);
+    if (threadIdx.x < p.vc)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[threadIdx.x * 8 + i] = m[i];
+    __syncthreads();
+}
+
+// The affine map of a thread's channels: z = (x - mean) * scale + shift. Padding: all 0.
+struct Affine {
+    float mean[8], scale[8], shift[8];
+};
+template <class MeanOf, class RstdOf>
+__device__ __forceinline__ void affine_of(const Params& p, const Part& t, Affine& f, MeanOf mean_of, RstdOf rstd_of) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        f.mean[i] = f.scale[i] = f.shift[i] = 0.f;
+        if (i < t.nval) {
+            const int c = t.c0 + i, g = c / p.cpg;
+            f.mean[i] = mean_of(g);
+            f.scale[i] = rstd_of(g) * (p.gamma ? p.gamma[c] : 1.f);
+            f.shift[i] = p.beta ? p.beta[c] : 0.f;
+        }
+    }
+}
+template <int DT, int ACT>
+__device__ __forceinline__ Vec<DT> apply(const Vec<DT>& v, const Affine& f, int nval) {
+    float x[8];
+    unpack<DT>(v, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < nval ? act_fwd<ACT>(fmaf(x[i] - f.mean[i], f.scale[i], f.shift[i])) : 0.f;
+    return pack<DT>(x);
+}
+
+// ---------------------------------------------------------------- one launch, unit in a cluster
+template <int DT, int ACT>
+__global__ void __launch_bounds__(T, 2) gn_fwd_unit_kernel(const Params p) {
+    extern __shared__ uint4 sm[];
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = (int)cl.block_rank(), unit = blockIdx.x / p.cluster;
+    const int n = unit / p.nslab, slab = unit % p.nslab;
+    const Part t = part_of(p, n, slab, rank);
+    float* red = reinterpret_cast<float*>(sm + p.iters * Elem<DT>::V16 * T);
+    float* sums = red + T * 16;
+    float* group = sums + p.vc * 16;        // mean and m2 of each group over the CTA's pixels
+    float* total = group + 2 * MAX_GROUPS;  // mean and rstd over the unit
+    for (int s = 0, r = t.first; r < t.end; ++s, r += t.step) copy_in<DT>(sm, s, p.x, at(p, t, r));
+    copies_done();
+    Stats st;
+    st.clear();
+    int s = 0, r = t.first;
+    for (; r + 3 * t.step < t.end; s += 4, r += 4 * t.step) {
+        float v[4][8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) unpack<DT>(own<DT>(sm, s + j), v[j]);
+        st.add<4>(v);
+    }
+    for (; r < t.end; ++s, r += t.step) {
+        float v[1][8];
+        unpack<DT>(own<DT>(sm, s), v[0]);
+        st.add<1>(v);
+    }
+    const int c_lo = slab * p.vc * 8, g_lo = c_lo / p.cpg;
+    const int ng = max(0, min(p.C, c_lo + p.vc * 8) - c_lo) / p.cpg;     // whole groups of the slab
+    const float mine = (float)max(0, min((rank + 1) * p.rows, p.HW) - rank * p.rows);
+    block_stats(p, st, fmaxf(mine, 1.f), red, sums);
+    for (int g = threadIdx.x; g < ng; g += T) {
+        float m = 0.f, q = 0.f;
+        for (int c = 0; c < p.cpg; ++c) m += sums[g * p.cpg + c];
+        m /= (float)p.cpg;
+        for (int c = 0; c < p.cpg; ++c) {
+            const float d = sums[g * p.cpg + c] - m;
+            q += sums[p.vc * 8 + g * p.cpg + c] + mine * d * d;
+        }
+        group[2 * g] = m;
+        group[2 * g + 1] = q;
+    }
+    if (p.cluster > 1) cl.sync(); else __syncthreads();
+    for (int g = threadIdx.x; g < ng; g += T) {
+        float m = 0.f, q = 0.f;
+        for (int k = 0; k < p.cluster; ++k) {
+            const float cnt = (float)max(0, min((k + 1) * p.rows, p.HW) - k * p.rows);
+            m += cnt * cl.map_shared_rank(group, k)[2 * g];
+        }
+        m /= (float)p.HW;
+        for (int k = 0; k < p.cluster; ++k) {
+            const float cnt = (float)max(0, min((k + 1) * p.rows, p.HW) - k * p.rows);
+            const float* o = cl.map_shared_rank(group, k);
+            const float d = o[2 * g] - m;
+            q += o[2 * g + 1] + cnt * (float)p.cpg * d * d;
+        }
+        const float rs = 1.f / sqrtf(q / ((float)p.HW * (float)p.cpg) + p.eps);
+        total[2 * g] = m;
+        total[2 * g + 1] = rs;
+        if (rank == 0) {
+            if (p.mean) p.mean[(long long)n * p.G + g_lo + g] = m;
+            if (p.rstd) p.rstd[(long long)n * p.G + g_lo + g] = rs;
+        }
+    }
+    // also: no CTA of the cluster leaves while another reads its sums
+    if (p.cluster > 1) cl.sync(); else __syncthreads();
+    Affine f;
+    affine_of(p, t, f, [&](int g) { return total[2 * (g - g_lo)]; }, [&](int g) { return total[2 * (g - g_lo) + 1]; });
+    s = 0;
+    for (r = t.first; r < t.end; ++s, r += t.step)
+        store<DT>(p.out, at(p, t, r), apply<DT, ACT>(own<DT>(sm, s), f, t.nval));
+}
+
+// The backward's terms of 8 channels of one pixel: dz and xh
+struct BwdAffine {
+    float mean[8], rstd[8], gamma[8], beta[8];
+};
+__device__ __forceinline__ void bwd_affine_of(const Params& p, const Part& t, BwdAffine& f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        f.mean[i] = f.rstd[i] = f.gamma[i] = f.beta[i] = 0.f;
+        if (i < t.nval) {
+            const int c = t.c0 + i;
+            const long long g = (long long)t.n * p.G + c / p.cpg;
+            f.mean[i] = p.mean[g];
+            f.rstd[i] = p.rstd[g];
+            f.gamma[i] = p.gamma ? p.gamma[c] : 1.f;
+            f.beta[i] = p.beta ? p.beta[c] : 0.f;
+        }
+    }
+}
+template <int DT, int ACT>
+__device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy, const BwdAffine& f, float (&dz)[8],
+                                          float (&xh)[8]) {
+    unpack<DT>(vx, xh);
+    unpack<DT>(vdy, dz);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        xh[i] = (xh[i] - f.mean[i]) * f.rstd[i];
+        dz[i] = act_bwd<ACT>(dz[i], fmaf(xh[i], f.gamma[i], f.beta[i]));
+    }
+}
+template <int DT>
+__device__ __forceinline__ Vec<DT> bwd_out(const float (&dz)[8], const float (&xh)[8], const BwdAffine& f,
+                                           const float (&m1)[8], const float (&m2)[8], int nval) {
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        d[i] = i < nval ? f.rstd[i] * (fmaf(dz[i], f.gamma[i], -m1[i]) - xh[i] * m2[i]) : 0.f;
+    return pack<DT>(d);
+}
+
+// ws: per sample and channel (sum dz, sum dz xh), for gn_params_kernel
+template <int DT, int ACT>
+__global__ void __launch_bounds__(T, 2) gn_bwd_unit_kernel(const Params p) {
+    extern __shared__ uint4 sm[];
+    cg::cluster_group cl = cg::this_cluster();
+    const int rank = (int)cl.block_rank(), unit = blockIdx.x / p.cluster;
+    const int n = unit / p.nslab, slab = unit % p.nslab;
+    const Part t = part_of(p, n, slab, rank);
+    uint4* sm_dy = sm + p.iters * Elem<DT>::V16 * T;
+    float* red = reinterpret_cast<float*>(sm + 2 * p.iters * Elem<DT>::V16 * T);
+    float* sums = red + T * 16;             // the CTA's sums, read by the cluster
+    float* total = red;                     // the unit's, once red is free
+    for (int s = 0, r = t.first; r < t.end; ++s, r += t.step) {
+        copy_in<DT>(sm, s, p.x, at(p, t, r));
+        copy_in<DT>(sm_dy, s, p.dy, at(p, t, r));
+    }
+    BwdAffine f;
+    bwd_affine_of(p, t, f);
+    copies_done();
+    float a[8] = {}, b[8] = {};
+    int s = 0;
+    for (int r = t.first; r < t.end; ++s, r += t.step) {
+        float dz[8], xh[8];
+        bwd_terms<DT, ACT>(own<DT>(sm, s), own<DT>(sm_dy, s), f, dz, xh);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            a[i] += dz[i];
+            b[i] = fmaf(dz[i], xh[i], b[i]);
+        }
+    }
+    reduce_channels(p, a, b, red, sums);
+    if (p.cluster > 1) cl.sync();
+    const int c_lo = slab * p.vc * 8, nc = max(0, min(p.C - c_lo, p.vc * 8));
+    for (int c = threadIdx.x; c < p.vc * 16; c += T) {
+        float v = 0.f;
+        for (int k = 0; k < p.cluster; ++k) v += cl.map_shared_rank(sums, k)[c];
+        total[c] = v;
+        if (rank == 0 && p.ws && c % (p.vc * 8) < nc)
+            p.ws[((long long)(c / (p.vc * 8)) * p.N + n) * p.C + c_lo + c % (p.vc * 8)] = v;
+    }
+    if (p.cluster > 1) cl.sync(); else __syncthreads();
+    float* means = total + p.vc * 16;       // the groups' mean(t) and mean(t xh)
+    const float inv = 1.f / ((float)p.HW * (float)p.cpg);
+    for (int g = threadIdx.x; g < nc / p.cpg; g += T) {
+        float m1 = 0.f, m2 = 0.f;
+        for (int c = 0; c < p.cpg; ++c) {
+            const float w = p.gamma ? p.gamma[c_lo + g * p.cpg + c] : 1.f;
+            m1 = fmaf(w, total[g * p.cpg + c], m1);
+            m2 = fmaf(w, total[p.vc * 8 + g * p.cpg + c], m2);
+        }
+        means[2 * g] = m1 * inv;
+        means[2 * g + 1] = m2 * inv;
+    }
+    __syncthreads();
+    float m1[8], m2[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int g = i < t.nval ? (t.c0 + i - c_lo) / p.cpg : 0;
+        m1[i] = i < t.nval ? means[2 * g] : 0.f;
+        m2[i] = i < t.nval ? means[2 * g + 1] : 0.f;
+    }
+    s = 0;
+    for (int r = t.first; r < t.end; ++s, r += t.step) {
+        float dz[8], xh[8];
+        bwd_terms<DT, ACT>(own<DT>(sm, s), own<DT>(sm_dy, s), f, dz, xh);
+        store<DT>(p.out, at(p, t, r), bwd_out<DT>(dz, xh, f, m1, m2, t.nval));
+    }
+}
+
+// dgamma and dbeta: the samples' sums, in order
+__global__ void gn_params_kernel(const float* ws, float* dgamma, float* dbeta, int N, int C) {
+    const int c = blockIdx.x * blockDim.x + threadIdx.x;
+    if (c >= 2 * C) return;
+    const bool second = c >= C;
+    const float* s = ws + (second ? (long long)N * C : 0) + c % C;
+    float v = 0.f;
+#pragma unroll 8
+    for (int n = 0; n < N; ++n) v += s[(long long)n * C];
+    float* d = second ? dgamma : dbeta;
+    if (d) d[c % C] = v;
+}
+
+// ---------------------------------------------------------------- three launches
+// Grid (chunk, slab, sample). Partials at ws[sample][value][chunk][channel], value 0 and 1: mean
+// and centred sum of squares (forward), sum dz and sum dz xh (backward).
+__device__ __forceinline__ long long partial_at(const Params& p, int n, int value, int chunk, int c) {
+    return (((long long)n * 2 + value) * p.nchunk + chunk) * p.Cs + c;
+}
+template <int DT, int ACT, bool BWD>
+__global__ void __launch_bounds__(T) gn_partial_kernel(const Params p) {
+    extern __shared__ uint4 sm[];
+    float* red = reinterpret_cast<float*>(sm);
+    float* sums = red + T * 16;
+    const Part t = part_of(p, blockIdx.z, blockIdx.y, blockIdx.x);
+    if constexpr (BWD) {
+        BwdAffine f;
+        bwd_affine_of(p, t, f);
+        float a[8] = {}, b[8] = {};
+#pragma unroll 4
+        for (int r = t.first; r < t.end; r += t.step) {
+            float dz[8], xh[8];
+            bwd_terms<DT, ACT>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, dz, xh);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[i] += dz[i];
+                b[i] = fmaf(dz[i], xh[i], b[i]);
+            }
+        }
+        reduce_channels(p, a, b, red, sums);
+    } else {
+        Stats st;
+        st.clear();
+        int r = t.first;
+        for (; r + 3 * t.step < t.end; r += 4 * t.step) {
+            Vec<DT> q[4];
+            float v[4][8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q[j] = load<DT>(p.x, at(p, t, r + j * t.step));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) unpack<DT>(q[j], v[j]);
+            st.add<4>(v);
+        }
+        for (; r < t.end; r += t.step) {
+            float v[1][8];
+            unpack<DT>(load<DT>(p.x, at(p, t, r)), v[0]);
+            st.add<1>(v);
+        }
+        block_stats(p, st, (float)(min((int)(blockIdx.x + 1) * p.rows, p.HW) - (int)blockIdx.x * p.rows), red, sums);
+    }
+    const int c_lo = blockIdx.y * p.vc * 8;
+    for (int c = threadIdx.x; c < p.vc * 8; c += T)
+        if (c_lo + c < p.Cs) {
+            p.ws[partial_at(p, t.n, 0, blockIdx.x, c_lo + c)] = sums[c];
+            p.ws[partial_at(p, t.n, 1, blockIdx.x, c_lo + c)] = sums[p.vc * 8 + c];
+        }
+}
+
 __device__ float block_sum(float v, float* sh) {
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
     __syncthreads();
     if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = v;
     __syncthreads();
     v = 0.f;
-    for (int w = 0; w < (int)blockDim.x / 32; ++w) v += sh[w];
+    for (int w = 0; w < T / 32; ++w) v += sh[w];
     return v;
 }
-
-// One block per (sample, group); group G stands for the stored channels past C, which become 0.
-template <int DT>
-__global__ void gn_fwd_kernel(const Params p) {
-    using T = typename Elem<DT>::T;
-    __shared__ float sh[32];
-    const int n = blockIdx.x / (p.G + 1), g = blockIdx.x % (p.G + 1);
-    const T* x = static_cast<const T*>(p.x) + (long long)n * p.HW * p.Cs;
-    T* y = static_cast<T*>(p.out) + (long long)n * p.HW * p.Cs;
-    if (g == p.G) {
-        const int pad = p.Cs - p.C;
-        for (long long i = threadIdx.x; i < (long long)p.HW * pad; i += blockDim.x)
-            y[i / pad * p.Cs + p.C + i % pad] = T(0.f);
-        return;
-    }
-    const int cpg = p.C / p.G, c0 = g * cpg;
-    const long long M = (long long)p.HW * cpg;
-    float s = 0.f;
-    for (long long i = threadIdx.x; i < M; i += blockDim.x)
-        s += to_f(x[i / cpg * p.Cs + c0 + i % cpg]);
-    const float mean = block_sum(s, sh) / (float)M;
-    s = 0.f;
-    for (long long i = threadIdx.x; i < M; i += blockDim.x) {
-        const float d = to_f(x[i / cpg * p.Cs + c0 + i % cpg]) - mean;
-        s += d * d;
-    }
-    const float rstd = rsqrtf(block_sum(s, sh) / (float)M + p.eps);
-    if (threadIdx.x == 0) {
-        if (p.mean) p.mean[n * p.G + g] = mean;
-        if (p.rstd) p.rstd[n * p.G + g] = rstd;
-    }
-    for (long long i = threadIdx.x; i < M; i += blockDim.x) {
-        const int c = c0 + (int)(i % cpg);
-        const long long at = i / cpg * p.Cs + c;
-        const float xh = (to_f(x[at]) - mean) * rstd;
-        from_f(act_fwd(xh * (p.gamma ? p.gamma[c] : 1.f) + (p.beta ? p.beta[c] : 0.f), p.act), y[at]);
-    }
-}
-
-template <int DT>
-__device__ __forceinline__ void bwd_point(const Params& p, long long at, int c, float mean,
-                                          float rstd, float& dz, float& xh) {
-    using T = typename Elem<DT>::T;
-    xh = (to_f(static_cast<const T*>(p.x)[at]) - mean) * rstd;
-    const float z = xh * (p.gamma ? p.gamma[c] : 1.f) + (p.beta ? p.beta[c] : 0.f);
-    dz = act_bwd(to_f(static_cast<const T*>(p.dy)[at]), z, p.act);
-}
-
-// Per channel: dgamma and dbeta over samples and pixels.
-template <int DT>
-__global__ void gn_bwd_params_kernel(const Params p) {
-    __shared__ float sh[32];
-    const int c = blockIdx.x, g = c / (p.C / p.G);
+// One block per (group, sample): the chunks' and channels' statistics -> stat[sample][group]:
+// forward mean and rstd, backward mean(t) and mean(t xh), with the samples' channel sums for
+// gn_params_kernel in chan[value][sample][channel].
+template <bool BWD>
+__global__ void __launch_bounds__(T) gn_combine_kernel(const Params p, float* stat, float* chan) {
+    __shared__ float sh[T / 32];
+    const int g = blockIdx.x, n = blockIdx.y, c0 = g * p.cpg;
+    const long long M = (long long)p.nchunk * p.cpg;
     float a = 0.f, b = 0.f;
-    for (long long i = threadIdx.x; i < (long long)p.N * p.HW; i += blockDim.x) {
-        const int n = (int)(i / p.HW);
-        float dz, xh;
-        bwd_point<DT>(p, i * p.Cs + c, c, p.mean[n * p.G + g], p.rstd[n * p.G + g], dz, xh);
-        a += dz * xh;
-        b += dz;
+    if constexpr (BWD) {
+        // a thread per channel, so that the channel's sums come out whole
+        for (int c = threadIdx.x; c < p.cpg; c += T) {
+            float sa = 0.f, sb = 0.f;
+            for (int k = 0; k < p.nchunk; ++k) {
+                sa += p.ws[partial_at(p, n, 0, k, c0 + c)];
+                sb += p.ws[partial_at(p, n, 1, k, c0 + c)];
+            }
+            chan[(long long)n * p.C + c0 + c] = sa;
+            chan[((long long)p.N + n) * p.C + c0 + c] = sb;
+            const float w = p.gamma ? p.gamma[c0 + c] : 1.f;
+            a = fmaf(w, sa, a);
+            b = fmaf(w, sb, b);
+        }
+        a = block_sum(a, sh);
+        b = block_sum(b, sh);
+        if (threadIdx.x == 0) {
+            const float inv = 1.f / ((float)p.HW * (float)p.cpg);
+            stat[2 * ((long long)n * p.G + g)] = a * inv;
+            stat[2 * ((long long)n * p.G + g) + 1] = b * inv;
+        }
+    } else {
+        for (long long i = threadIdx.x; i < M; i += T) {
+            const int k = (int)(i / p.cpg), c = (int)(i % p.cpg);
+            a += (float)(min((k + 1) * p.rows, p.HW) - k * p.rows) * p.ws[partial_at(p, n, 0, k, c0 + c)];
+        }
+        const float total = (float)p.HW * (float)p.cpg, m = block_sum(a, sh) / total;
+        for (long long i = threadIdx.x; i < M; i += T) {
+            const int k = (int)(i / p.cpg), c = (int)(i % p.cpg);
+            const float d = p.ws[partial_at(p, n, 0, k, c0 + c)] - m;
+            b += p.ws[partial_at(p, n, 1, k, c0 + c)] +
+                 (float)(min((k + 1) * p.rows, p.HW) - k * p.rows) * d * d;
+        }
+        b = block_sum(b, sh);
+        if (threadIdx.x == 0) {
+            const float rs = 1.f / sqrtf(b / total + p.eps);
+            const long long o = (long long)n * p.G + g;
+            stat[2 * o] = m;
+            stat[2 * o + 1] = rs;
+            if (p.mean) p.mean[o] = m;
+            if (p.rstd) p.rstd[o] = rs;
+        }
     }
-    a = block_sum(a, sh);
-    b = block_sum(b, sh);
-    if (threadIdx.x == 0) {
-        if (p.dgamma) p.dgamma[c] = a;
-        if (p.dbeta) p.dbeta[c] = b;
+}
+// The last chunks first: they are the ones that the partial pass left in L2.
+template <int DT, int ACT, bool BWD>
+__global__ void __launch_bounds__(T) gn_apply_kernel(const Params p, const float* stat) {
+    const Part t = part_of(p, gridDim.z - 1 - blockIdx.z, gridDim.y - 1 - blockIdx.y, gridDim.x - 1 - blockIdx.x);
+    const float* s = stat + 2 * (long long)t.n * p.G;
+    if constexpr (BWD) {
+        BwdAffine f;
+        bwd_affine_of(p, t, f);
+        float m1[8], m2[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int g = i < t.nval ? (t.c0 + i) / p.cpg : 0;
+            m1[i] = i < t.nval ? s[2 * g] : 0.f;
+            m2[i] = i < t.nval ? s[2 * g + 1] : 0.f;
+        }
+#pragma unroll 4
+        for (int r = t.first; r < t.end; r += t.step) {
+            float dz[8], xh[8];
+            bwd_terms<DT, ACT>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, dz, xh);
+            store<DT>(p.out, at(p, t, r), bwd_out<DT>(dz, xh, f, m1, m2, t.nval));
+        }
+    } else {
+        Affine f;
+        affine_of(p, t, f, [&](int g) { return s[2 * g]; }, [&](int g) { return s[2 * g + 1]; });
+#pragma unroll 4
+        for (int r = t.first; r < t.end; r += t.step)
+            store<DT>(p.out, at(p, t, r), apply<DT, ACT>(load<DT>(p.x, at(p, t, r)), f, t.nval));
     }
 }
 
-template <int DT>
-__global__ void gn_bwd_kernel(const Params p) {
-    using T = typename Elem<DT>::T;
-    __shared__ float sh[32];
-    const int n = blockIdx.x / (p.G + 1), g = blockIdx.x % (p.G + 1);
-    const long long base = (long long)n * p.HW * p.Cs;
-    T* dx = static_cast<T*>(p.out);
-    if (g == p.G) {
-        const int pad = p.Cs - p.C;
-        for (long long i = threadIdx.x; i < (long long)p.HW * pad; i += blockDim.x)
-            dx[base + i / pad * p.Cs + p.C + i % pad] = T(0.f);
-        return;
-    }
-    const int cpg = p.C / p.G, c0 = g * cpg;
-    const long long M = (long long)p.HW * cpg;
-    const float mean = p.mean[n * p.G + g], rstd = p.rstd[n * p.G + g];
-    float a = 0.f, b = 0.f;
-    for (long long i = threadIdx.x; i < M; i += blockDim.x) {
-        const int c = c0 + (int)(i % cpg);
-        float dz, xh;
-        bwd_point<DT>(p, base + i / cpg * p.Cs + c, c, mean, rstd, dz, xh);
-        const float t = dz * (p.gamma ? p.gamma[c] : 1.f);
-        a += t;
-        b += t * xh;
-    }
-    a = block_sum(a, sh) / (float)M;
-    b = block_sum(b, sh) / (float)M;
-    for (long long i = threadIdx.x; i < M; i += blockDim.x) {
-        const int c = c0 + (int)(i % cpg);
-        const long long at = base + i / cpg * p.Cs + c;
-        float dz, xh;
-        bwd_point<DT>(p, at, c, mean, rstd, dz, xh);
-        from_f(rstd * (dz * (p.gamma ? p.gamma[c] : 1.f) - a - xh * b), dx[at]);
-    }
-}
-
+// ---------------------------------------------------------------- host
 static int check_shape(int nN, int nHW, int nC, int nCs, int nGroups, int nDtype) {
     if (nN < 0 || nHW <= 0 || nC <= 0 || nCs < nC || nCs % 8 || nGroups <= 0 || nC % nGroups)
         return OM_ERR_INVALID;
     if (nDtype != OM_DTYPE_F32 && nDtype != OM_DTYPE_BF16 && nDtype != OM_DTYPE_F16)
         return OM_ERR_UNSUPPORTED;
+    if (nHW > (1 << 30)) return OM_ERR_UNSUPPORTED;
     return OM_OK;
 }
 static bool aligned(const void* p, int a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// Fills in the split of the work: p->cluster > 0 for the one-launch form with `smem` bytes,
+// 0 for the three-launch form.
+static void plan(Params* p, int dtype, bool bwd, size_t* smem) {
+    const int size = dtype == OM_DTYPE_F32 ? 4 : 2;
+    p->cpg = p->C / p->G;
+    // whole groups in whole vectors, 64 bytes of a pixel where the channels give as many
+    long long unit = p->cpg;
+    int gcd = 8;
+    while (unit % gcd) gcd /= 2;
+    unit *= 8 / gcd;
+    long long slab = unit;
+    while (slab * size < 64 && slab < p->C) slab += unit;
+    if (slab >= p->C) slab = p->Cs;
+    const int per_vec = 8 * size * (bwd ? 2 : 1);        // bytes kept for a vector
+    p->cluster = 0;
+    if (slab / 8 <= MAX_VC) {
+        p->vc = (int)(slab / 8);
+        p->nslab = (int)((p->Cs + slab - 1) / slab);
+        const int step = T / p->vc;
+        const size_t fixed = (size_t)T * 16 * 4 + (size_t)p->vc * 16 * 4 + (bwd ? 0 : 4 * MAX_GROUPS * 4);
+        for (int k = 1; k <= MAX_CLUSTER; k *= 2) {
+            const int rows = (p->HW + k - 1) / k, iters = (rows + step - 1) / step;
+            const size_t need = (size_t)iters * T * per_vec + fixed;
+            if (need > SMEM_MAX) continue;
+            p->cluster = k; p->rows = rows; p->iters = iters; *smem = need;
+            // enough parts to fill the GPU, with two CTAs on an SM
+            if ((long long)p->N * p->nslab * k >= 2 * 148 && need <= SMEM_MAX / 2 - 1024) break;
+            if (iters <= 4) break;
+        }
+    }
+    if (p->cluster) return;
+    p->vc = p->Cs / 8 < MAX_VC ? p->Cs / 8 : MAX_VC;
+    p->nslab = (p->Cs / 8 + p->vc - 1) / p->vc;
+    const int step = T / p->vc;
+    int iters = 16;
+    while (iters < 256 && (long long)p->N * p->nslab * ((p->HW + step * iters - 1) / (step * iters)) > 148 * 16) iters *= 2;
+    p->rows = step * iters;
+    p->iters = iters;
+    p->nchunk = (p->HW + p->rows - 1) / p->rows;
+    *smem = (size_t)T * 16 * 4 + (size_t)p->vc * 16 * 4;
+}
+static long long ws_floats(const Params& p, bool bwd) {
+    const long long chan = bwd ? 2LL * p.N * p.C : 0;
+    if (p.cluster) return chan;
+    return chan + 2LL * p.N * p.G + 2LL * p.N * p.nchunk * p.Cs;
+}
+
+template <int DT, int ACT, bool BWD>
+static int launch(DeviceCtx* c, Params p, size_t smem) {
+    static bool attr_set[64] = {false};
+    if (p.cluster) {
+        auto kern = BWD ? gn_bwd_unit_kernel<DT, ACT> : gn_fwd_unit_kernel<DT, ACT>;
+        if (!attr_set[c->device]) {
+            OMB_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
+            attr_set[c->device] = true;
+        }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)((long long)p.N * p.nslab * p.cluster));
+        cfg.blockDim = dim3(T);
+        cfg.dynamicSmemBytes = smem;
+        cfg.stream = c->compute;
+        cudaLaunchAttribute a[1];
+        a[0].id = cudaLaunchAttributeClusterDimension;
+        a[0].val.clusterDim.x = p.cluster;
+        a[0].val.clusterDim.y = a[0].val.clusterDim.z = 1;
+        cfg.attrs = a;
+        cfg.numAttrs = 1;
+        OMB_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+        if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
+    } else {
+        float* chan = p.ws;
+        float* stat = chan + (BWD ? 2LL * p.N * p.C : 0);
+        p.ws = stat + 2LL * p.N * p.G;
+        const dim3 grid(p.nchunk, p.nslab, p.N);
+        gn_partial_kernel<DT, ACT, BWD><<<grid, T, smem, c->compute>>>(p);
+        if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
+        gn_combine_kernel<BWD><<<dim3(p.G, p.N), T, 0, c->compute>>>(p, stat, chan);
+        if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
+        gn_apply_kernel<DT, ACT, BWD><<<grid, T, 0, c->compute>>>(p, stat);
+        if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
+        p.ws = chan;
+    }
+    if (BWD && (p.dgamma || p.dbeta)) {
+        gn_params_kernel<<<(2 * p.C + 127) / 128, 128, 0, c->compute>>>(p.ws, p.dgamma, p.dbeta, p.N, p.C);
+        return after_launch(c);
+    }
+    return OM_OK;
+}
+template <int DT, bool BWD>
+static int launch_act(DeviceCtx* c, const Params& p, size_t smem, int act) {
+    switch (act) {
+        case OM_ACT_NONE: return launch<DT, OM_ACT_NONE, BWD>(c, p, smem);
+        case OM_ACT_RELU: return launch<DT, OM_ACT_RELU, BWD>(c, p, smem);
+        case OM_ACT_RELU6: return launch<DT, OM_ACT_RELU6, BWD>(c, p, smem);
+        default: return launch<DT, OM_ACT_SILU, BWD>(c, p, smem);
+    }
+}
+template <bool BWD>
+static int dispatch(DeviceCtx* c, Params p, int act, int dtype) {
+    size_t smem = 0;
+    plan(&p, dtype, BWD, &smem);
+    if (ws_floats(p, BWD) > 0 && (!p.ws || !aligned(p.ws, 16))) return OM_ERR_INVALID;
+    if (p.cluster ? (long long)p.N * p.nslab * p.cluster > 0x7FFFFFFF : p.N > 65535)
+        return OM_ERR_UNSUPPORTED;      // the grid's limits
+    if (dtype == OM_DTYPE_F32) return launch_act<OM_DTYPE_F32, BWD>(c, p, smem, act);
+    if (dtype == OM_DTYPE_BF16) return launch_act<OM_DTYPE_BF16, BWD>(c, p, smem, act);
+    return launch_act<OM_DTYPE_F16, BWD>(c, p, smem, act);
+}
 
 }  // namespace gn
 }  // namespace omb
@@ -173,7 +744,12 @@ using namespace omb;
 extern "C" long long omCudaGroupNormNhwcWorkspaceBytes(int nN, int nHW, int nC, int nCs,
                                                        int nGroups, int nDtype, int bBackward) {
     const int st = gn::check_shape(nN, nHW, nC, nCs, nGroups, nDtype);
-    return st != OM_OK ? st : 0;
+    if (st != OM_OK) return st;
+    gn::Params p = {};
+    p.N = nN; p.HW = nHW; p.C = nC; p.Cs = nCs; p.G = nGroups;
+    size_t smem;
+    gn::plan(&p, nDtype, bBackward != 0, &smem);
+    return gn::ws_floats(p, bBackward != 0) * 4;
 }
 
 extern "C" int omCudaGroupNormActNhwc(const void* pIn, void* pOut, const float* pGamma,
@@ -188,15 +764,9 @@ extern "C" int omCudaGroupNormActNhwc(const void* pIn, void* pOut, const float* 
     if (!pIn || !pOut || !gn::aligned(pIn, 16) || !gn::aligned(pOut, 16)) return OM_ERR_INVALID;
     gn::Params p = {};
     p.x = pIn; p.out = pOut; p.gamma = pGamma; p.beta = pBeta; p.mean = pMean; p.rstd = pInvStd;
-    p.N = nN; p.HW = nHW; p.C = nC; p.Cs = nCs; p.G = nGroups; p.act = nAct; p.eps = fEps;
-    const int grid = nN * (nGroups + 1);
-    if (nDtype == OM_DTYPE_F32)
-        gn::gn_fwd_kernel<OM_DTYPE_F32><<<grid, 256, 0, c->compute>>>(p);
-    else if (nDtype == OM_DTYPE_BF16)
-        gn::gn_fwd_kernel<OM_DTYPE_BF16><<<grid, 256, 0, c->compute>>>(p);
-    else
-        gn::gn_fwd_kernel<OM_DTYPE_F16><<<grid, 256, 0, c->compute>>>(p);
-    return after_launch(c);
+    p.ws = static_cast<float*>(pWorkspace);
+    p.N = nN; p.HW = nHW; p.C = nC; p.Cs = nCs; p.G = nGroups; p.eps = fEps;
+    return gn::dispatch<false>(c, p, nAct, nDtype);
 }
 
 extern "C" int omCudaGroupNormActNhwcBackward(const void* pGradOut, const void* pIn,
@@ -221,22 +791,7 @@ extern "C" int omCudaGroupNormActNhwcBackward(const void* pGradOut, const void* 
     p.x = pIn; p.dy = pGradOut; p.out = pGradIn; p.gamma = pGamma; p.beta = pBeta;
     p.mean = const_cast<float*>(pMean); p.rstd = const_cast<float*>(pInvStd);
     p.dgamma = pGradGamma; p.dbeta = pGradBeta;
-    p.N = nN; p.HW = nHW; p.C = nC; p.Cs = nCs; p.G = nGroups; p.act = nAct;
-    const int grid = nN * (nGroups + 1);
-    if (pGradGamma || pGradBeta) {  // before dX, which may overwrite dY
-        if (nDtype == OM_DTYPE_F32)
-            gn::gn_bwd_params_kernel<OM_DTYPE_F32><<<nC, 256, 0, c->compute>>>(p);
-        else if (nDtype == OM_DTYPE_BF16)
-            gn::gn_bwd_params_kernel<OM_DTYPE_BF16><<<nC, 256, 0, c->compute>>>(p);
-        else
-            gn::gn_bwd_params_kernel<OM_DTYPE_F16><<<nC, 256, 0, c->compute>>>(p);
-        if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
-    }
-    if (nDtype == OM_DTYPE_F32)
-        gn::gn_bwd_kernel<OM_DTYPE_F32><<<grid, 256, 0, c->compute>>>(p);
-    else if (nDtype == OM_DTYPE_BF16)
-        gn::gn_bwd_kernel<OM_DTYPE_BF16><<<grid, 256, 0, c->compute>>>(p);
-    else
-        gn::gn_bwd_kernel<OM_DTYPE_F16><<<grid, 256, 0, c->compute>>>(p);
-    return after_launch(c);
+    p.ws = static_cast<float*>(pWorkspace);
+    p.N = nN; p.HW = nHW; p.C = nC; p.Cs = nCs; p.G = nGroups;
+    return gn::dispatch<true>(c, p, nAct, nDtype);
 }
