@@ -27,6 +27,7 @@ constexpr int T = 256;                    // threads of every block
 constexpr int MAX_VC = 256;               // 8-channel vectors of a pixel that one block covers
 constexpr int MAX_CLUSTER = 8;
 constexpr int SMEM_MAX = 227 * 1024;
+constexpr int KEEP_MAX = SMEM_MAX / 2 - 1024, KEEP_GOOD = SMEM_MAX / 4 - 1024;
 constexpr int MAX_GROUPS = 40;            // of a slab: it ends with the first unit of lcm(cpg, 8)
                                           // channels that reaches 32, so below 32 / cpg + 8
 
@@ -99,21 +100,24 @@ __device__ __forceinline__ Vec<DT> own(const uint4* sm, int s) {
     for (int i = 0; i < Elem<DT>::V16; ++i) v.q[i] = sm[(s * Elem<DT>::V16 + i) * T + threadIdx.x];
     return v;
 }
-__device__ __forceinline__ void copies_done() {
-    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+// sigmoid(z) = 1 / (1 + 2^(-z log2 e)): an overflowing power gives 0
+__device__ __forceinline__ float sigmoid(float z) {
+    float e, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+    return s;
 }
-
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
-    if (ACT == OM_ACT_SILU) return __fdividef(z, 1.f + __expf(fminf(-z, 80.f)));
+    if (ACT == OM_ACT_SILU) return z * sigmoid(z);
     return apply_act(z, ACT);
 }
 // dz = dy * act'(z)
 template <int ACT>
 __device__ __forceinline__ float act_bwd(float dy, float z) {
     if (ACT == OM_ACT_SILU) {
-        const float s = __fdividef(1.f, 1.f + __expf(fminf(-z, 80.f)));
-        return dy * (s * (1.f + z * (1.f - s)));
+        const float s = sigmoid(z);
+        return dy * s * fmaf(z, 1.f - s, 1.f);
     }
     if (ACT == OM_ACT_RELU) return z > 0.f ? dy : 0.f;
     if (ACT == OM_ACT_RELU6) return z > 0.f && z < 6.f ? dy : 0.f;
@@ -162,157 +166,194 @@ __device__ __forceinline__ long long at(const Params& p, const Part& t, int pixe
     return t.base + (long long)pixel * p.Cs;
 }
 
-// Two per-channel values of every thread, added over the threads of the same channel: the
-// results land in sums[2][vc * 8]. red: T * 16 floats. A fixed order; ends with a barrier.
-__device__ void reduce_channels(const Params& p, float (&a)[8], float (&b)[8], float* red, float* sums) {
+// NV pairs of values of every thread, added over the threads of the same vector column: the
+// results land in sums[2][vc * NV]. red: T * 2 * NV floats. A fixed order; ends with a barrier.
+template <int NV>
+__device__ void reduce_columns(const Params& p, float (&a)[NV], float (&b)[NV], float* red, float* sums) {
     const int R = T / p.vc, cv = threadIdx.x % p.vc, r = threadIdx.x / p.vc;
-    int rows = R;
+    int rows = R, slot = threadIdx.x;
+    bool write = r < R;
     if (p.vc <= 16 && (p.vc & (p.vc - 1)) == 0) {   // a warp holds 32 / vc whole rows
         for (int o = 16; o >= p.vc; o >>= 1)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
+            for (int i = 0; i < NV; ++i) {
                 a[i] += __shfl_xor_sync(~0u, a[i], o);
                 b[i] += __shfl_xor_sync(~0u, b[i], o);
             }
         rows = T / 32;
-        if (threadIdx.x % 32 < p.vc)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                red[(threadIdx.x / 32 * p.vc + cv) * 16 + i] = a[i];
-                red[(threadIdx.x / 32 * p.vc + cv) * 16 + 8 + i] = b[i];
-            }
-    } else if (r < R) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            red[(r * p.vc + cv) * 16 + i] = a[i];
-            red[(r * p.vc + cv) * 16 + 8 + i] = b[i];
-        }
+        slot = threadIdx.x / 32 * p.vc + cv;
+        write = threadIdx.x % 32 < p.vc;
     }
+    if (write)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            red[slot * 2 * NV + i] = a[i];
+            red[slot * 2 * NV + NV + i] = b[i];
+        }
     __syncthreads();
-    for (int c = threadIdx.x; c < p.vc * 16; c += T) {   // c: vector, then a or b, then channel
+    for (int c = threadIdx.x; c < p.vc * 2 * NV; c += T) {   // c: vector, then a or b, then value
         float s = 0.f;
-        for (int k = 0; k < rows; ++k) s += red[k * p.vc * 16 + c];
-        sums[(c % 16 / 8) * p.vc * 8 + c / 16 * 8 + c % 8] = s;
+        for (int k = 0; k < rows; ++k) s += red[k * p.vc * 2 * NV + c];
+        sums[c % (2 * NV) / NV * p.vc * NV + c / (2 * NV) * NV + c % NV] = s;
     }
     __syncthreads();
 }
 
-// Per-thread running statistics of 8 channels: batches of up to 4 pixels are centred on their own
-// mean and merged.
+// Per-thread running statistics of the GV entries of a vector, 8 / GV channels each: batches of B
+// pixels are centred on their own mean and merged.
+template <int GV>
 struct Stats {
-    float mean[8], m2[8], n;
+    float mean[GV], m2[GV], n;
     __device__ __forceinline__ void clear() {
         n = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mean[i] = m2[i] = 0.f;
+        for (int g = 0; g < GV; ++g) mean[g] = m2[g] = 0.f;
     }
     template <int B>
     __device__ __forceinline__ void add(const float (&v)[B][8]) {
-        const float w = (float)B / (n + (float)B), k = n * w;
+        constexpr int PER = 8 / GV;
+        constexpr float cnt = B * PER;
+        const float w = __fdividef(cnt, n + cnt), k = n * w;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int g = 0; g < GV; ++g) {
             float s = 0.f, q = 0.f;
 #pragma unroll
-            for (int j = 0; j < B; ++j) s += v[j][i];
-            const float m = s * (1.f / B);
+            for (int j = 0; j < B; ++j)
 #pragma unroll
-            for (int j = 0; j < B; ++j) q += (v[j][i] - m) * (v[j][i] - m);
-            const float d = m - mean[i];
-            mean[i] += d * w;
-            m2[i] += q + d * d * k;
+                for (int i = 0; i < PER; ++i) s += v[j][g * PER + i];
+            const float m = s * (1.f / cnt);
+#pragma unroll
+            for (int j = 0; j < B; ++j)
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    const float e = v[j][g * PER + i] - m;
+                    q = fmaf(e, e, q);
+                }
+            const float d = m - mean[g];
+            mean[g] = fmaf(d, w, mean[g]);
+            m2[g] += fmaf(d * d, k, q);
         }
-        n += (float)B;
+        n += cnt;
     }
 };
-// The mean and centred sum of squares of each channel over the block's pixels (count of them),
-// into sums[0][c], sums[1][c].
-__device__ void block_stats(const Params& p, const Stats& st, float count, float* red, float* sums) {
-    float a[8], b[8];
+// The mean and centred sum of squares of each entry over the block's pixels (count values of an
+// entry), into sums[0][e], sums[1][e].
+template <int GV>
+__device__ void block_stats(const Params& p, const Stats<GV>& st, float count, float* red, float* sums) {
+    float a[GV], b[GV], m[GV];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) { a[i] = st.mean[i] * st.n; b[i] = 0.f; }
-    reduce_channels(p, a, b, red, sums);
+    for (int i = 0; i < GV; ++i) { a[i] = st.mean[i] * st.n; b[i] = 0.f; }
+    reduce_columns<GV>(p, a, b, red, sums);
     const int cv = threadIdx.x % p.vc;
-    float m[8];
+    const float inv = 1.f / count;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        m[i] = sums[cv * 8 + i] / count;
+    for (int i = 0; i < GV; ++i) {
+        m[i] = sums[cv * GV + i] * inv;
         const float d = st.mean[i] - m[i];
         a[i] = 0.f;
-        b[i] = st.n > 0.f ? st.m2[i] + st.n * d * d : 0.f;
+        b[i] = st.n > 0.f ? fmaf(st.n * d, d, st.m2[i]) : 0.f;
     }
     __syncthreads();
-    reduce_channels(p, a, b, red, sums);
+    reduce_columns<GV>(p, a, b, red, sums);
     if (threadIdx.x < p.vc)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[threadIdx.x * 8 + i] = m[i];
+        for (int i = 0; i < GV; ++i) sums[threadIdx.x * GV + i] = m[i];
     __syncthreads();
 }
 
-// The affine map of a thread's channels: z = (x - mean) * scale + shift. Padding: all 0.
+// z = (x - mean) scale + shift of a thread's 8 channels; with 16-bit inputs the mean is folded
+// into the shift (its rounding, 2^-24 of mean * scale, is far below the output's). Padding: 0.
+template <int DT>
 struct Affine {
-    float mean[8], scale[8], shift[8];
+    float mean[DT == OM_DTYPE_F32 ? 8 : 1], scale[8], shift[8];
 };
-template <class MeanOf, class RstdOf>
-__device__ __forceinline__ void affine_of(const Params& p, const Part& t, Affine& f, MeanOf mean_of, RstdOf rstd_of) {
+template <int DT, class MeanOf, class RstdOf>
+__device__ __forceinline__ void affine_of(const Params& p, const Part& t, Affine<DT>& f, MeanOf mean_of, RstdOf rstd_of) {
+    int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);     // group of the channel, channels left in it
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        f.mean[i] = f.scale[i] = f.shift[i] = 0.f;
+        float m = 0.f;
+        f.scale[i] = f.shift[i] = 0.f;
         if (i < t.nval) {
-            const int c = t.c0 + i, g = c / p.cpg;
-            f.mean[i] = mean_of(g);
+            const int c = t.c0 + i;
+            m = mean_of(g);
             f.scale[i] = rstd_of(g) * (p.gamma ? p.gamma[c] : 1.f);
             f.shift[i] = p.beta ? p.beta[c] : 0.f;
+            if (DT != OM_DTYPE_F32) f.shift[i] = fmaf(-m, f.scale[i], f.shift[i]);
         }
+        if (DT == OM_DTYPE_F32) f.mean[i] = m;
+        if (--left == 0) { ++g; left = p.cpg; }
     }
 }
 template <int DT, int ACT>
-__device__ __forceinline__ Vec<DT> apply(const Vec<DT>& v, const Affine& f, int nval) {
+__device__ __forceinline__ Vec<DT> apply(const Vec<DT>& v, const Affine<DT>& f, int nval) {
     float x[8];
     unpack<DT>(v, x);
+    if (nval < 8)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = i < nval ? act_fwd<ACT>(fmaf(x[i] - f.mean[i], f.scale[i], f.shift[i])) : 0.f;
+        for (int i = 0; i < 8; ++i) x[i] = i < nval ? x[i] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = act_fwd<ACT>(fmaf(DT == OM_DTYPE_F32 ? x[i] - f.mean[i] : x[i], f.scale[i], f.shift[i]));
     return pack<DT>(x);
 }
 
 // ---------------------------------------------------------------- one launch, unit in a cluster
-template <int DT, int ACT>
-__global__ void __launch_bounds__(T, 2) gn_fwd_unit_kernel(const Params p) {
+// GV: entries of a vector whose statistics are kept apart: 1 where a vector lies within a group
+// (channels per group a multiple of 8), 2 with 4 channels a group, else 8.
+template <int DT, int ACT, int GV>
+__global__ void __launch_bounds__(T, 4) gn_fwd_unit_kernel(const Params p) {
     extern __shared__ uint4 sm[];
     cg::cluster_group cl = cg::this_cluster();
     const int rank = (int)cl.block_rank(), unit = blockIdx.x / p.cluster;
-    const int n = unit / p.nslab, slab = unit % p.nslab;
+    const int n = unit / p.nslab, slab = unit - n * p.nslab;
     const Part t = part_of(p, n, slab, rank);
     float* red = reinterpret_cast<float*>(sm + p.iters * Elem<DT>::V16 * T);
-    float* sums = red + T * 16;
-    float* group = sums + p.vc * 16;        // mean and m2 of each group over the CTA's pixels
+    float* sums = red + T * 2 * GV;
+    float* group = sums + p.vc * 2 * GV;        // mean and m2 of each group over the CTA's pixels
     float* total = group + 2 * MAX_GROUPS;  // mean and rstd over the unit
-    for (int s = 0, r = t.first; r < t.end; ++s, r += t.step) copy_in<DT>(sm, s, p.x, at(p, t, r));
-    copies_done();
-    Stats st;
+    const long long step = (long long)t.step * p.Cs;
+    const int mine_rows = t.first < t.end ? (t.end - t.first + t.step - 1) / t.step : 0;
+    const int half = mine_rows / 2 & ~3;    // statistics of the first half while the second arrives
+    {
+        long long e = at(p, t, t.first);
+        for (int s = 0; s < half; ++s, e += step) copy_in<DT>(sm, s, p.x, e);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        for (int s = half; s < mine_rows; ++s, e += step) copy_in<DT>(sm, s, p.x, e);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    Stats<GV> st;
     st.clear();
-    int s = 0, r = t.first;
-    for (; r + 3 * t.step < t.end; s += 4, r += 4 * t.step) {
-        float v[4][8];
+    auto take = [&](int s, int end) {
+        for (; s + 3 < end; s += 4) {
+            float v[4][8];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) unpack<DT>(own<DT>(sm, s + j), v[j]);
-        st.add<4>(v);
-    }
-    for (; r < t.end; ++s, r += t.step) {
-        float v[1][8];
-        unpack<DT>(own<DT>(sm, s), v[0]);
-        st.add<1>(v);
-    }
+            for (int j = 0; j < 4; ++j) unpack<DT>(own<DT>(sm, s + j), v[j]);
+            st.template add<4>(v);
+        }
+        for (; s < end; ++s) {
+            float v[1][8];
+            unpack<DT>(own<DT>(sm, s), v[0]);
+            st.template add<1>(v);
+        }
+    };
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    take(0, half);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    take(half, mine_rows);
+    constexpr float PER = 8 / GV;
     const int c_lo = slab * p.vc * 8, g_lo = c_lo / p.cpg;
     const int ng = max(0, min(p.C, c_lo + p.vc * 8) - c_lo) / p.cpg;     // whole groups of the slab
-    const float mine = (float)max(0, min((rank + 1) * p.rows, p.HW) - rank * p.rows);
-    block_stats(p, st, fmaxf(mine, 1.f), red, sums);
+    const int epg = p.cpg * GV / 8;                                      // entries of a group
+    const float mine = PER * (float)max(0, min((rank + 1) * p.rows, p.HW) - rank * p.rows);
+    block_stats<GV>(p, st, fmaxf(mine, 1.f), red, sums);
     for (int g = threadIdx.x; g < ng; g += T) {
         float m = 0.f, q = 0.f;
-        for (int c = 0; c < p.cpg; ++c) m += sums[g * p.cpg + c];
-        m /= (float)p.cpg;
-        for (int c = 0; c < p.cpg; ++c) {
-            const float d = sums[g * p.cpg + c] - m;
-            q += sums[p.vc * 8 + g * p.cpg + c] + mine * d * d;
+        for (int e = 0; e < epg; ++e) m += sums[g * epg + e];
+        m /= (float)epg;
+        for (int e = 0; e < epg; ++e) {
+            const float d = sums[g * epg + e] - m;
+            q += sums[p.vc * GV + g * epg + e] + mine * d * d;
         }
         group[2 * g] = m;
         group[2 * g + 1] = q;
@@ -341,55 +382,79 @@ __global__ void __launch_bounds__(T, 2) gn_fwd_unit_kernel(const Params p) {
     }
     // also: no CTA of the cluster leaves while another reads its sums
     if (p.cluster > 1) cl.sync(); else __syncthreads();
-    Affine f;
-    affine_of(p, t, f, [&](int g) { return total[2 * (g - g_lo)]; }, [&](int g) { return total[2 * (g - g_lo) + 1]; });
-    s = 0;
-    for (r = t.first; r < t.end; ++s, r += t.step)
-        store<DT>(p.out, at(p, t, r), apply<DT, ACT>(own<DT>(sm, s), f, t.nval));
+    Affine<DT> f;
+    affine_of<DT>(p, t, f, [&](int g) { return total[2 * (g - g_lo)]; }, [&](int g) { return total[2 * (g - g_lo) + 1]; });
+    long long e = at(p, t, t.first);
+    for (int s = 0; s < mine_rows; ++s, e += step) store<DT>(p.out, e, apply<DT, ACT>(own<DT>(sm, s), f, t.nval));
 }
 
-// The backward's terms of 8 channels of one pixel: dz and xh
+// The backward's coefficients of a thread's 8 channels; statistics once per entry of GV (channel
+// i belongs to entry i * GV / 8).
+template <int GV>
 struct BwdAffine {
-    float mean[8], rstd[8], gamma[8], beta[8];
+    float mean[GV], rstd[GV], gamma[8], beta[8];
 };
-__device__ __forceinline__ void bwd_affine_of(const Params& p, const Part& t, BwdAffine& f) {
+template <int GV>
+__device__ __forceinline__ void bwd_affine_of(const Params& p, const Part& t, BwdAffine<GV>& f) {
+    int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        f.mean[i] = f.rstd[i] = f.gamma[i] = f.beta[i] = 0.f;
-        if (i < t.nval) {
-            const int c = t.c0 + i;
-            const long long g = (long long)t.n * p.G + c / p.cpg;
-            f.mean[i] = p.mean[g];
-            f.rstd[i] = p.rstd[g];
-            f.gamma[i] = p.gamma ? p.gamma[c] : 1.f;
-            f.beta[i] = p.beta ? p.beta[c] : 0.f;
+        const bool in = i < t.nval;
+        if (i % (8 / GV) == 0) {
+            f.mean[i * GV / 8] = in ? p.mean[(long long)t.n * p.G + g] : 0.f;
+            f.rstd[i * GV / 8] = in ? p.rstd[(long long)t.n * p.G + g] : 0.f;
         }
+        f.gamma[i] = !in ? 0.f : p.gamma ? p.gamma[t.c0 + i] : 1.f;
+        f.beta[i] = in && p.beta ? p.beta[t.c0 + i] : 0.f;
+        if (--left == 0) { ++g; left = p.cpg; }
     }
 }
-template <int DT, int ACT>
-__device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy, const BwdAffine& f, float (&dz)[8],
-                                          float (&xh)[8]) {
-    unpack<DT>(vx, xh);
-    unpack<DT>(vdy, dz);
+// rstd times the means of t and t xh, from pairs of means per group starting at group g0
+template <int GV>
+__device__ __forceinline__ void bwd_means_of(const Params& p, const Part& t, const BwdAffine<GV>& f, const float* pairs,
+                                             int g0, float (&m1)[GV], float (&m2)[GV]) {
+    int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        xh[i] = (xh[i] - f.mean[i]) * f.rstd[i];
+        if (i % (8 / GV) == 0) {
+            m1[i * GV / 8] = i < t.nval ? f.rstd[i * GV / 8] * pairs[2 * (g - g0)] : 0.f;
+            m2[i * GV / 8] = i < t.nval ? f.rstd[i * GV / 8] * pairs[2 * (g - g0) + 1] : 0.f;
+        }
+        if (--left == 0) { ++g; left = p.cpg; }
+    }
+}
+// dz and xh of 8 channels of one pixel (0 for padding, whatever it holds)
+template <int DT, int ACT, int GV>
+__device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy, const BwdAffine<GV>& f, int nval,
+                                          float (&dz)[8], float (&xh)[8]) {
+    unpack<DT>(vx, xh);
+    unpack<DT>(vdy, dz);
+    if (nval < 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            xh[i] = i < nval ? xh[i] : 0.f;
+            dz[i] = i < nval ? dz[i] : 0.f;
+        }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        xh[i] = (xh[i] - f.mean[i * GV / 8]) * f.rstd[i * GV / 8];
         dz[i] = act_bwd<ACT>(dz[i], fmaf(xh[i], f.gamma[i], f.beta[i]));
     }
 }
-template <int DT>
-__device__ __forceinline__ Vec<DT> bwd_out(const float (&dz)[8], const float (&xh)[8], const BwdAffine& f,
-                                           const float (&m1)[8], const float (&m2)[8], int nval) {
+// dx = rstd (gamma dz - mean(t) - xh mean(t xh)), m1 and m2 with their rstd
+template <int DT, int GV>
+__device__ __forceinline__ Vec<DT> bwd_out(const float (&dz)[8], const float (&xh)[8], const BwdAffine<GV>& f,
+                                           const float (&m1)[GV], const float (&m2)[GV]) {
     float d[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-        d[i] = i < nval ? f.rstd[i] * (fmaf(dz[i], f.gamma[i], -m1[i]) - xh[i] * m2[i]) : 0.f;
+        d[i] = fmaf(dz[i] * f.gamma[i], f.rstd[i * GV / 8], -fmaf(xh[i], m2[i * GV / 8], m1[i * GV / 8]));
     return pack<DT>(d);
 }
 
 // ws: per sample and channel (sum dz, sum dz xh), for gn_params_kernel
-template <int DT, int ACT>
-__global__ void __launch_bounds__(T, 2) gn_bwd_unit_kernel(const Params p) {
+template <int DT, int ACT, int GV>
+__global__ void __launch_bounds__(T, GV == 8 ? 2 : 3) gn_bwd_unit_kernel(const Params p) {
     extern __shared__ uint4 sm[];
     cg::cluster_group cl = cg::this_cluster();
     const int rank = (int)cl.block_rank(), unit = blockIdx.x / p.cluster;
@@ -399,25 +464,37 @@ __global__ void __launch_bounds__(T, 2) gn_bwd_unit_kernel(const Params p) {
     float* red = reinterpret_cast<float*>(sm + 2 * p.iters * Elem<DT>::V16 * T);
     float* sums = red + T * 16;             // the CTA's sums, read by the cluster
     float* total = red;                     // the unit's, once red is free
-    for (int s = 0, r = t.first; r < t.end; ++s, r += t.step) {
-        copy_in<DT>(sm, s, p.x, at(p, t, r));
-        copy_in<DT>(sm_dy, s, p.dy, at(p, t, r));
-    }
-    BwdAffine f;
-    bwd_affine_of(p, t, f);
-    copies_done();
-    float a[8] = {}, b[8] = {};
-    int s = 0;
-    for (int r = t.first; r < t.end; ++s, r += t.step) {
-        float dz[8], xh[8];
-        bwd_terms<DT, ACT>(own<DT>(sm, s), own<DT>(sm_dy, s), f, dz, xh);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            a[i] += dz[i];
-            b[i] = fmaf(dz[i], xh[i], b[i]);
+    const long long step = (long long)t.step * p.Cs;
+    const int mine_rows = t.first < t.end ? (t.end - t.first + t.step - 1) / t.step : 0;
+    const int half = mine_rows / 2;         // sums of the first half while the second arrives
+    {
+        long long e = at(p, t, t.first);
+        for (int s = 0; s < mine_rows; ++s, e += step) {
+            if (s == half) asm volatile("cp.async.commit_group;" ::: "memory");
+            copy_in<DT>(sm, s, p.x, e);
+            copy_in<DT>(sm_dy, s, p.dy, e);
         }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    reduce_channels(p, a, b, red, sums);
+    BwdAffine<GV> f;
+    bwd_affine_of<GV>(p, t, f);
+    float a[8] = {}, b[8] = {};
+    auto take = [&](int s, int end) {
+        for (; s < end; ++s) {
+            float dz[8], xh[8];
+            bwd_terms<DT, ACT, GV>(own<DT>(sm, s), own<DT>(sm_dy, s), f, t.nval, dz, xh);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                a[i] += dz[i];
+                b[i] = fmaf(dz[i], xh[i], b[i]);
+            }
+        }
+    };
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    take(0, half);
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    take(half, mine_rows);
+    reduce_columns<8>(p, a, b, red, sums);
     if (p.cluster > 1) cl.sync();
     const int c_lo = slab * p.vc * 8, nc = max(0, min(p.C - c_lo, p.vc * 8));
     for (int c = threadIdx.x; c < p.vc * 16; c += T) {
@@ -441,18 +518,13 @@ __global__ void __launch_bounds__(T, 2) gn_bwd_unit_kernel(const Params p) {
         means[2 * g + 1] = m2 * inv;
     }
     __syncthreads();
-    float m1[8], m2[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int g = i < t.nval ? (t.c0 + i - c_lo) / p.cpg : 0;
-        m1[i] = i < t.nval ? means[2 * g] : 0.f;
-        m2[i] = i < t.nval ? means[2 * g + 1] : 0.f;
-    }
-    s = 0;
-    for (int r = t.first; r < t.end; ++s, r += t.step) {
+    float m1[GV], m2[GV];
+    bwd_means_of<GV>(p, t, f, means, c_lo / p.cpg, m1, m2);
+    long long e = at(p, t, t.first);
+    for (int s = 0; s < mine_rows; ++s, e += step) {
         float dz[8], xh[8];
-        bwd_terms<DT, ACT>(own<DT>(sm, s), own<DT>(sm_dy, s), f, dz, xh);
-        store<DT>(p.out, at(p, t, r), bwd_out<DT>(dz, xh, f, m1, m2, t.nval));
+        bwd_terms<DT, ACT, GV>(own<DT>(sm, s), own<DT>(sm_dy, s), f, t.nval, dz, xh);
+        store<DT>(p.out, e, bwd_out<DT, GV>(dz, xh, f, m1, m2));
     }
 }
 
@@ -482,22 +554,22 @@ __global__ void __launch_bounds__(T) gn_partial_kernel(const Params p) {
     float* sums = red + T * 16;
     const Part t = part_of(p, blockIdx.z, blockIdx.y, blockIdx.x);
     if constexpr (BWD) {
-        BwdAffine f;
-        bwd_affine_of(p, t, f);
+        BwdAffine<8> f;
+        bwd_affine_of<8>(p, t, f);
         float a[8] = {}, b[8] = {};
 #pragma unroll 4
         for (int r = t.first; r < t.end; r += t.step) {
             float dz[8], xh[8];
-            bwd_terms<DT, ACT>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, dz, xh);
+            bwd_terms<DT, ACT, 8>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 a[i] += dz[i];
                 b[i] = fmaf(dz[i], xh[i], b[i]);
             }
         }
-        reduce_channels(p, a, b, red, sums);
+        reduce_columns<8>(p, a, b, red, sums);
     } else {
-        Stats st;
+        Stats<8> st;
         st.clear();
         int r = t.first;
         for (; r + 3 * t.step < t.end; r += 4 * t.step) {
@@ -507,14 +579,14 @@ __global__ void __launch_bounds__(T) gn_partial_kernel(const Params p) {
             for (int j = 0; j < 4; ++j) q[j] = load<DT>(p.x, at(p, t, r + j * t.step));
 #pragma unroll
             for (int j = 0; j < 4; ++j) unpack<DT>(q[j], v[j]);
-            st.add<4>(v);
+            st.template add<4>(v);
         }
         for (; r < t.end; r += t.step) {
             float v[1][8];
             unpack<DT>(load<DT>(p.x, at(p, t, r)), v[0]);
-            st.add<1>(v);
+            st.template add<1>(v);
         }
-        block_stats(p, st, (float)(min((int)(blockIdx.x + 1) * p.rows, p.HW) - (int)blockIdx.x * p.rows), red, sums);
+        block_stats<8>(p, st, (float)(min((int)(blockIdx.x + 1) * p.rows, p.HW) - (int)blockIdx.x * p.rows), red, sums);
     }
     const int c_lo = blockIdx.y * p.vc * 8;
     for (int c = threadIdx.x; c < p.vc * 8; c += T)
@@ -543,18 +615,26 @@ __global__ void __launch_bounds__(T) gn_combine_kernel(const Params p, float* st
     const long long M = (long long)p.nchunk * p.cpg;
     float a = 0.f, b = 0.f;
     if constexpr (BWD) {
-        // a thread per channel, so that the channel's sums come out whole
-        for (int c = threadIdx.x; c < p.cpg; c += T) {
+        // 8 lanes per channel, each a stride of the chunks, joined in lane order
+        const int sub = threadIdx.x % 8;
+        for (int c = threadIdx.x / 8; c - (int)threadIdx.x / 8 < p.cpg; c += T / 8) {
             float sa = 0.f, sb = 0.f;
-            for (int k = 0; k < p.nchunk; ++k) {
-                sa += p.ws[partial_at(p, n, 0, k, c0 + c)];
-                sb += p.ws[partial_at(p, n, 1, k, c0 + c)];
+            if (c < p.cpg)
+                for (int k = sub; k < p.nchunk; k += 8) {
+                    sa += p.ws[partial_at(p, n, 0, k, c0 + c)];
+                    sb += p.ws[partial_at(p, n, 1, k, c0 + c)];
+                }
+            for (int o = 4; o; o >>= 1) {
+                sa += __shfl_xor_sync(~0u, sa, o);
+                sb += __shfl_xor_sync(~0u, sb, o);
             }
-            chan[(long long)n * p.C + c0 + c] = sa;
-            chan[((long long)p.N + n) * p.C + c0 + c] = sb;
-            const float w = p.gamma ? p.gamma[c0 + c] : 1.f;
-            a = fmaf(w, sa, a);
-            b = fmaf(w, sb, b);
+            if (c < p.cpg && sub == 0) {
+                chan[(long long)n * p.C + c0 + c] = sa;
+                chan[((long long)p.N + n) * p.C + c0 + c] = sb;
+                const float w = p.gamma ? p.gamma[c0 + c] : 1.f;
+                a = fmaf(w, sa, a);
+                b = fmaf(w, sb, b);
+            }
         }
         a = block_sum(a, sh);
         b = block_sum(b, sh);
@@ -592,24 +672,19 @@ __global__ void __launch_bounds__(T) gn_apply_kernel(const Params p, const float
     const Part t = part_of(p, gridDim.z - 1 - blockIdx.z, gridDim.y - 1 - blockIdx.y, gridDim.x - 1 - blockIdx.x);
     const float* s = stat + 2 * (long long)t.n * p.G;
     if constexpr (BWD) {
-        BwdAffine f;
-        bwd_affine_of(p, t, f);
+        BwdAffine<8> f;
+        bwd_affine_of<8>(p, t, f);
         float m1[8], m2[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int g = i < t.nval ? (t.c0 + i) / p.cpg : 0;
-            m1[i] = i < t.nval ? s[2 * g] : 0.f;
-            m2[i] = i < t.nval ? s[2 * g + 1] : 0.f;
-        }
+        bwd_means_of<8>(p, t, f, s, 0, m1, m2);
 #pragma unroll 4
         for (int r = t.first; r < t.end; r += t.step) {
             float dz[8], xh[8];
-            bwd_terms<DT, ACT>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, dz, xh);
-            store<DT>(p.out, at(p, t, r), bwd_out<DT>(dz, xh, f, m1, m2, t.nval));
+            bwd_terms<DT, ACT, 8>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
+            store<DT>(p.out, at(p, t, r), bwd_out<DT, 8>(dz, xh, f, m1, m2));
         }
     } else {
-        Affine f;
-        affine_of(p, t, f, [&](int g) { return s[2 * g]; }, [&](int g) { return s[2 * g + 1]; });
+        Affine<DT> f;
+        affine_of<DT>(p, t, f, [&](int g) { return s[2 * g]; }, [&](int g) { return s[2 * g + 1]; });
 #pragma unroll 4
         for (int r = t.first; r < t.end; r += t.step)
             store<DT>(p.out, at(p, t, r), apply<DT, ACT>(load<DT>(p.x, at(p, t, r)), f, t.nval));
@@ -626,6 +701,9 @@ static int check_shape(int nN, int nHW, int nC, int nCs, int nGroups, int nDtype
     return OM_OK;
 }
 static bool aligned(const void* p, int a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
+
+// GV of a number of channels per group
+static int entries(int cpg) { return cpg % 8 == 0 ? 1 : cpg == 4 ? 2 : 8; }
 
 // Fills in the split of the work: p->cluster > 0 for the one-launch form with `smem` bytes,
 // 0 for the three-launch form.
@@ -646,14 +724,16 @@ static void plan(Params* p, int dtype, bool bwd, size_t* smem) {
         p->vc = (int)(slab / 8);
         p->nslab = (int)((p->Cs + slab - 1) / slab);
         const int step = T / p->vc;
-        const size_t fixed = (size_t)T * 16 * 4 + (size_t)p->vc * 16 * 4 + (bwd ? 0 : 4 * MAX_GROUPS * 4);
+        const int nv = bwd ? 8 : entries(p->cpg);
+        const size_t fixed = (size_t)(T + p->vc) * 2 * nv * 4 + (bwd ? 0 : 4 * MAX_GROUPS * 4);
         for (int k = 1; k <= MAX_CLUSTER; k *= 2) {
             const int rows = (p->HW + k - 1) / k, iters = (rows + step - 1) / step;
             const size_t need = (size_t)iters * T * per_vec + fixed;
-            if (need > SMEM_MAX) continue;
+            // one CTA on an SM leaves loads, sums and stores one after another: only for one wave
+            if (need > ((long long)p->N * p->nslab * k <= 148 ? SMEM_MAX : KEEP_MAX)) continue;
             p->cluster = k; p->rows = rows; p->iters = iters; *smem = need;
             // enough parts to fill the GPU, with two CTAs on an SM
-            if ((long long)p->N * p->nslab * k >= 2 * 148 && need <= SMEM_MAX / 2 - 1024) break;
+            if ((long long)p->N * p->nslab * k >= 2 * 148 && need <= KEEP_GOOD) break;
             if (iters <= 4) break;
         }
     }
@@ -661,7 +741,7 @@ static void plan(Params* p, int dtype, bool bwd, size_t* smem) {
     p->vc = p->Cs / 8 < MAX_VC ? p->Cs / 8 : MAX_VC;
     p->nslab = (p->Cs / 8 + p->vc - 1) / p->vc;
     const int step = T / p->vc;
-    int iters = 16;
+    int iters = 8;
     while (iters < 256 && (long long)p->N * p->nslab * ((p->HW + step * iters - 1) / (step * iters)) > 148 * 16) iters *= 2;
     p->rows = step * iters;
     p->iters = iters;
@@ -678,11 +758,17 @@ template <int DT, int ACT, bool BWD>
 static int launch(DeviceCtx* c, Params p, size_t smem) {
     static bool attr_set[64] = {false};
     if (p.cluster) {
-        auto kern = BWD ? gn_bwd_unit_kernel<DT, ACT> : gn_fwd_unit_kernel<DT, ACT>;
+        using Kern = void (*)(const Params);
+        const Kern kerns[3] = {BWD ? gn_bwd_unit_kernel<DT, ACT, 1> : gn_fwd_unit_kernel<DT, ACT, 1>,
+                               BWD ? gn_bwd_unit_kernel<DT, ACT, 2> : gn_fwd_unit_kernel<DT, ACT, 2>,
+                               BWD ? gn_bwd_unit_kernel<DT, ACT, 8> : gn_fwd_unit_kernel<DT, ACT, 8>};
         if (!attr_set[c->device]) {
-            OMB_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
+            for (Kern k : kerns)
+                OMB_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MAX));
             attr_set[c->device] = true;
         }
+        const int gv = entries(p.cpg);
+        const Kern kern = kerns[gv == 1 ? 0 : gv == 2 ? 1 : 2];
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)((long long)p.N * p.nslab * p.cluster));
         cfg.blockDim = dim3(T);
