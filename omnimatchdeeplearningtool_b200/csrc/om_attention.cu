@@ -14,7 +14,7 @@ struct View {          // a [batch, token, head, D] tensor: element strides, D c
 struct Params {
     View q, k, v, o, dout, dq, dk, dv;
     float* lse;        // [B, H, Sq]
-    float* delta;      // [B, H, Sq], scale times the row sums of dO o O
+    float* delta;      // [B, H, Sq], -scale times the row sums of dO o O
     const int *qlens, *kvlens;
     int B, H, Hkv, Sq, Sk, D, causal;
     float scale;
@@ -92,6 +92,34 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two fp32 operations in one instruction
+struct F2 { float x, y; };
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 template <int DT>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -179,9 +207,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     constexpr int W_LOAD = NT * 4, W_MMA = NT * 4 + 1;
-    const int h = blockIdx.y % p.H, b = blockIdx.y / p.H, hk = h / (p.H / p.Hkv);
-    // the longest rows of a causal mask first
-    const int q0 = (p.causal ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * (NT * 128);
+    // causal: heads fastest and the longest rows first, so that the last CTAs to start are short
+    const int tiles = (p.Sq + NT * 128 - 1) / (NT * 128), heads = p.B * p.H;
+    const int bh = p.causal ? blockIdx.x % heads : blockIdx.x / tiles;
+    const int h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hkv);
+    const int q0 = (p.causal ? tiles - 1 - blockIdx.x / heads : blockIdx.x % tiles) * (NT * 128);
     const int ql = len_of(p.qlens, b, p.Sq), kl = len_of(p.kvlens, b, p.Sk);
     int end = q0 < ql ? kl : 0;
     if (p.causal) end = min(end, min(q0 + NT * 128, ql) - 1 + kl - ql + 1);
@@ -293,17 +323,39 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 #pragma unroll
                 for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
             }
-            float mx[4] = {s[0], s[1], s[2], s[3]};
+            float mx[4] = {m, s[0], s[1], s[2]};
 #pragma unroll
-            for (int c = 4; c < 128; ++c) mx[c % 4] = fmaxf(mx[c % 4], s[c]);
-            const float m_new = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), m);
+            for (int c = 3; c < 127; c += 2) mx[c / 2 % 4] = max3(mx[c / 2 % 4], s[c], s[c + 1]);
+            const float m_new = max3(fmaxf(mx[0], s[127]), mx[1], fmaxf(mx[2], mx[3]));
+            // the reference maximum moves when a row's maximum has grown by more than 2^8
+            const bool grow = j > 0 && __any_sync(~0u, (m_new - m) * p.scale2 > 8.f);
+            float f = 1.f;
             if (j == 0) {
                 m = m_new;
-            } else if (__any_sync(~0u, (m_new - m) * p.scale2 > 8.f)) {
-                // S_j is complete, so every product issued before it is: O may be changed
-                const float f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale2);
+            } else if (grow) {
+                f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale2);
                 l *= f;
                 m = m_new;
+            }
+            const float sub = m == -INFINITY ? 0.f : -m * p.scale2;
+            const F2 sc = {p.scale2, p.scale2}, sb = {sub, sub};
+            F2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t w[16];
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                    F2 e = fma2({s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]}, sc, sb);
+                    e.x = ex2(e.x);
+                    e.y = ex2(e.y);
+                    sum[x % 2] = add2(sum[x % 2], e);
+                    w[x] = pack16<DT>(e.x, e.y);
+                }
+                tmem_st16(s_addr + c * 16, w);
+            }
+            sum[0] = add2(sum[0], sum[1]);
+            l += sum[0].x + sum[0].y;
+            if (grow)                     // S_j is complete, so every product issued before it is
                 for (int c = 0; c < p.D; c += 32) {
                     uint32_t o[32];
                     tmem_ld32_issue(o_addr + c, o);
@@ -312,24 +364,6 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
                     tmem_st32(o_addr + c, o);
                 }
-                tmem_st_wait();
-            }
-            const float sub = m == -INFINITY ? 0.f : -m * p.scale2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t w[16];
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    const float a = ex2(fmaf(s[c * 32 + 2 * x], p.scale2, sub));
-                    const float d = ex2(fmaf(s[c * 32 + 2 * x + 1], p.scale2, sub));
-                    sum[x % 2 * 2] += a;
-                    sum[x % 2 * 2 + 1] += d;
-                    w[x] = pack16<DT>(a, d);
-                }
-                tmem_st16(s_addr + c * 16, w);
-            }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             // keys past the sequence's length may hold anything
             if (t == 0 && j == nblk - 1 && kl - j * 128 < 128) {
                 const int iv = 2 * j + 1;
@@ -428,9 +462,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     constexpr int W_LOAD = 8, W_MMA = 9;
     const int rep = p.H / p.Hkv, heads = KV ? p.Hkv : p.H;
-    const int hx = blockIdx.y % heads, b = blockIdx.y / heads;   // head of the kept tiles
+    // causal: heads fastest and the tiles with the longest rows (first columns) first
+    const int tiles = ((KV ? p.Sk : p.Sq) + 127) / 128, bhs = p.B * heads;
+    const int bh = p.causal ? blockIdx.x % bhs : blockIdx.x / tiles;
+    const int tile_x = p.causal ? blockIdx.x / bhs : blockIdx.x % tiles;
+    const int hx = bh % heads, b = bh / heads;                   // head of the kept tiles
     const int hy0 = KV ? hx * rep : hx / rep;                    // first head of the streamed ones
-    const int r0 = (p.causal && !KV ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * 128;
+    const int r0 = (p.causal && !KV ? tiles - 1 - tile_x : tile_x) * 128;
     const int ql = len_of(p.qlens, b, p.Sq), kl = len_of(p.kvlens, b, p.Sk);
     // streamed blocks: first .. first + per of each streamed head
     int first = 0, per = 0;
@@ -545,7 +583,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         const uint32_t s_addr = tmem + lanes + w * 64, dp_addr = s_addr + 128;
         constexpr float LOG2E = 1.4426950408889634f;
         bool ok = true;
-        float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's lse * log2(e) and scale * delta
+        float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's -lse * log2(e) and -scale * delta
         int row_lo = 0, row_hi = 0;           // the streamed rows that this row meets
         if (KV) {
             if (r < kl) {
@@ -569,12 +607,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                         d += f.x * g.x + f.y * g.y;
                     }
                 }
-                lse2 = p.lse[((long long)b * p.H + hx) * p.Sq + r] * LOG2E;
+                lse2 = -p.lse[((long long)b * p.H + hx) * p.Sq + r] * LOG2E;
             }
             stat[tid] = d;
             mbar_arrive(stat_ready);
             ok = __all_sync(~0u, mbar_wait(stat_ready, 0, abort_flag));
-            ds0 = (stat[row] + stat[row + 128]) * p.scale;
+            ds0 = -(stat[row] + stat[row + 128]) * p.scale;
             if (ok && w == 0 && r < p.Sq) p.delta[((long long)b * p.H + hx) * p.Sq + r] = ds0;
         }
         // KV: thread tid fetches lse (tid < 128) or delta of one query of the next block
@@ -582,7 +620,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const int i = (first + blk % per) * 128 + tid % 128;
             if (i >= ql) return 0.f;
             const long long at = ((long long)b * p.H + hy0 + blk / per) * p.Sq + i;
-            return tid < 128 ? p.lse[at] * LOG2E : p.delta[at];
+            return tid < 128 ? -p.lse[at] * LOG2E : p.delta[at];
         };
         float next = KV && nblk > 0 ? fetch(0) : 0.f;
         for (int i = 0; ok && i < nblk; ++i) {
@@ -610,7 +648,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const int lo = row_lo - y0 - w * 64, hi = row_hi - y0 - w * 64;
             const bool mask = __any_sync(~0u, lo > 0 || hi < 64);
 #pragma unroll
-            for (int c = 0; c < 64; ++c) pr[c] = ex2(fmaf(pr[c], p.scale2, KV ? -c_lse[c] : -lse2));
+            for (int c = 0; c < 64; c += 2) {
+                const F2 sub = KV ? F2{c_lse[c], c_lse[c + 1]} : F2{lse2, lse2};
+                const F2 e = fma2({pr[c], pr[c + 1]}, {p.scale2, p.scale2}, sub);
+                pr[c] = ex2(e.x);
+                pr[c + 1] = ex2(e.y);
+            }
             if (mask) {
 #pragma unroll
                 for (int c = 0; c < 64; ++c) pr[c] = c >= lo && c < hi ? pr[c] : 0.f;
@@ -641,7 +684,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             tmem_ld_wait<64>(dv);
             float* dp = reinterpret_cast<float*>(dv);
 #pragma unroll
-            for (int c = 0; c < 64; ++c) dp[c] = pr[c] * fmaf(dp[c], p.scale, KV ? -c_ds[c] : -ds0);
+            for (int c = 0; c < 64; c += 2) {
+                const F2 sub = KV ? F2{c_ds[c], c_ds[c + 1]} : F2{ds0, ds0};
+                const F2 e = mul2({pr[c], pr[c + 1]}, fma2({dp[c], dp[c + 1]}, {p.scale, p.scale}, sub));
+                dp[c] = e.x;
+                dp[c + 1] = e.y;
+            }
             if (mask) {                       // 0 * what a masked place holds
 #pragma unroll
                 for (int c = 0; c < 64; ++c) dp[c] = c >= lo && c < hi ? dp[c] : 0.f;
@@ -696,7 +744,7 @@ static int check_sizes(int nBatch, int nHeads, int nKvHeads, int nSq, int nSk, i
     if (nBatch < 0 || nHeads <= 0 || nKvHeads <= 0 || nHeads % nKvHeads || nSq < 0 || nSk < 0 ||
         nHeadDim <= 0)
         return OM_ERR_INVALID;
-    if (nHeadDim % 8 || nHeadDim > 128 || (long long)nBatch * nHeads > 65535)
+    if (nHeadDim % 8 || nHeadDim > 128)
         return OM_ERR_UNSUPPORTED;
     return OM_OK;
 }
@@ -751,8 +799,9 @@ static int launch_fwd(DeviceCtx* c, const Params& p) {
     if (st == OM_OK && p.Sk > 0) st = encode(&mk, p.k, p.B, p.Sk, p.Hkv, p.D, DT);
     if (st == OM_OK && p.Sk > 0) st = encode(&mv, p.v, p.B, p.Sk, p.Hkv, p.D, DT);
     if (st != OM_OK) return st;
-    const dim3 grid((p.Sq + NT * 128 - 1) / (NT * 128), p.B * p.H);
-    kern<<<grid, Cf::THREADS, Cf::SMEM, c->compute>>>(mq, mk, mv, p);
+    const long long grid = (long long)((p.Sq + NT * 128 - 1) / (NT * 128)) * p.B * p.H;
+    if (grid > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
+    kern<<<(unsigned)grid, Cf::THREADS, Cf::SMEM, c->compute>>>(mq, mk, mv, p);
     return after_launch(c);
 }
 template <int DT>
@@ -770,7 +819,9 @@ static int launch_bwd(DeviceCtx* c, const CUtensorMap (&m)[4], const Params& p) 
         OMB_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::SMEM));
         attr_set[c->device] = true;
     }
-    const dim3 grid(((KV ? p.Sk : p.Sq) + 127) / 128, p.B * (KV ? p.Hkv : p.H));
+    const long long n = (long long)(((KV ? p.Sk : p.Sq) + 127) / 128) * p.B * (KV ? p.Hkv : p.H);
+    if (n > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
+    const unsigned grid = (unsigned)n;
     if (KV)
         kern<<<grid, Cf::THREADS, Cf::SMEM, c->compute>>>(m[1], m[2], m[0], m[3], p);
     else
