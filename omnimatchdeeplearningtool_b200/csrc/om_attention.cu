@@ -35,14 +35,27 @@ __device__ __forceinline__ int len_of(const int* lens, int b, int most) {
     return lens ? min(max(lens[b], 0), most) : most;
 }
 // ---------------------------------------------------------------- tcgen05 pieces
-// D[tmem] (+)= A[tmem] * B[smem]: A holds 16-bit pairs, one row per lane, K along the columns.
-__device__ __forceinline__ void tc_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc,
-                                          uint32_t idesc, uint32_t accumulate) {
+// The low word of a shared-memory descriptor moves with the operand's address; the high word
+// (8 rows of 128 bytes apart, 128-byte swizzle) is the same for every operand here. The products
+// are issued by one thread, so each takes few instructions: the descriptors of a tile's steps are
+// its first one plus constants.
+constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (LAYOUT_SW128 << 29);
+template <bool ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate));
+        "{\n\t.reg .b64 a, b;\n\t.reg .pred p;\n\t"
+        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(DESC_HI), "n"(ACC ? 1 : 0));
+}
+// D[tmem] (+)= A[tmem] * B[smem]: A holds 16-bit pairs, one row per lane, K along the columns.
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
+                                       uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .b64 b;\n\t.reg .pred p;\n\t"
+        "mov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(DESC_HI), "r"(accumulate));
 }
 // 32 columns of this warp's lanes, without waiting: tmem_ld_wait orders the registers.
 __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* v) {
@@ -94,7 +107,7 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 // two fp32 operations in one instruction
-struct F2 { float x, y; };
+struct alignas(8) F2 { float x, y; };
 __device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
     F2 d;
     asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
@@ -137,13 +150,27 @@ __device__ __forceinline__ uint32_t idesc_f16(bool f16, int n, bool b_mn, bool n
 // A [128 rows, DP] 16-bit tile lies in shared memory as DP / 64 panels of 128 rows x 128 bytes
 // with the 128-byte swizzle, as TMA writes it.
 constexpr int PANEL = 128 * 128;
-// K-major operand (rows = M or N, K = the head dimension), 16 columns at step k.
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int k) {
-    return smem_desc(tile + (k / 4) * PANEL + (k % 4) * 32, 16, 1024, LAYOUT_SW128);
+// Low descriptor words. K-major operand (rows = M or N, K = the head dimension): 16 columns are 32
+// bytes, 64 a panel. MN-major operand (rows = K, N = the head dimension): 16 rows are 2048 bytes,
+// panels of 64 columns PANEL apart.
+__device__ __forceinline__ uint32_t desc_k(uint32_t tile) { return (tile >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t tile) { return (tile >> 4) | ((uint32_t)(PANEL >> 4) << 16); }
+// D = X Y^T over the head dimension, ks steps of 16 (X, Y: tiles of 128 rows)
+template <int DP>
+__device__ __forceinline__ void product_k(uint32_t d_tmem, uint32_t x, uint32_t y, uint32_t idesc, int ks) {
+    const uint32_t a = desc_k(x), b = desc_k(y);
+    mma_ss<false>(d_tmem, a, b, idesc);
+#pragma unroll
+    for (int k = 1; k < DP / 16; ++k)
+        if (k < ks) mma_ss<true>(d_tmem, a + (k / 4) * (PANEL >> 4) + (k % 4) * 2, b + (k / 4) * (PANEL >> 4) + (k % 4) * 2, idesc);
 }
-// MN-major operand (rows = K, N = the head dimension), 16 rows at step k.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int k) {
-    return smem_desc(tile + k * 2048, PANEL, 1024, LAYOUT_SW128);
+// D (+)= A Y over Y's 128 rows; columns CW w .. of A are the CW / 2 words at a_tmem + CW w
+template <int CW>
+__device__ __forceinline__ void product_mn(uint32_t d_tmem, uint32_t a_tmem, uint32_t y, uint32_t idesc, bool accumulate) {
+    const uint32_t b = desc_mn(y);
+    mma_ts(d_tmem, a_tmem, b, idesc, accumulate);
+#pragma unroll
+    for (int k = 1; k < 8; ++k) mma_ts(d_tmem, a_tmem + k * 16 / CW * CW + k * 16 % CW / 2, b + k * 128, idesc, 1);
 }
 template <int DP>
 __device__ __forceinline__ void load_tile(uint32_t dst_off, uint8_t* smem, const CUtensorMap* map,
@@ -264,8 +291,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             const uint32_t q_tile = smem_u32(smem);
             auto qk = [&](int t, int i) {
                 const uint32_t kt = kv_base + (i % Cf::SLOTS) * Cf::TILE;
-                for (int k = 0; k < ks; ++k)
-                    tc_mma(tmem + t * 128, desc_k(q_tile + t * Cf::TILE, k), desc_k(kt, k), id_s, k > 0);
+                product_k<DP>(tmem + t * 128, q_tile + t * Cf::TILE, kt, id_s, ks);
                 tc_commit(s_full + t);
             };
             auto wait_kv = [&](int i) { return mbar_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
@@ -283,9 +309,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     ok = mbar_wait(p_full + t, j & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    for (int k = 0; k < 8; ++k)
-                        tc_mma_ts(tmem + Cf::O_COL + t * Cf::O_STEP, tmem + t * 128 + k * 8, desc_mn(vt, k), id_o,
-                                  j > 0 || k > 0);
+                    product_mn<128>(tmem + Cf::O_COL + t * Cf::O_STEP, tmem + t * 128, vt, id_o, j > 0);
                     if (more) qk(t, 2 * j + 2);
                 }
                 if (!ok) break;
@@ -429,8 +453,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 // operands of the first products and as MN-major operands of the others. dQ and dK, dV are
 // summed in two passes that each recompute S (7 products instead of 5): every sum is kept in one
 // CTA's TMEM, so no fp32 gradient is accumulated in memory by atomics and results are repeatable.
-// Two warpgroups share the tile: warpgroup w has columns 64 w .. 64 w + 63.
-// TMEM: S at 0, dP at 128 (P and dS over the first half of each 64 columns), accumulators behind.
+// Four warpgroups share the tile: warpgroup w has columns 32 w .. 32 w + 31 (with two, each
+// scheduler had two warps to hide the TMEM and exponential latencies behind).
+// TMEM: S at 0, dP at 128 (P and dS over the first half of each 32 columns), accumulators behind.
+constexpr int BWD_WG = 4, BWD_COLS = 128 / BWD_WG;
 template <int DP>
 struct BwdCfg {
     static constexpr int TILE = DP / 64 * PANEL;
@@ -438,12 +464,12 @@ struct BwdCfg {
     static constexpr int STAT_OFF = (2 + SLOTS) * TILE;      // lse and delta of a block, two buffers
     static constexpr int BAR_OFF = STAT_OFF + 2 * 2 * 128 * 4;
     static constexpr int SMEM = BAR_OFF + 512 + 1024;
-    static constexpr int THREADS = 256 + 64;
+    static constexpr int THREADS = BWD_WG * 128 + 64;
     static constexpr int ACC = 256, TMEM_COLS = 512;
 };
 
 template <int DP, bool KV, int DT>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(BWD_WG * 128 + 64, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2,
                 const __grid_constant__ CUtensorMap my1, const __grid_constant__ CUtensorMap my2,
                 const Params p) {
@@ -460,7 +486,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    constexpr int W_LOAD = 8, W_MMA = 9;
+    constexpr int W_LOAD = BWD_WG * 4, W_MMA = W_LOAD + 1, CW = BWD_COLS;
     const int rep = p.H / p.Hkv, heads = KV ? p.Hkv : p.H;
     // causal: heads fastest and the tiles with the longest rows (first columns) first
     const int tiles = ((KV ? p.Sk : p.Sq) + 127) / 128, bhs = p.B * heads;
@@ -485,7 +511,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     const int nblk = KV ? per * rep : per;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 8; ++i) mbar_init(bars + i, i == 3 || i == 4 || i == 5 ? 256 : 1);
+        for (int i = 0; i < 8; ++i) mbar_init(bars + i, i == 3 || i == 4 || i == 5 ? BWD_WG * 128 : 1);
         for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -531,14 +557,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             auto tile = [&](int i) { return y + (i % Cf::SLOTS) * Cf::TILE; };
             auto wait_y = [&](int i) { return mbar_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
             auto score = [&](uint32_t d, uint32_t x, int i, uint32_t id, uint64_t* bar) {
-                for (int k = 0; k < ks; ++k) tc_mma(tmem + d, desc_k(x, k), desc_k(tile(i), k), id, k > 0);
+                product_k<DP>(tmem + d, x, tile(i), id, ks);
                 tc_commit(bar);
             };
-            // the 128-long product over the rows of Y: the left operand's columns 0..63 are the 32
-            // words at `a`, columns 64..127 the 32 words at `a` + 64
             auto accumulate = [&](uint32_t d, uint32_t a, int i, bool more) {
-                for (int k = 0; k < 8; ++k)
-                    tc_mma_ts(tmem + d, tmem + a + (k / 4) * 64 + (k % 4) * 8, desc_mn(tile(i), k), id_acc, more || k > 0);
+                product_mn<CW>(tmem + d, tmem + a, tile(i), id_acc, more);
             };
             bool ok = mbar_wait(x_full, 0, abort_flag) && wait_y(0);
             if (ok) { tc_fence_after(); score(0, x1, 0, id_s, s_full); ok = wait_y(1); }
@@ -580,7 +603,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         const int w = warp / 4, row = (warp % 4) * 32 + lane, tid = threadIdx.x;
         const int r = r0 + row;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;
-        const uint32_t s_addr = tmem + lanes + w * 64, dp_addr = s_addr + 128;
+        const uint32_t s_addr = tmem + lanes + w * CW, dp_addr = s_addr + 128;
         constexpr float LOG2E = 1.4426950408889634f;
         bool ok = true;
         float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's -lse * log2(e) and -scale * delta
@@ -594,10 +617,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             row_hi = r < ql ? kl : 0;
             if (p.causal) row_hi = min(row_hi, r + kl - ql + 1);
             float d = 0.f;
-            if (row_hi > 0) {                 // half of dO . O, 8 elements at a time
+            if (row_hi > 0) {                 // a part of dO . O, 8 elements at a time
                 const auto* go = attn::row<DT>(p.dout, b, r, hx);
                 const auto* o = attn::row<DT>(p.o, b, r, hx);
-                for (int c = w; c < p.D / 8; c += 2) {
+                for (int c = w; c < p.D / 8; c += BWD_WG) {
                     const uint4 u = reinterpret_cast<const uint4*>(go)[c], v = reinterpret_cast<const uint4*>(o)[c];
                     const auto* a2 = reinterpret_cast<const typename Half16<DT>::T2*>(&u);
                     const auto* b2 = reinterpret_cast<const typename Half16<DT>::T2*>(&v);
@@ -612,7 +635,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             stat[tid] = d;
             mbar_arrive(stat_ready);
             ok = __all_sync(~0u, mbar_wait(stat_ready, 0, abort_flag));
-            ds0 = -(stat[row] + stat[row + 128]) * p.scale;
+            for (int x = 0; x < BWD_WG; ++x) ds0 += stat[row + x * 128];
+            ds0 *= -p.scale;
             if (ok && w == 0 && r < p.Sq) p.delta[((long long)b * p.H + hx) * p.Sq + r] = ds0;
         }
         // KV: thread tid fetches lse (tid < 128) or delta of one query of the next block
@@ -622,55 +646,54 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const long long at = ((long long)b * p.H + hy0 + blk / per) * p.Sq + i;
             return tid < 128 ? -p.lse[at] * LOG2E : p.delta[at];
         };
-        float next = KV && nblk > 0 ? fetch(0) : 0.f;
+        float next = KV && nblk > 0 && tid < 256 ? fetch(0) : 0.f;
         for (int i = 0; ok && i < nblk; ++i) {
             const int y0 = (first + i % per) * 128;
-            const float *c_lse = stat + (i & 1) * 256 + w * 64, *c_ds = c_lse + 128;
+            const float *c_lse = stat + (i & 1) * 256 + w * CW, *c_ds = c_lse + 128;
             if (KV) {
-                stat[(i & 1) * 256 + tid] = next;
+                if (tid < 256) stat[(i & 1) * 256 + tid] = next;
                 mbar_arrive(stat_ready);
-                if (i + 1 < nblk) next = fetch(i + 1);
+                if (i + 1 < nblk && tid < 256) next = fetch(i + 1);
                 ok = __all_sync(~0u, mbar_wait(stat_ready, i & 1, abort_flag));
                 if (!ok) break;
             }
             ok = __all_sync(~0u, mbar_wait(s_full, i & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            uint32_t pv[64];
+            uint32_t pv[CW];
             tmem_ld32_issue(s_addr, pv);
-            tmem_ld32_issue(s_addr + 32, pv + 32);
-            tmem_ld_wait<64>(pv);
+            tmem_ld_wait<CW>(pv);
             float* pr = reinterpret_cast<float*>(pv);
             if (!KV) {                        // S may be overwritten: P stays in registers
                 tc_fence_before();
                 mbar_arrive(p_ready);
             }
-            const int lo = row_lo - y0 - w * 64, hi = row_hi - y0 - w * 64;
-            const bool mask = __any_sync(~0u, lo > 0 || hi < 64);
+            const int lo = row_lo - y0 - w * CW, hi = row_hi - y0 - w * CW;
+            const bool mask = __any_sync(~0u, lo > 0 || hi < CW);
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-                const F2 sub = KV ? F2{c_lse[c], c_lse[c + 1]} : F2{lse2, lse2};
+            for (int c = 0; c < CW; c += 2) {
+                const F2 sub = KV ? *reinterpret_cast<const F2*>(c_lse + c) : F2{lse2, lse2};
                 const F2 e = fma2({pr[c], pr[c + 1]}, {p.scale2, p.scale2}, sub);
                 pr[c] = ex2(e.x);
                 pr[c + 1] = ex2(e.y);
             }
             if (mask) {
 #pragma unroll
-                for (int c = 0; c < 64; ++c) pr[c] = c >= lo && c < hi ? pr[c] : 0.f;
+                for (int c = 0; c < CW; ++c) pr[c] = c >= lo && c < hi ? pr[c] : 0.f;
             }
             // streamed rows past the sequence's length may hold anything
             const int y_end = KV ? ql : kl;
-            if (y_end - y0 < 128) {
+            if (w < 2 && y_end - y0 < 128) {
                 const int iy = 2 * i + w;
                 ok = __all_sync(~0u, mbar_wait(full + iy % Cf::SLOTS, (iy / Cf::SLOTS) & 1, abort_flag));
                 if (!ok) break;
                 zero_tail<DP>(smem + (2 + iy % Cf::SLOTS) * Cf::TILE, y_end - y0, row);
             }
             if (KV) {
-                uint32_t pk[32];
+                uint32_t pk[CW / 2];
 #pragma unroll
-                for (int c = 0; c < 32; ++c) pk[c] = pack16<DT>(pr[2 * c], pr[2 * c + 1]);
-                tmem_st32(s_addr, pk);
+                for (int c = 0; c < CW / 2; ++c) pk[c] = pack16<DT>(pr[2 * c], pr[2 * c + 1]);
+                tmem_st16(s_addr, pk);
                 tmem_st_wait();
                 tc_fence_before();
                 mbar_arrive(p_ready);
@@ -678,25 +701,24 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             ok = __all_sync(~0u, mbar_wait(dp_full, i & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            uint32_t dv[64], dk[32];
+            uint32_t dv[CW], dk[CW / 2];
             tmem_ld32_issue(dp_addr, dv);
-            tmem_ld32_issue(dp_addr + 32, dv + 32);
-            tmem_ld_wait<64>(dv);
+            tmem_ld_wait<CW>(dv);
             float* dp = reinterpret_cast<float*>(dv);
 #pragma unroll
-            for (int c = 0; c < 64; c += 2) {
-                const F2 sub = KV ? F2{c_ds[c], c_ds[c + 1]} : F2{ds0, ds0};
+            for (int c = 0; c < CW; c += 2) {
+                const F2 sub = KV ? *reinterpret_cast<const F2*>(c_ds + c) : F2{ds0, ds0};
                 const F2 e = mul2({pr[c], pr[c + 1]}, fma2({dp[c], dp[c + 1]}, {p.scale, p.scale}, sub));
                 dp[c] = e.x;
                 dp[c + 1] = e.y;
             }
             if (mask) {                       // 0 * what a masked place holds
 #pragma unroll
-                for (int c = 0; c < 64; ++c) dp[c] = c >= lo && c < hi ? dp[c] : 0.f;
+                for (int c = 0; c < CW; ++c) dp[c] = c >= lo && c < hi ? dp[c] : 0.f;
             }
 #pragma unroll
-            for (int c = 0; c < 32; ++c) dk[c] = pack16<DT>(dp[2 * c], dp[2 * c + 1]);
-            tmem_st32(dp_addr, dk);
+            for (int c = 0; c < CW / 2; ++c) dk[c] = pack16<DT>(dp[2 * c], dp[2 * c + 1]);
+            tmem_st16(dp_addr, dk);
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(ds_ready);
@@ -707,12 +729,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             err = ERR_MATH;
         } else {
             tc_fence_after();
-            // dQ: the warpgroups take alternate 32 columns; KV: the first writes dK, the second dV
+            // the warpgroups take alternate 32 columns, the first two of dK, the others of dV for KV
             const int rows = KV ? p.Sk : p.Sq;
-            const View& view = !KV ? p.dq : w == 0 ? p.dk : p.dv;
+            const View& view = !KV ? p.dq : w < 2 ? p.dk : p.dv;
             auto* out = r < rows ? row_out<DT>(view, b, r, hx) : nullptr;
-            const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w * DP : 0);
-            for (int c = KV ? 0 : w * 32; c < p.D; c += KV ? 32 : 64) {
+            const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w / 2 * DP : 0);
+            for (int c = (KV ? w % 2 : w) * 32; c < p.D; c += KV ? 64 : 128) {
                 uint32_t o[32];
                 if (nblk > 0) {
                     tmem_ld32_issue(acc + c, o);
