@@ -40,22 +40,44 @@ __device__ __forceinline__ int len_of(const int* lens, int b, int most) {
 // are issued by one thread, so each takes few instructions: the descriptors of a tile's steps are
 // its first one plus constants.
 constexpr uint32_t DESC_HI = (1024u >> 4) | (1u << 14) | (LAYOUT_SW128 << 29);
+// The whole warp runs the issuing code, so that addresses stay in uniform registers (under a
+// branch on one lane each product cost about 85 clocks of register moves); `leader` is 1 in the one
+// lane whose instruction takes effect.
 template <bool ACC>
-__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
     asm volatile(
-        "{\n\t.reg .b64 a, b;\n\t.reg .pred p;\n\t"
-        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(DESC_HI), "n"(ACC ? 1 : 0));
+        "{\n\t.reg .b64 a, b;\n\t.reg .pred p, q;\n\t"
+        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(DESC_HI), "n"(ACC ? 1 : 0), "r"(leader));
 }
 // D[tmem] (+)= A[tmem] * B[smem]: A holds 16-bit pairs, one row per lane, K along the columns.
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo,
                                        uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .b64 b;\n\t.reg .pred p;\n\t"
-        "mov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
-        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(DESC_HI), "r"(accumulate));
+        "{\n\t.reg .b64 b;\n\t.reg .pred p, q;\n\t"
+        "mov.b64 b, {%2, %4};\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(DESC_HI), "r"(accumulate), "r"(leader));
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+    return one;
+}
+// a value that is the same in every lane, where the compiler can see it
+template <class V>
+__device__ __forceinline__ V uniform(V v) { return __shfl_sync(~0u, v, 0); }
+// a bounded wait of a whole warp
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+    return __all_sync(~0u, mbar_wait(bar, parity, abort_flag));
 }
 // 32 columns of this warp's lanes, without waiting: tmem_ld_wait orders the registers.
 __device__ __forceinline__ void tmem_ld32_issue(uint32_t taddr, uint32_t* v) {
@@ -157,20 +179,20 @@ __device__ __forceinline__ uint32_t desc_k(uint32_t tile) { return (tile >> 4) |
 __device__ __forceinline__ uint32_t desc_mn(uint32_t tile) { return (tile >> 4) | ((uint32_t)(PANEL >> 4) << 16); }
 // D = X Y^T over the head dimension, ks steps of 16 (X, Y: tiles of 128 rows)
 template <int DP>
-__device__ __forceinline__ void product_k(uint32_t d_tmem, uint32_t x, uint32_t y, uint32_t idesc, int ks) {
+__device__ __forceinline__ void product_k(uint32_t leader, uint32_t d_tmem, uint32_t x, uint32_t y, uint32_t idesc, int ks) {
     const uint32_t a = desc_k(x), b = desc_k(y);
-    mma_ss<false>(d_tmem, a, b, idesc);
+    mma_ss<false>(leader, d_tmem, a, b, idesc);
 #pragma unroll
     for (int k = 1; k < DP / 16; ++k)
-        if (k < ks) mma_ss<true>(d_tmem, a + (k / 4) * (PANEL >> 4) + (k % 4) * 2, b + (k / 4) * (PANEL >> 4) + (k % 4) * 2, idesc);
+        if (k < ks) mma_ss<true>(leader, d_tmem, a + (k / 4) * (PANEL >> 4) + (k % 4) * 2, b + (k / 4) * (PANEL >> 4) + (k % 4) * 2, idesc);
 }
 // D (+)= A Y over Y's 128 rows; columns CW w .. of A are the CW / 2 words at a_tmem + CW w
 template <int CW>
-__device__ __forceinline__ void product_mn(uint32_t d_tmem, uint32_t a_tmem, uint32_t y, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void product_mn(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t y, uint32_t idesc, bool accumulate) {
     const uint32_t b = desc_mn(y);
-    mma_ts(d_tmem, a_tmem, b, idesc, accumulate);
+    mma_ts(leader, d_tmem, a_tmem, b, idesc, accumulate);
 #pragma unroll
-    for (int k = 1; k < 8; ++k) mma_ts(d_tmem, a_tmem + k * 16 / CW * CW + k * 16 % CW / 2, b + k * 128, idesc, 1);
+    for (int k = 1; k < 8; ++k) mma_ts(leader, d_tmem, a_tmem + k * 16 / CW * CW + k * 16 % CW / 2, b + k * 128, idesc, 1);
 }
 template <int DP>
 __device__ __forceinline__ void load_tile(uint32_t dst_off, uint8_t* smem, const CUtensorMap* map,
@@ -232,7 +254,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     constexpr int W_LOAD = NT * 4, W_MMA = NT * 4 + 1;
     // causal: heads fastest and the longest rows first, so that the last CTAs to start are short
     const int tiles = (p.Sq + NT * 128 - 1) / (NT * 128), heads = p.B * p.H;
@@ -242,7 +264,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     const int ql = len_of(p.qlens, b, p.Sq), kl = len_of(p.kvlens, b, p.Sk);
     int end = q0 < ql ? kl : 0;
     if (p.causal) end = min(end, min(q0 + NT * 128, ql) - 1 + kl - ql + 1);
-    const int nblk = end > 0 ? (end + 127) / 128 : 0;
+    const int nblk = uniform(end > 0 ? (end + 127) / 128 : 0);
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -261,7 +283,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_holder;
+    const uint32_t tmem = uniform(*tmem_holder);
     const uint32_t kv_base = smem_u32(smem) + NT * Cf::TILE;
     unsigned int err = 0;
 
@@ -284,46 +306,46 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             }
         }
     } else if (warp == W_MMA) {
-        if (lane == 0 && nblk > 0) {
+        if (nblk > 0) {
+            const uint32_t leader = elect();
             const int ks = (p.D + 15) / 16;
             const uint32_t id_s = idesc_f16(DT == OM_DTYPE_F16, 128, false, p.neg);
             const uint32_t id_o = idesc_f16(DT == OM_DTYPE_F16, ks * 16, true, false);
             const uint32_t q_tile = smem_u32(smem);
             auto qk = [&](int t, int i) {
                 const uint32_t kt = kv_base + (i % Cf::SLOTS) * Cf::TILE;
-                product_k<DP>(tmem + t * 128, q_tile + t * Cf::TILE, kt, id_s, ks);
-                tc_commit(s_full + t);
+                product_k<DP>(leader, tmem + t * 128, q_tile + t * Cf::TILE, kt, id_s, ks);
+                commit(leader, s_full + t);
             };
-            auto wait_kv = [&](int i) { return mbar_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
-            bool ok = mbar_wait(q_full, 0, abort_flag) && wait_kv(0);
+            auto wait_kv = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
+            bool ok = warp_wait(q_full, 0, abort_flag) && wait_kv(0);
             if (ok) {
                 tc_fence_after();
                 for (int t = 0; t < NT; ++t) qk(t, 0);
-                tc_commit(empty + 0);
+                commit(leader, empty + 0);
             }
             for (int j = 0; ok && j < nblk; ++j) {
                 const bool more = j + 1 < nblk;
                 ok = wait_kv(2 * j + 1) && (!more || wait_kv(2 * j + 2));
                 const uint32_t vt = kv_base + ((2 * j + 1) % Cf::SLOTS) * Cf::TILE;
                 for (int t = 0; ok && t < NT; ++t) {
-                    ok = mbar_wait(p_full + t, j & 1, abort_flag);
+                    ok = warp_wait(p_full + t, j & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    product_mn<128>(tmem + Cf::O_COL + t * Cf::O_STEP, tmem + t * 128, vt, id_o, j > 0);
+                    product_mn<128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + t * 128, vt, id_o, j > 0);
                     if (more) qk(t, 2 * j + 2);
                 }
                 if (!ok) break;
-                tc_commit(empty + (2 * j + 1) % Cf::SLOTS);
-                tc_commit(more ? empty + (2 * j + 2) % Cf::SLOTS : o_full);
+                commit(leader, empty + (2 * j + 1) % Cf::SLOTS);
+                commit(leader, more ? empty + (2 * j + 2) % Cf::SLOTS : o_full);
             }
             if (!ok) {                    // no MMA may run on when the CTA ends
                 *abort_flag = 1;
                 err = ERR_MMA;
-                tc_commit(drain);
+                commit(leader, drain);
                 if (!mbar_wait_drain(drain, 0)) err |= ERR_DRAIN;
             }
         }
-        __syncwarp();
     } else {
         const int t = warp / 4, row = (warp % 4) * 32 + lane;
         const int i = q0 + t * 128 + row;
@@ -334,7 +356,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nblk; ++j) {
-            ok = __all_sync(~0u, mbar_wait(s_full + t, j & 1, abort_flag));
+            ok = warp_wait(s_full + t, j & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             uint32_t sv[128];
@@ -391,7 +413,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             // keys past the sequence's length may hold anything
             if (t == 0 && j == nblk - 1 && kl - j * 128 < 128) {
                 const int iv = 2 * j + 1;
-                ok = __all_sync(~0u, mbar_wait(full + iv % Cf::SLOTS, (iv / Cf::SLOTS) & 1, abort_flag));
+                ok = warp_wait(full + iv % Cf::SLOTS, (iv / Cf::SLOTS) & 1, abort_flag);
                 if (!ok) break;
                 zero_tail<DP>(smem + (NT + iv % Cf::SLOTS) * Cf::TILE, kl - j * 128, row);
             }
@@ -399,7 +421,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             tc_fence_before();
             mbar_arrive(p_full + t);
         }
-        if (ok && nblk > 0) ok = __all_sync(~0u, mbar_wait(o_full, 0, abort_flag));
+        if (ok && nblk > 0) ok = warp_wait(o_full, 0, abort_flag);
         if (!ok) {
             *abort_flag = 1;
             err = ERR_MATH;
@@ -485,7 +507,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
     constexpr int W_LOAD = BWD_WG * 4, W_MMA = W_LOAD + 1, CW = BWD_COLS;
     const int rep = p.H / p.Hkv, heads = KV ? p.Hkv : p.H;
     // causal: heads fastest and the tiles with the longest rows (first columns) first
@@ -508,7 +530,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         if (p.causal) end = min(end, min(r0 + 128, ql) + kl - ql);
         per = end > 0 ? (end + 127) / 128 : 0;
     }
-    const int nblk = KV ? per * rep : per;
+    const int nblk = uniform(KV ? per * rep : per);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) mbar_init(bars + i, i == 3 || i == 4 || i == 5 ? BWD_WG * 128 : 1);
@@ -524,7 +546,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_holder;
+    const uint32_t tmem = uniform(*tmem_holder);
     unsigned int err = 0;
 
     if (warp == W_LOAD) {
@@ -548,27 +570,28 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             }
         }
     } else if (warp == W_MMA) {
-        if (lane == 0 && nblk > 0) {
+        if (nblk > 0) {
+            const uint32_t leader = elect();
             const int ks = (p.D + 15) / 16;
             const bool f16 = DT == OM_DTYPE_F16;
             const uint32_t id_s = idesc_f16(f16, 128, false, p.neg), id_dp = idesc_f16(f16, 128, false, false);
             const uint32_t id_acc = idesc_f16(f16, ks * 16, true, false);
             const uint32_t x1 = smem_u32(smem), x2 = x1 + Cf::TILE, y = x1 + 2 * Cf::TILE;
             auto tile = [&](int i) { return y + (i % Cf::SLOTS) * Cf::TILE; };
-            auto wait_y = [&](int i) { return mbar_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
+            auto wait_y = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
             auto score = [&](uint32_t d, uint32_t x, int i, uint32_t id, uint64_t* bar) {
-                product_k<DP>(tmem + d, x, tile(i), id, ks);
-                tc_commit(bar);
+                product_k<DP>(leader, tmem + d, x, tile(i), id, ks);
+                commit(leader, bar);
             };
             auto accumulate = [&](uint32_t d, uint32_t a, int i, bool more) {
-                product_mn<CW>(tmem + d, tmem + a, tile(i), id_acc, more);
+                product_mn<CW>(leader, tmem + d, tmem + a, tile(i), id_acc, more);
             };
-            bool ok = mbar_wait(x_full, 0, abort_flag) && wait_y(0);
+            bool ok = warp_wait(x_full, 0, abort_flag) && wait_y(0);
             if (ok) { tc_fence_after(); score(0, x1, 0, id_s, s_full); ok = wait_y(1); }
             if (ok) score(128, x2, 1, id_dp, dp_full);
             for (int i = 0; ok && i < nblk; ++i) {
                 const bool more = i + 1 < nblk;
-                ok = mbar_wait(p_ready, i & 1, abort_flag);
+                ok = warp_wait(p_ready, i & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 if (KV) accumulate(Cf::ACC + DP, 0, 2 * i + 1, i > 0);
@@ -577,28 +600,27 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                     if (!ok) break;
                     score(0, x1, 2 * i + 2, id_s, s_full);
                 }
-                ok = mbar_wait(ds_ready, i & 1, abort_flag);
+                ok = warp_wait(ds_ready, i & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 accumulate(Cf::ACC, 128, 2 * i, i > 0);
-                tc_commit(empty + (2 * i) % Cf::SLOTS);
-                tc_commit(empty + (2 * i + 1) % Cf::SLOTS);
+                commit(leader, empty + (2 * i) % Cf::SLOTS);
+                commit(leader, empty + (2 * i + 1) % Cf::SLOTS);
                 if (more) {
                     ok = wait_y(2 * i + 3);
                     if (!ok) break;
                     score(128, x2, 2 * i + 3, id_dp, dp_full);
                 } else {
-                    tc_commit(acc_full);
+                    commit(leader, acc_full);
                 }
             }
             if (!ok) {                    // no MMA may run on when the CTA ends
                 *abort_flag = 1;
                 err = ERR_MMA;
-                tc_commit(drain);
+                commit(leader, drain);
                 if (!mbar_wait_drain(drain, 0)) err |= ERR_DRAIN;
             }
         }
-        __syncwarp();
     } else {
         const int w = warp / 4, row = (warp % 4) * 32 + lane, tid = threadIdx.x;
         const int r = r0 + row;
@@ -634,7 +656,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             }
             stat[tid] = d;
             mbar_arrive(stat_ready);
-            ok = __all_sync(~0u, mbar_wait(stat_ready, 0, abort_flag));
+            ok = warp_wait(stat_ready, 0, abort_flag);
             for (int x = 0; x < BWD_WG; ++x) ds0 += stat[row + x * 128];
             ds0 *= -p.scale;
             if (ok && w == 0 && r < p.Sq) p.delta[((long long)b * p.H + hx) * p.Sq + r] = ds0;
@@ -654,10 +676,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 if (tid < 256) stat[(i & 1) * 256 + tid] = next;
                 mbar_arrive(stat_ready);
                 if (i + 1 < nblk && tid < 256) next = fetch(i + 1);
-                ok = __all_sync(~0u, mbar_wait(stat_ready, i & 1, abort_flag));
+                ok = warp_wait(stat_ready, i & 1, abort_flag);
                 if (!ok) break;
             }
-            ok = __all_sync(~0u, mbar_wait(s_full, i & 1, abort_flag));
+            ok = warp_wait(s_full, i & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             uint32_t pv[CW];
@@ -685,7 +707,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const int y_end = KV ? ql : kl;
             if (w < 2 && y_end - y0 < 128) {
                 const int iy = 2 * i + w;
-                ok = __all_sync(~0u, mbar_wait(full + iy % Cf::SLOTS, (iy / Cf::SLOTS) & 1, abort_flag));
+                ok = warp_wait(full + iy % Cf::SLOTS, (iy / Cf::SLOTS) & 1, abort_flag);
                 if (!ok) break;
                 zero_tail<DP>(smem + (2 + iy % Cf::SLOTS) * Cf::TILE, y_end - y0, row);
             }
@@ -698,7 +720,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 tc_fence_before();
                 mbar_arrive(p_ready);
             }
-            ok = __all_sync(~0u, mbar_wait(dp_full, i & 1, abort_flag));
+            ok = warp_wait(dp_full, i & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             uint32_t dv[CW], dk[CW / 2];
@@ -723,7 +745,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             tc_fence_before();
             mbar_arrive(ds_ready);
         }
-        if (ok && nblk > 0) ok = __all_sync(~0u, mbar_wait(acc_full, 0, abort_flag));
+        if (ok && nblk > 0) ok = warp_wait(acc_full, 0, abort_flag);
         if (!ok) {
             *abort_flag = 1;
             err = ERR_MATH;
