@@ -14,7 +14,7 @@ struct View {          // a [batch, token, head, D] tensor: element strides, D c
 struct Params {
     View q, k, v, o, dout, dq, dk, dv;
     float* lse;        // [B, H, Sq]
-    float* delta;      // [B, H, Sq], -scale times the row sums of dO o O
+    float* stat;       // the backward's workspace: see stat_tile
     const int *qlens, *kvlens;
     int B, H, Hkv, Sq, Sk, D, causal;
     float scale;
@@ -479,15 +479,29 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 // scheduler had two warps to hide the TMEM and exponential latencies behind).
 // TMEM: S at 0, dP at 128 (P and dS over the first half of each 32 columns), accumulators behind.
 constexpr int BWD_WG = 4, BWD_COLS = 128 / BWD_WG;
+// What the dQ kernel leaves of a tile of 128 queries for the KV kernel, in the workspace as
+// [batch][head][tile]: 128 times -log2(e) lse, 128 times -scale delta.
+constexpr int STAT_TILE = 256;
+__device__ __forceinline__ float* stat_tile(const Params& p, int b, int h, int tile) {
+    return p.stat + (((long long)b * p.H + h) * ((p.Sq + 127) / 128) + tile) * STAT_TILE;
+}
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                     smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+}
+constexpr int max_of(int a, int b) { return a > b ? a : b; }
 template <int DP>
 struct BwdCfg {
     static constexpr int TILE = DP / 64 * PANEL;
     static constexpr int SLOTS = DP == 128 ? 4 : 8;
-    static constexpr int STAT_OFF = (2 + SLOTS) * TILE;      // lse and delta of a block, two buffers
-    static constexpr int BAR_OFF = STAT_OFF + 2 * 2 * 128 * 4;
+    static constexpr int STAT_OFF = (2 + SLOTS) * TILE;      // a block's STAT_TILE per pair of slots
+    static constexpr int BAR_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT_TILE, BWD_WG * 128) * 4;
     static constexpr int SMEM = BAR_OFF + 512 + 1024;
     static constexpr int THREADS = BWD_WG * 128 + 64;
-    static constexpr int ACC = 256, TMEM_COLS = 512;
+    // with heads up to 64 there is room for two S tiles: the next block's scores are ready before
+    // this block's probabilities are taken
+    static constexpr int NS = DP == 64 ? 2 : 1;
+    static constexpr int DP_COL = NS * 128, ACC = DP_COL + 128, TMEM_COLS = 512;
 };
 
 template <int DP, bool KV, int DT>
@@ -500,9 +514,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* stat = reinterpret_cast<float*>(smem + Cf::STAT_OFF);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BAR_OFF);
-    uint64_t *x_full = bars, *s_full = bars + 1, *dp_full = bars + 2, *p_ready = bars + 3, *ds_ready = bars + 4,
-             *stat_ready = bars + 5, *acc_full = bars + 6, *drain = bars + 7;
-    uint64_t* full = bars + 8;
+    // s_full and p_ready: one per S tile, as the warpgroups may be a block ahead of the MMA warp
+    uint64_t *x_full = bars, *s_full = bars + 1, *dp_full = bars + 3, *p_ready = bars + 4, *ds_ready = bars + 6,
+             *stat_ready = bars + 7, *acc_full = bars + 8, *drain = bars + 9;
+    uint64_t* full = bars + 10;
     uint64_t* empty = full + Cf::SLOTS;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -533,7 +548,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     const int nblk = uniform(KV ? per * rep : per);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 8; ++i) mbar_init(bars + i, i == 3 || i == 4 || i == 5 ? BWD_WG * 128 : 1);
+        for (int i = 0; i < 10; ++i) mbar_init(bars + i, i >= 4 && i <= 7 ? BWD_WG * 128 : 1);
         for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -554,13 +569,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             mbar_expect_tx(x_full, 2 * Cf::TILE);
             load_tile<DP>(0, smem, &mx1, x_full, r0, hx, b);
             load_tile<DP>(Cf::TILE, smem, &mx2, x_full, r0, hx, b);
-            int i = 0;
-            for (; i < 2 * nblk; ++i) {   // Y1, Y2 of each block in turn
-                const int slot = i % Cf::SLOTS, blk = i / 2;
+            int i = 0, y = first, hy = hy0;
+            for (; i < 2 * nblk; ++i) {   // Y1 (KV: and its queries' statistics), Y2 of each block in turn
+                const int slot = i % Cf::SLOTS;
                 if (!mbar_wait(empty + slot, ((i / Cf::SLOTS) & 1) ^ 1, abort_flag)) { err = ERR_LOAD; break; }
-                mbar_expect_tx(full + slot, Cf::TILE);
-                load_tile<DP>((2 + slot) * Cf::TILE, smem, i & 1 ? &my2 : &my1, full + slot,
-                              (first + blk % per) * 128, hy0 + blk / per, b);
+                mbar_expect_tx(full + slot, Cf::TILE + (KV && !(i & 1) ? STAT_TILE * 4 : 0));
+                if (KV && !(i & 1))
+                    bulk_load(stat + slot / 2 * STAT_TILE, stat_tile(p, b, hy, y), STAT_TILE * 4, full + slot);
+                load_tile<DP>((2 + slot) * Cf::TILE, smem, i & 1 ? &my2 : &my1, full + slot, y * 128, hy, b);
+                if (i & 1 && ++y == first + per) { y = first; ++hy; }
             }
             if (err || *abort_flag) {     // every load issued has to land before the CTA ends
                 *abort_flag = 1;
@@ -586,30 +603,37 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             auto accumulate = [&](uint32_t d, uint32_t a, int i, bool more) {
                 product_mn<CW>(leader, tmem + d, tmem + a, tile(i), id_acc, more);
             };
-            bool ok = warp_wait(x_full, 0, abort_flag) && wait_y(0);
-            if (ok) { tc_fence_after(); score(0, x1, 0, id_s, s_full); ok = wait_y(1); }
-            if (ok) score(128, x2, 1, id_dp, dp_full);
-            for (int i = 0; ok && i < nblk; ++i) {
-                const bool more = i + 1 < nblk;
-                ok = warp_wait(p_ready, i & 1, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                if (KV) accumulate(Cf::ACC + DP, 0, 2 * i + 1, i > 0);
-                if (more) {
-                    ok = wait_y(2 * i + 2);
-                    if (!ok) break;
-                    score(0, x1, 2 * i + 2, id_s, s_full);
+            auto scores = [&](int i) {    // S of block i, whose Y1 has to be there
+                const bool ok = wait_y(2 * i);
+                if (ok) {
+                    tc_fence_after();
+                    score(i % Cf::NS * 128, x1, 2 * i, id_s, s_full + i % Cf::NS);
                 }
-                ok = warp_wait(ds_ready, i & 1, abort_flag);
+                return ok;
+            };
+            bool ok = warp_wait(x_full, 0, abort_flag) && scores(0) && wait_y(1);
+            if (ok) {
+                score(Cf::DP_COL, x2, 1, id_dp, dp_full);
+                if (Cf::NS == 2 && nblk > 1) ok = scores(1);
+            }
+            for (int i = 0; ok && i < nblk; ++i) {
+                // products run in the order of their issue: S of block i + NS may overwrite P of
+                // block i right behind the product that reads it
+                ok = warp_wait(p_ready + i % Cf::NS, i / Cf::NS & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                accumulate(Cf::ACC, 128, 2 * i, i > 0);
+                if (KV) accumulate(Cf::ACC + DP, i % Cf::NS * 128, 2 * i + 1, i > 0);
+                if (i + Cf::NS < nblk) ok = scores(i + Cf::NS);
+                ok = ok && warp_wait(ds_ready, i & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                accumulate(Cf::ACC, Cf::DP_COL, 2 * i, i > 0);
                 commit(leader, empty + (2 * i) % Cf::SLOTS);
                 commit(leader, empty + (2 * i + 1) % Cf::SLOTS);
-                if (more) {
+                if (i + 1 < nblk) {
                     ok = wait_y(2 * i + 3);
                     if (!ok) break;
-                    score(128, x2, 2 * i + 3, id_dp, dp_full);
+                    score(Cf::DP_COL, x2, 2 * i + 3, id_dp, dp_full);
                 } else {
                     commit(leader, acc_full);
                 }
@@ -625,7 +649,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         const int w = warp / 4, row = (warp % 4) * 32 + lane, tid = threadIdx.x;
         const int r = r0 + row;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;
-        const uint32_t s_addr = tmem + lanes + w * CW, dp_addr = s_addr + 128;
+        const uint32_t s_base = tmem + lanes + w * CW, dp_addr = s_base + Cf::DP_COL;
         constexpr float LOG2E = 1.4426950408889634f;
         bool ok = true;
         float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's -lse * log2(e) and -scale * delta
@@ -659,27 +683,21 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             ok = warp_wait(stat_ready, 0, abort_flag);
             for (int x = 0; x < BWD_WG; ++x) ds0 += stat[row + x * 128];
             ds0 *= -p.scale;
-            if (ok && w == 0 && r < p.Sq) p.delta[((long long)b * p.H + hx) * p.Sq + r] = ds0;
+            if (ok && w == 0) {           // for the KV kernel
+                float* out = stat_tile(p, b, hx, r0 / 128) + row;
+                out[0] = lse2;
+                out[128] = ds0;
+            }
         }
-        // KV: thread tid fetches lse (tid < 128) or delta of one query of the next block
-        auto fetch = [&](int blk) {
-            const int i = (first + blk % per) * 128 + tid % 128;
-            if (i >= ql) return 0.f;
-            const long long at = ((long long)b * p.H + hy0 + blk / per) * p.Sq + i;
-            return tid < 128 ? -p.lse[at] * LOG2E : p.delta[at];
-        };
-        float next = KV && nblk > 0 && tid < 256 ? fetch(0) : 0.f;
+        int y0 = first * 128;
         for (int i = 0; ok && i < nblk; ++i) {
-            const int y0 = (first + i % per) * 128;
-            const float *c_lse = stat + (i & 1) * 256 + w * CW, *c_ds = c_lse + 128;
-            if (KV) {
-                if (tid < 256) stat[(i & 1) * 256 + tid] = next;
-                mbar_arrive(stat_ready);
-                if (i + 1 < nblk && tid < 256) next = fetch(i + 1);
-                ok = warp_wait(stat_ready, i & 1, abort_flag);
+            const float *c_lse = stat + i % (Cf::SLOTS / 2) * STAT_TILE + w * CW, *c_ds = c_lse + 128;
+            const uint32_t s_addr = s_base + i % Cf::NS * 128;
+            if (KV) {                     // the block's statistics came with Y1
+                ok = warp_wait(full + 2 * i % Cf::SLOTS, (2 * i / Cf::SLOTS) & 1, abort_flag);
                 if (!ok) break;
             }
-            ok = warp_wait(s_full, i & 1, abort_flag);
+            ok = warp_wait(s_full + i % Cf::NS, i / Cf::NS & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             uint32_t pv[CW];
@@ -688,7 +706,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             float* pr = reinterpret_cast<float*>(pv);
             if (!KV) {                        // S may be overwritten: P stays in registers
                 tc_fence_before();
-                mbar_arrive(p_ready);
+                mbar_arrive(p_ready + i % Cf::NS);
             }
             const int lo = row_lo - y0 - w * CW, hi = row_hi - y0 - w * CW;
             const bool mask = __any_sync(~0u, lo > 0 || hi < CW);
@@ -718,7 +736,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 tmem_st16(s_addr, pk);
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(p_ready);
+                mbar_arrive(p_ready + i % Cf::NS);
             }
             ok = warp_wait(dp_full, i & 1, abort_flag);
             if (!ok) break;
@@ -744,6 +762,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(ds_ready);
+            y0 += 128;
+            if (KV && y0 == (first + per) * 128) y0 = first * 128;
         }
         if (ok && nblk > 0) ok = warp_wait(acc_full, 0, abort_flag);
         if (!ok) {
@@ -895,7 +915,7 @@ extern "C" long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int n
                                                    int nSk, int nHeadDim, int bBackward) {
     const int st = attn::check_sizes(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim);
     if (st != OM_OK) return st;
-    return bBackward ? (long long)nBatch * nHeads * nSq * 4 : 0;
+    return bBackward ? (long long)nBatch * nHeads * ((nSq + 127) / 128) * attn::STAT_TILE * 4 : 0;
 }
 
 extern "C" int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut,
@@ -947,7 +967,7 @@ extern "C" int omCudaAttentionBackward(const void* pGradOut, const void* pQ, con
     if (nBatch == 0) return OM_OK;
     if (nSq > 0 && (!pLse || !pWorkspace || reinterpret_cast<uintptr_t>(pWorkspace) % 16))
         return OM_ERR_INVALID;
-    p.lse = const_cast<float*>(pLse); p.delta = static_cast<float*>(pWorkspace);
+    p.lse = const_cast<float*>(pLse); p.stat = static_cast<float*>(pWorkspace);
     p.qlens = pQLens; p.kvlens = pKvLens;
     p.B = nBatch; p.H = nHeads; p.Hkv = nKvHeads; p.Sq = nSq; p.Sk = nSk; p.D = nHeadDim;
     p.causal = bCausal != 0; p.err = c->err_word;
