@@ -72,9 +72,14 @@ __device__ __forceinline__ uint32_t elect() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
     return one;
 }
-// a value that is the same in every lane, where the compiler can see it
-template <class V>
-__device__ __forceinline__ V uniform(V v) { return __shfl_sync(~0u, v, 0); }
+// a value that is the same in every lane, in a uniform register (the warp reduction writes one)
+__device__ __forceinline__ int uniform(int v) { return __reduce_max_sync(~0u, v); }
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(~0u, v); }
+// one arrival for the whole warp, behind what its lanes have done
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) mbar_arrive(bar);
+}
 // a bounded wait of a whole warp
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
     return __all_sync(~0u, mbar_wait(bar, parity, abort_flag));
@@ -174,43 +179,46 @@ __device__ __forceinline__ uint32_t idesc_f16(bool f16, int n, bool b_mn, bool n
 constexpr int PANEL = 128 * 128;
 // Low descriptor words. K-major operand (rows = M or N, K = the head dimension): 16 columns are 32
 // bytes, 64 a panel. MN-major operand (rows = K, N = the head dimension): 16 rows are 2048 bytes,
-// panels of 64 columns PANEL apart.
+// panels of 64 columns as far apart as they are long.
 __device__ __forceinline__ uint32_t desc_k(uint32_t tile) { return (tile >> 4) | (1u << 16); }
-__device__ __forceinline__ uint32_t desc_mn(uint32_t tile) { return (tile >> 4) | ((uint32_t)(PANEL >> 4) << 16); }
-// D = X Y^T over the head dimension, ks steps of 16 (X, Y: tiles of 128 rows)
-template <int DP>
+__device__ __forceinline__ uint32_t desc_mn(uint32_t tile, int panel) { return (tile >> 4) | ((uint32_t)(panel >> 4) << 16); }
+// D = X Y^T over the head dimension, ks steps of 16 (X: a tile of 128 rows, Y: of ROWS)
+template <int DP, int ROWS>
 __device__ __forceinline__ void product_k(uint32_t leader, uint32_t d_tmem, uint32_t x, uint32_t y, uint32_t idesc, int ks) {
     const uint32_t a = desc_k(x), b = desc_k(y);
     mma_ss<false>(leader, d_tmem, a, b, idesc);
 #pragma unroll
     for (int k = 1; k < DP / 16; ++k)
-        if (k < ks) mma_ss<true>(leader, d_tmem, a + (k / 4) * (PANEL >> 4) + (k % 4) * 2, b + (k / 4) * (PANEL >> 4) + (k % 4) * 2, idesc);
+        if (k < ks)
+            mma_ss<true>(leader, d_tmem, a + (k / 4) * (PANEL >> 4) + (k % 4) * 2,
+                         b + (k / 4) * (ROWS * 128 >> 4) + (k % 4) * 2, idesc);
 }
-// D (+)= A Y over Y's 128 rows; columns CW w .. of A are the CW / 2 words at a_tmem + CW w
-template <int CW>
+// D (+)= A Y over Y's ROWS rows; columns CW w .. of A are the CW / 2 words at a_tmem + CW w
+template <int CW, int ROWS>
 __device__ __forceinline__ void product_mn(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint32_t y, uint32_t idesc, bool accumulate) {
-    const uint32_t b = desc_mn(y);
+    const uint32_t b = desc_mn(y, ROWS * 128);
     mma_ts(leader, d_tmem, a_tmem, b, idesc, accumulate);
 #pragma unroll
-    for (int k = 1; k < 8; ++k) mma_ts(leader, d_tmem, a_tmem + k * 16 / CW * CW + k * 16 % CW / 2, b + k * 128, idesc, 1);
+    for (int k = 1; k < ROWS / 16; ++k)
+        mma_ts(leader, d_tmem, a_tmem + k * 16 / CW * CW + k * 16 % CW / 2, b + k * 128, idesc, 1);
 }
-template <int DP>
+template <int DP, int ROWS = 128>
 __device__ __forceinline__ void load_tile(uint32_t dst_off, uint8_t* smem, const CUtensorMap* map,
                                           uint64_t* bar, int t0, int h, int b) {
 #pragma unroll
     for (int c = 0; c < DP / 64; ++c)
-        tma_load_4d(smem + dst_off + c * PANEL, map, bar, c * 64, t0, h, b);
+        tma_load_4d(smem + dst_off + c * ROWS * 128, map, bar, c * 64, t0, h, b);
 }
-// Rows [first, 128) of a tile become zeros: what lies past a sequence's length must not reach a
+// Rows [first, ROWS) of a tile become zeros: what lies past a sequence's length must not reach a
 // product, since 0 * NaN is NaN. One thread per row.
-template <int DP>
+template <int DP, int ROWS = 128>
 __device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int row) {
-    if (row >= first) {
+    if (row >= first && row < ROWS) {
 #pragma unroll
         for (int c = 0; c < DP / 64; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-                reinterpret_cast<uint4*>(tile + c * PANEL + row * 128)[i] = make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(tile + c * ROWS * 128 + row * 128)[i] = make_uint4(0, 0, 0, 0);
     }
     fence_async_smem();
 }
@@ -270,7 +278,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         mbar_init(q_full, 1);
         mbar_init(o_full, 1);
         mbar_init(drain, 1);
-        for (int t = 0; t < NT; ++t) { mbar_init(s_full + t, 1); mbar_init(p_full + t, 128); }
+        for (int t = 0; t < NT; ++t) { mbar_init(s_full + t, 1); mbar_init(p_full + t, 4); }
         for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -314,7 +322,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             const uint32_t q_tile = smem_u32(smem);
             auto qk = [&](int t, int i) {
                 const uint32_t kt = kv_base + (i % Cf::SLOTS) * Cf::TILE;
-                product_k<DP>(leader, tmem + t * 128, q_tile + t * Cf::TILE, kt, id_s, ks);
+                product_k<DP, 128>(leader, tmem + t * 128, q_tile + t * Cf::TILE, kt, id_s, ks);
                 commit(leader, s_full + t);
             };
             auto wait_kv = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
@@ -332,7 +340,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     ok = warp_wait(p_full + t, j & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
-                    product_mn<128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + t * 128, vt, id_o, j > 0);
+                    product_mn<128, 128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + t * 128, vt, id_o, j > 0);
                     if (more) qk(t, 2 * j + 2);
                 }
                 if (!ok) break;
@@ -419,7 +427,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             }
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(p_full + t);
+            warp_arrive(p_full + t);
         }
         if (ok && nblk > 0) ok = warp_wait(o_full, 0, abort_flag);
         if (!ok) {
@@ -475,15 +483,18 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 // operands of the first products and as MN-major operands of the others. dQ and dK, dV are
 // summed in two passes that each recompute S (7 products instead of 5): every sum is kept in one
 // CTA's TMEM, so no fp32 gradient is accumulated in memory by atomics and results are repeatable.
-// Four warpgroups share the tile: warpgroup w has columns 32 w .. 32 w + 31 (with two, each
-// scheduler had two warps to hide the TMEM and exponential latencies behind).
-// TMEM: S at 0, dP at 128 (P and dS over the first half of each 32 columns), accumulators behind.
-constexpr int BWD_WG = 4, BWD_COLS = 128 / BWD_WG;
-// What the dQ kernel leaves of a tile of 128 queries for the KV kernel, in the workspace as
-// [batch][head][tile]: 128 times -log2(e) lse, 128 times -scale delta.
-constexpr int STAT_TILE = 256;
+// BN: streamed rows of a block; BN / 32 warpgroups share its tile, warpgroup w has columns 32 w ..
+// Heads up to 64: BN 64 and two CTAs on an SM, so that one's products run while the other's warps
+// wait, and one's exponentials beside the other's dS (one CTA with BN 128: 464 us for 2 x 12 heads
+// of 4096 tokens, its MMA warp idle between a block's barriers). Longer heads fill TMEM: BN 128.
+// TMEM: S at 0, dP at BN (P and dS over the first half of each 32 columns), accumulators behind.
+constexpr int BWD_COLS = 32;
+// What the dQ kernel leaves of 64 queries for the KV kernel, in the workspace as
+// [batch][head][64 queries]: 64 times -log2(e) lse, 64 times -scale delta.
+constexpr int STAT_TILE = 128;
+__host__ __device__ constexpr int stat_tiles(int nSq) { return (nSq + 127) / 128 * 2; }
 __device__ __forceinline__ float* stat_tile(const Params& p, int b, int h, int tile) {
-    return p.stat + (((long long)b * p.H + h) * ((p.Sq + 127) / 128) + tile) * STAT_TILE;
+    return p.stat + (((long long)b * p.H + h) * stat_tiles(p.Sq) + tile) * STAT_TILE;
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -492,20 +503,21 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 template <int DP>
 struct BwdCfg {
-    static constexpr int TILE = DP / 64 * PANEL;
-    static constexpr int SLOTS = DP == 128 ? 4 : 8;
-    static constexpr int STAT_OFF = (2 + SLOTS) * TILE;      // a block's STAT_TILE per pair of slots
-    static constexpr int BAR_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT_TILE, BWD_WG * 128) * 4;
+    static constexpr int BN = DP == 64 ? 64 : 128, OCC = DP == 64 ? 2 : 1;
+    static constexpr int WG = BN / BWD_COLS, THREADS = WG * 128 + 64;
+    static constexpr int TILE = DP / 64 * PANEL, Y_TILE = DP / 64 * BN * 128;
+    static constexpr int SLOTS = DP == 64 ? 8 : 4;
+    static constexpr int Y_OFF = 2 * TILE;
+    static constexpr int STAT = BN / 64 * STAT_TILE;         // statistics of a block, per pair of slots
+    static constexpr int STAT_OFF = Y_OFF + SLOTS * Y_TILE;
+    static constexpr int BAR_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT, WG * 128) * 4;
     static constexpr int SMEM = BAR_OFF + 512 + 1024;
-    static constexpr int THREADS = BWD_WG * 128 + 64;
-    // with heads up to 64 there is room for two S tiles: the next block's scores are ready before
-    // this block's probabilities are taken
-    static constexpr int NS = DP == 64 ? 2 : 1;
-    static constexpr int DP_COL = NS * 128, ACC = DP_COL + 128, TMEM_COLS = 512;
+    static constexpr int DP_COL = BN, ACC = 2 * BN, TMEM_COLS = 2 * BN + 2 * DP;
+    static_assert(TMEM_COLS * OCC <= 512 && SMEM * OCC <= 227 * 1024, "on-chip memory");
 };
 
 template <int DP, bool KV, int DT>
-__global__ void __launch_bounds__(BWD_WG * 128 + 64, 1)
+__global__ void __launch_bounds__(BwdCfg<DP>::THREADS, BwdCfg<DP>::OCC)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2,
                 const __grid_constant__ CUtensorMap my1, const __grid_constant__ CUtensorMap my2,
                 const Params p) {
@@ -514,16 +526,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* stat = reinterpret_cast<float*>(smem + Cf::STAT_OFF);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BAR_OFF);
-    // s_full and p_ready: one per S tile, as the warpgroups may be a block ahead of the MMA warp
-    uint64_t *x_full = bars, *s_full = bars + 1, *dp_full = bars + 3, *p_ready = bars + 4, *ds_ready = bars + 6,
-             *stat_ready = bars + 7, *acc_full = bars + 8, *drain = bars + 9;
-    uint64_t* full = bars + 10;
+    uint64_t *x_full = bars, *s_full = bars + 1, *dp_full = bars + 2, *acc_full = bars + 3, *drain = bars + 4,
+             *p_ready = bars + 5, *ds_ready = bars + 6, *stat_ready = bars + 7;
+    uint64_t* full = bars + 8;
     uint64_t* empty = full + Cf::SLOTS;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
     const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
-    constexpr int W_LOAD = BWD_WG * 4, W_MMA = W_LOAD + 1, CW = BWD_COLS;
+    constexpr int W_LOAD = Cf::WG * 4, W_MMA = W_LOAD + 1, CW = BWD_COLS, BN = Cf::BN;
     const int rep = p.H / p.Hkv, heads = KV ? p.Hkv : p.H;
     // causal: heads fastest and the tiles with the longest rows (first columns) first
     const int tiles = ((KV ? p.Sk : p.Sq) + 127) / 128, bhs = p.B * heads;
@@ -537,18 +548,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     int first = 0, per = 0;
     if (KV) {
         if (r0 < kl) {
-            first = p.causal ? max(0, r0 - (kl - ql)) / 128 : 0;
-            per = max(0, (ql + 127) / 128 - first);
+            first = p.causal ? max(0, r0 - (kl - ql)) / BN : 0;
+            per = max(0, (ql + BN - 1) / BN - first);
         }
     } else {
         int end = r0 < ql ? kl : 0;
         if (p.causal) end = min(end, min(r0 + 128, ql) + kl - ql);
-        per = end > 0 ? (end + 127) / 128 : 0;
+        per = end > 0 ? (end + BN - 1) / BN : 0;
     }
     const int nblk = uniform(KV ? per * rep : per);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 10; ++i) mbar_init(bars + i, i >= 4 && i <= 7 ? BWD_WG * 128 : 1);
+        for (int i = 0; i < 8; ++i) mbar_init(bars + i, i < 5 ? 1 : Cf::WG * 4);
         for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -573,10 +584,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             for (; i < 2 * nblk; ++i) {   // Y1 (KV: and its queries' statistics), Y2 of each block in turn
                 const int slot = i % Cf::SLOTS;
                 if (!mbar_wait(empty + slot, ((i / Cf::SLOTS) & 1) ^ 1, abort_flag)) { err = ERR_LOAD; break; }
-                mbar_expect_tx(full + slot, Cf::TILE + (KV && !(i & 1) ? STAT_TILE * 4 : 0));
+                mbar_expect_tx(full + slot, Cf::Y_TILE + (KV && !(i & 1) ? Cf::STAT * 4 : 0));
                 if (KV && !(i & 1))
-                    bulk_load(stat + slot / 2 * STAT_TILE, stat_tile(p, b, hy, y), STAT_TILE * 4, full + slot);
-                load_tile<DP>((2 + slot) * Cf::TILE, smem, i & 1 ? &my2 : &my1, full + slot, y * 128, hy, b);
+                    bulk_load(stat + slot / 2 * Cf::STAT, stat_tile(p, b, hy, y * (BN / 64)), Cf::STAT * 4, full + slot);
+                load_tile<DP, BN>(Cf::Y_OFF + slot * Cf::Y_TILE, smem, i & 1 ? &my2 : &my1, full + slot, y * BN, hy, b);
                 if (i & 1 && ++y == first + per) { y = first; ++hy; }
             }
             if (err || *abort_flag) {     // every load issued has to land before the CTA ends
@@ -591,52 +602,41 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const uint32_t leader = elect();
             const int ks = (p.D + 15) / 16;
             const bool f16 = DT == OM_DTYPE_F16;
-            const uint32_t id_s = idesc_f16(f16, 128, false, p.neg), id_dp = idesc_f16(f16, 128, false, false);
+            const uint32_t id_s = idesc_f16(f16, BN, false, p.neg), id_dp = idesc_f16(f16, BN, false, false);
             const uint32_t id_acc = idesc_f16(f16, ks * 16, true, false);
-            const uint32_t x1 = smem_u32(smem), x2 = x1 + Cf::TILE, y = x1 + 2 * Cf::TILE;
-            auto tile = [&](int i) { return y + (i % Cf::SLOTS) * Cf::TILE; };
+            const uint32_t x1 = smem_u32(smem), x2 = x1 + Cf::TILE, y = x1 + Cf::Y_OFF;
+            auto tile = [&](int i) { return y + (i % Cf::SLOTS) * Cf::Y_TILE; };
             auto wait_y = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
             auto score = [&](uint32_t d, uint32_t x, int i, uint32_t id, uint64_t* bar) {
-                product_k<DP>(leader, tmem + d, x, tile(i), id, ks);
+                tc_fence_after();
+                product_k<DP, BN>(leader, tmem + d, x, tile(i), id, ks);
                 commit(leader, bar);
             };
-            auto accumulate = [&](uint32_t d, uint32_t a, int i, bool more) {
-                product_mn<CW>(leader, tmem + d, tmem + a, tile(i), id_acc, more);
-            };
-            auto scores = [&](int i) {    // S of block i, whose Y1 has to be there
-                const bool ok = wait_y(2 * i);
-                if (ok) {
-                    tc_fence_after();
-                    score(i % Cf::NS * 128, x1, 2 * i, id_s, s_full + i % Cf::NS);
-                }
-                return ok;
-            };
-            bool ok = warp_wait(x_full, 0, abort_flag) && scores(0) && wait_y(1);
+            bool ok = warp_wait(x_full, 0, abort_flag) && wait_y(0);
             if (ok) {
-                score(Cf::DP_COL, x2, 1, id_dp, dp_full);
-                if (Cf::NS == 2 && nblk > 1) ok = scores(1);
+                score(0, x1, 0, id_s, s_full);
+                ok = wait_y(1);
             }
+            if (ok) score(Cf::DP_COL, x2, 1, id_dp, dp_full);
             for (int i = 0; ok && i < nblk; ++i) {
-                // products run in the order of their issue: S of block i + NS may overwrite P of
-                // block i right behind the product that reads it
-                ok = warp_wait(p_ready + i % Cf::NS, i / Cf::NS & 1, abort_flag);
+                // products run in the order of their issue: S of the next block may overwrite P
+                // right behind the product that reads it, and dP its dS
+                const bool more = i + 1 < nblk;
+                ok = (!more || wait_y(2 * i + 2)) && warp_wait(p_ready, i & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                if (KV) accumulate(Cf::ACC + DP, i % Cf::NS * 128, 2 * i + 1, i > 0);
-                if (i + Cf::NS < nblk) ok = scores(i + Cf::NS);
-                ok = ok && warp_wait(ds_ready, i & 1, abort_flag);
+                if (KV) product_mn<CW, BN>(leader, tmem + Cf::ACC + DP, tmem, tile(2 * i + 1), id_acc, i > 0);
+                if (more) score(0, x1, 2 * i + 2, id_s, s_full);
+                ok = (!more || wait_y(2 * i + 3)) && warp_wait(ds_ready, i & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                accumulate(Cf::ACC, Cf::DP_COL, 2 * i, i > 0);
+                product_mn<CW, BN>(leader, tmem + Cf::ACC, tmem + Cf::DP_COL, tile(2 * i), id_acc, i > 0);
                 commit(leader, empty + (2 * i) % Cf::SLOTS);
                 commit(leader, empty + (2 * i + 1) % Cf::SLOTS);
-                if (i + 1 < nblk) {
-                    ok = wait_y(2 * i + 3);
-                    if (!ok) break;
+                if (more)
                     score(Cf::DP_COL, x2, 2 * i + 3, id_dp, dp_full);
-                } else {
+                else
                     commit(leader, acc_full);
-                }
             }
             if (!ok) {                    // no MMA may run on when the CTA ends
                 *abort_flag = 1;
@@ -649,7 +649,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         const int w = warp / 4, row = (warp % 4) * 32 + lane, tid = threadIdx.x;
         const int r = r0 + row;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;
-        const uint32_t s_base = tmem + lanes + w * CW, dp_addr = s_base + Cf::DP_COL;
+        const uint32_t s_addr = tmem + lanes + w * CW, dp_addr = s_addr + Cf::DP_COL;
         constexpr float LOG2E = 1.4426950408889634f;
         bool ok = true;
         float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's -lse * log2(e) and -scale * delta
@@ -666,7 +666,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             if (row_hi > 0) {                 // a part of dO . O, 8 elements at a time
                 const auto* go = attn::row<DT>(p.dout, b, r, hx);
                 const auto* o = attn::row<DT>(p.o, b, r, hx);
-                for (int c = w; c < p.D / 8; c += BWD_WG) {
+                for (int c = w; c < p.D / 8; c += Cf::WG) {
                     const uint4 u = reinterpret_cast<const uint4*>(go)[c], v = reinterpret_cast<const uint4*>(o)[c];
                     const auto* a2 = reinterpret_cast<const typename Half16<DT>::T2*>(&u);
                     const auto* b2 = reinterpret_cast<const typename Half16<DT>::T2*>(&v);
@@ -679,25 +679,25 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 lse2 = -p.lse[((long long)b * p.H + hx) * p.Sq + r] * LOG2E;
             }
             stat[tid] = d;
-            mbar_arrive(stat_ready);
+            warp_arrive(stat_ready);
             ok = warp_wait(stat_ready, 0, abort_flag);
-            for (int x = 0; x < BWD_WG; ++x) ds0 += stat[row + x * 128];
+            for (int x = 0; x < Cf::WG; ++x) ds0 += stat[row + x * 128];
             ds0 *= -p.scale;
             if (ok && w == 0) {           // for the KV kernel
-                float* out = stat_tile(p, b, hx, r0 / 128) + row;
+                float* out = stat_tile(p, b, hx, (r0 + row) / 64) + row % 64;
                 out[0] = lse2;
-                out[128] = ds0;
+                out[64] = ds0;
             }
         }
-        int y0 = first * 128;
+        int y0 = first * BN;
         for (int i = 0; ok && i < nblk; ++i) {
-            const float *c_lse = stat + i % (Cf::SLOTS / 2) * STAT_TILE + w * CW, *c_ds = c_lse + 128;
-            const uint32_t s_addr = s_base + i % Cf::NS * 128;
+            const float *c_lse = stat + i % (Cf::SLOTS / 2) * Cf::STAT + w * CW / 64 * STAT_TILE + w * CW % 64,
+                        *c_ds = c_lse + 64;
             if (KV) {                     // the block's statistics came with Y1
                 ok = warp_wait(full + 2 * i % Cf::SLOTS, (2 * i / Cf::SLOTS) & 1, abort_flag);
                 if (!ok) break;
             }
-            ok = warp_wait(s_full + i % Cf::NS, i / Cf::NS & 1, abort_flag);
+            ok = warp_wait(s_full, i & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             uint32_t pv[CW];
@@ -706,7 +706,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             float* pr = reinterpret_cast<float*>(pv);
             if (!KV) {                        // S may be overwritten: P stays in registers
                 tc_fence_before();
-                mbar_arrive(p_ready + i % Cf::NS);
+                warp_arrive(p_ready);
             }
             const int lo = row_lo - y0 - w * CW, hi = row_hi - y0 - w * CW;
             const bool mask = __any_sync(~0u, lo > 0 || hi < CW);
@@ -723,11 +723,11 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             }
             // streamed rows past the sequence's length may hold anything
             const int y_end = KV ? ql : kl;
-            if (w < 2 && y_end - y0 < 128) {
+            if (w < 2 && y_end - y0 < BN) {
                 const int iy = 2 * i + w;
                 ok = warp_wait(full + iy % Cf::SLOTS, (iy / Cf::SLOTS) & 1, abort_flag);
                 if (!ok) break;
-                zero_tail<DP>(smem + (2 + iy % Cf::SLOTS) * Cf::TILE, y_end - y0, row);
+                zero_tail<DP, BN>(smem + Cf::Y_OFF + iy % Cf::SLOTS * Cf::Y_TILE, y_end - y0, row);
             }
             if (KV) {
                 uint32_t pk[CW / 2];
@@ -736,7 +736,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 tmem_st16(s_addr, pk);
                 tmem_st_wait();
                 tc_fence_before();
-                mbar_arrive(p_ready + i % Cf::NS);
+                warp_arrive(p_ready);
             }
             ok = warp_wait(dp_full, i & 1, abort_flag);
             if (!ok) break;
@@ -761,9 +761,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             tmem_st16(dp_addr, dk);
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(ds_ready);
-            y0 += 128;
-            if (KV && y0 == (first + per) * 128) y0 = first * 128;
+            warp_arrive(ds_ready);
+            y0 += BN;
+            if (KV && y0 == (first + per) * BN) y0 = first * BN;
         }
         if (ok && nblk > 0) ok = warp_wait(acc_full, 0, abort_flag);
         if (!ok) {
@@ -771,12 +771,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             err = ERR_MATH;
         } else {
             tc_fence_after();
-            // the warpgroups take alternate 32 columns, the first two of dK, the others of dV for KV
+            // the warpgroups take alternate 32 columns; KV: the first half of them dK, the others dV
+            constexpr int HALF = Cf::WG / 2;
             const int rows = KV ? p.Sk : p.Sq;
-            const View& view = !KV ? p.dq : w < 2 ? p.dk : p.dv;
+            const View& view = !KV ? p.dq : w < HALF ? p.dk : p.dv;
             auto* out = r < rows ? row_out<DT>(view, b, r, hx) : nullptr;
-            const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w / 2 * DP : 0);
-            for (int c = (KV ? w % 2 : w) * 32; c < p.D; c += KV ? 64 : 128) {
+            const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w / HALF * DP : 0);
+            for (int c = (KV ? w % HALF : w) * 32; c < p.D; c += (KV ? HALF : Cf::WG) * 32) {
                 uint32_t o[32];
                 if (nblk > 0) {
                     tmem_ld32_issue(acc + c, o);
@@ -832,15 +833,15 @@ static void set_scale(Params* p, float scale) {
     p->scale2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);
 }
 
-// A tensor map over a [batch, token, head, D] view with boxes of 64 columns x 128 tokens.
+// A tensor map over a [batch, token, head, D] view with boxes of 64 columns x `rows` tokens.
 // Strides of dimensions of length 1 are replaced by one that the map takes.
-static int encode(CUtensorMap* map, const View& v, int nB, int nT, int nH, int D, int dt) {
+static int encode(CUtensorMap* map, const View& v, int nB, int nT, int nH, int D, int dt, int rows = 128) {
     PFN_cuTensorMapEncodeTiled_v12000 fn = tc::encode_tiled_fn();
     if (!fn) return OM_ERR_DRIVER;
     cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)nT, (cuuint64_t)nH, (cuuint64_t)nB};
     cuuint64_t strides[3] = {nT > 1 ? (cuuint64_t)v.st * 2 : 256, nH > 1 ? (cuuint64_t)v.sh * 2 : 256,
                              nB > 1 ? (cuuint64_t)v.sb * 2 : 256};
-    cuuint32_t box[4] = {64, 128, 1, 1};
+    cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
     cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUresult r = fn(map, dt == OM_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                           4, v.p, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -874,8 +875,10 @@ static int forward(DeviceCtx* c, const Params& p) {
     return p.Sq <= 128 ? launch_fwd<128, 1, DT>(c, p) : launch_fwd<128, 2, DT>(c, p);
 }
 
+// x1, x2: maps of the kept tiles (128 rows), y1, y2: of the streamed ones (BN rows)
 template <int DP, bool KV, int DT>
-static int launch_bwd(DeviceCtx* c, const CUtensorMap (&m)[4], const Params& p) {
+static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& y1,
+                      const CUtensorMap& y2, const Params& p) {
     using Cf = BwdCfg<DP>;
     auto kern = attn_bwd_kernel<DP, KV, DT>;
     static bool attr_set[64] = {false};
@@ -885,24 +888,26 @@ static int launch_bwd(DeviceCtx* c, const CUtensorMap (&m)[4], const Params& p) 
     }
     const long long n = (long long)(((KV ? p.Sk : p.Sq) + 127) / 128) * p.B * (KV ? p.Hkv : p.H);
     if (n > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-    const unsigned grid = (unsigned)n;
-    if (KV)
-        kern<<<grid, Cf::THREADS, Cf::SMEM, c->compute>>>(m[1], m[2], m[0], m[3], p);
-    else
-        kern<<<grid, Cf::THREADS, Cf::SMEM, c->compute>>>(m[0], m[3], m[1], m[2], p);
+    kern<<<(unsigned)n, Cf::THREADS, Cf::SMEM, c->compute>>>(x1, x2, y1, y2, p);
     return after_launch(c);
 }
 template <int DP, int DT>
 static int backward(DeviceCtx* c, const Params& p) {
-    CUtensorMap m[4] = {};                // Q, K, V, dO
+    constexpr int BN = BwdCfg<DP>::BN;
+    CUtensorMap m[2][4] = {};             // Q, K, V, dO; boxes of 128 and of BN rows
+    const View* view[4] = {&p.q, &p.k, &p.v, &p.dout};
+    for (int i = 0; i < 4; ++i) {
+        const bool kv = i == 1 || i == 2;
+        if ((kv ? p.Sk : p.Sq) == 0) continue;
+        for (int r = 0; r < 2; ++r) {
+            const int st = encode(&m[r][i], *view[i], p.B, kv ? p.Sk : p.Sq, kv ? p.Hkv : p.H, p.D, DT, r ? BN : 128);
+            if (st != OM_OK) return st;
+        }
+    }
+    // dQ first: it leaves the queries' statistics for dK and dV
     int st = OM_OK;
-    if (p.Sq > 0) st = encode(&m[0], p.q, p.B, p.Sq, p.H, p.D, DT);
-    if (st == OM_OK && p.Sk > 0) st = encode(&m[1], p.k, p.B, p.Sk, p.Hkv, p.D, DT);
-    if (st == OM_OK && p.Sk > 0) st = encode(&m[2], p.v, p.B, p.Sk, p.Hkv, p.D, DT);
-    if (st == OM_OK && p.Sq > 0) st = encode(&m[3], p.dout, p.B, p.Sq, p.H, p.D, DT);
-    // dQ first: it leaves delta for dK and dV
-    if (st == OM_OK && p.Sq > 0) st = launch_bwd<DP, false, DT>(c, m, p);
-    if (st == OM_OK && p.Sk > 0) st = launch_bwd<DP, true, DT>(c, m, p);
+    if (p.Sq > 0) st = launch_bwd<DP, false, DT>(c, m[0][0], m[0][3], m[1][1], m[1][2], p);
+    if (st == OM_OK && p.Sk > 0) st = launch_bwd<DP, true, DT>(c, m[0][1], m[0][2], m[1][0], m[1][3], p);
     return st;
 }
 
@@ -915,7 +920,7 @@ extern "C" long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int n
                                                    int nSk, int nHeadDim, int bBackward) {
     const int st = attn::check_sizes(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim);
     if (st != OM_OK) return st;
-    return bBackward ? (long long)nBatch * nHeads * ((nSq + 127) / 128) * attn::STAT_TILE * 4 : 0;
+    return bBackward ? (long long)nBatch * nHeads * attn::stat_tiles(nSq) * attn::STAT_TILE * 4 : 0;
 }
 
 extern "C" int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut,
