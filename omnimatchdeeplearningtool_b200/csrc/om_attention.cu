@@ -1,4 +1,6 @@
 // Attention and its backward, which recomputes the probabilities from the saved log-sum-exp.
+#include <math.h>
+
 #include "om_common.cuh"
 #include "om_tc_ptx.cuh"
 
@@ -14,10 +16,12 @@ struct View {          // a [batch, token, head, D] tensor: element strides, D c
 struct Params {
     View q, k, v, o, dout, dq, dk, dv;
     float* lse;        // [B, H, Sq]
-    float* stat;       // the backward's workspace: see stat_tile
+    uint8_t* stat;     // the backward's workspace: see stat_tile
     const int *qlens, *kvlens;
     int B, H, Hkv, Sq, Sk, D, causal;
     float scale;
+    float lse_unit;    // the backward's 2^a near 1 / |scale|, and what turns -lse log2(e) into the
+    float lse_part;    // value whose parts are kept: 1 / (scale2 2^a)
     float scale2;      // |scale| * log2(e), not 0 (masked scores stay minus infinity)
     bool neg;          // scale < 0: the score products negate Q
     unsigned int* err;
@@ -489,12 +493,43 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 // of 4096 tokens, its MMA warp idle between a block's barriers). Longer heads fill TMEM: BN 128.
 // TMEM: S at 0, dP at BN (P and dS over the first half of each 32 columns), accumulators behind.
 constexpr int BWD_COLS = 32;
-// What the dQ kernel leaves of 64 queries for the KV kernel, in the workspace as
-// [batch][head][64 queries]: 64 times -log2(e) lse, 64 times -scale delta.
-constexpr int STAT_TILE = 128;
+// The KV kernel's lse and delta vary along the columns of S^T, where a thread would have to fetch
+// them one by one (from shared memory 1024 broadcast wavefronts a 128 x 128 tile, more than the
+// products' own operands take: 303 us against 211 us without any arithmetic, 24 heads of 4096
+// tokens x 64). So they enter through the products: one more step of 16 columns, in which the
+// streamed side has -lse / |scale| and -delta and the kept side constants. Each value is three
+// 16-bit parts, h + 2^-11 m + 2^-22 l (24 bits and more), so nothing of fp32 is lost:
+//   S^T - lse / |scale| = K Q^T + XE1 YE^T, dP^T - delta = V dO^T + XE2 YE^T,
+//   YE = (parts of -lse / |scale| / 2^a, parts of -delta / 16, 0 ...),
+//   XE1 = 2^a (1, 2^-11, 2^-22, 0 ...), XE2 = 16 (0, 0, 0, 1, 2^-11, 2^-22, 0 ...),
+// with 2^a near 1 / |scale| to keep the parts in range of fp16. Without swizzle, as core matrices of
+// 8 rows x 8 columns (128 bytes); the columns 8..15 are zeros.
+// The dQ kernel leaves YE in the workspace as [batch][head][64 queries][8 rows][2 cores].
+constexpr int STAT_TILE = 2048;                              // bytes of 64 queries
+constexpr int XE_REGION = 128 * 16, XE_BYTES = 3 * XE_REGION;   // XE2's and XE1's first cores, zeros
 __host__ __device__ constexpr int stat_tiles(int nSq) { return (nSq + 127) / 128 * 2; }
-__device__ __forceinline__ float* stat_tile(const Params& p, int b, int h, int tile) {
+__device__ __forceinline__ uint8_t* stat_tile(const Params& p, int b, int h, int tile) {
     return p.stat + (((long long)b * p.H + h) * stat_tiles(p.Sq) + tile) * STAT_TILE;
+}
+// low descriptor word of an unswizzled operand; the high word: rows of cores `rows` bytes apart
+__device__ __forceinline__ uint32_t desc_plain(uint32_t at, uint32_t cols) { return (at >> 4) | (cols >> 4 << 16); }
+__host__ __device__ constexpr uint32_t plain_hi(uint32_t rows) { return (rows >> 4) | (1u << 14); }
+// D += XE YE^T
+__device__ __forceinline__ void product_plain(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .b64 a, b;\n\t.reg .pred p, q;\n\t"
+        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %5};\n\tsetp.eq.b32 p, 0, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(plain_hi(128)), "r"(plain_hi(256)), "r"(leader));
+}
+// the three parts of a value in the first three elements at `out`
+template <int DT>
+__device__ __forceinline__ void three_parts(float v, typename Half16<DT>::T* out) {
+    using H16 = Half16<DT>;
+    out[0] = H16::from_f(v);
+    const float r = (v - H16::to_f(out[0])) * 2048.f;
+    out[1] = H16::from_f(r);
+    out[2] = H16::from_f((r - H16::to_f(out[1])) * 2048.f);
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -508,12 +543,13 @@ struct BwdCfg {
     static constexpr int TILE = DP / 64 * PANEL, Y_TILE = DP / 64 * BN * 128;
     static constexpr int SLOTS = DP == 64 ? 8 : 4;
     static constexpr int Y_OFF = 2 * TILE;
-    static constexpr int STAT = BN / 64 * STAT_TILE;         // statistics of a block, per pair of slots
+    static constexpr int STAT = BN / 64 * STAT_TILE;         // YE of a block, per pair of slots
     static constexpr int STAT_OFF = Y_OFF + SLOTS * Y_TILE;
-    static constexpr int BAR_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT, WG * 128) * 4;
+    static constexpr int XE_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT, WG * 128 * 4);
+    static constexpr int BAR_OFF = XE_OFF + XE_BYTES;
     static constexpr int SMEM = BAR_OFF + 512 + 1024;
     static constexpr int DP_COL = BN, ACC = 2 * BN, TMEM_COLS = 2 * BN + 2 * DP;
-    static_assert(TMEM_COLS * OCC <= 512 && SMEM * OCC <= 227 * 1024, "on-chip memory");
+    static_assert(TMEM_COLS * OCC <= 512 && (SMEM + 1024) * OCC <= 228 * 1024, "on-chip memory");
 };
 
 template <int DP, bool KV, int DT>
@@ -569,6 +605,18 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                          smem_u32(tmem_holder)), "r"(Cf::TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    if (KV) {                             // the constant operands, 8 columns of a row at a time
+        for (int i = threadIdx.x; i < XE_BYTES / 16; i += Cf::THREADS) {
+            alignas(16) typename Half16<DT>::T v[8];
+            const int region = i / 128;   // 0: XE2, 1: XE1, 2: zeros
+            for (int c = 0; c < 8; ++c) {
+                const float unit = c % 3 == 0 ? 1.f : c % 3 == 1 ? 1.f / 2048.f : 1.f / 4194304.f;
+                v[c] = Half16<DT>::from_f(region == 0 && c >= 3 && c < 6 ? 16.f * unit : region == 1 && c < 3 ? p.lse_unit * unit : 0.f);
+            }
+            reinterpret_cast<uint4*>(smem + Cf::XE_OFF)[i] = *reinterpret_cast<const uint4*>(v);
+        }
+        fence_async_smem();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -584,9 +632,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             for (; i < 2 * nblk; ++i) {   // Y1 (KV: and its queries' statistics), Y2 of each block in turn
                 const int slot = i % Cf::SLOTS;
                 if (!mbar_wait(empty + slot, ((i / Cf::SLOTS) & 1) ^ 1, abort_flag)) { err = ERR_LOAD; break; }
-                mbar_expect_tx(full + slot, Cf::Y_TILE + (KV && !(i & 1) ? Cf::STAT * 4 : 0));
+                mbar_expect_tx(full + slot, Cf::Y_TILE + (KV && !(i & 1) ? Cf::STAT : 0));
                 if (KV && !(i & 1))
-                    bulk_load(stat + slot / 2 * Cf::STAT, stat_tile(p, b, hy, y * (BN / 64)), Cf::STAT * 4, full + slot);
+                    bulk_load(smem + Cf::STAT_OFF + slot / 2 * Cf::STAT, stat_tile(p, b, hy, y * (BN / 64)), Cf::STAT,
+                              full + slot);
                 load_tile<DP, BN>(Cf::Y_OFF + slot * Cf::Y_TILE, smem, i & 1 ? &my2 : &my1, full + slot, y * BN, hy, b);
                 if (i & 1 && ++y == first + per) { y = first; ++hy; }
             }
@@ -605,11 +654,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const uint32_t id_s = idesc_f16(f16, BN, false, p.neg), id_dp = idesc_f16(f16, BN, false, false);
             const uint32_t id_acc = idesc_f16(f16, ks * 16, true, false);
             const uint32_t x1 = smem_u32(smem), x2 = x1 + Cf::TILE, y = x1 + Cf::Y_OFF;
+            const uint32_t xe = x1 + Cf::XE_OFF, ye = x1 + Cf::STAT_OFF;
             auto tile = [&](int i) { return y + (i % Cf::SLOTS) * Cf::Y_TILE; };
             auto wait_y = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
             auto score = [&](uint32_t d, uint32_t x, int i, uint32_t id, uint64_t* bar) {
                 tc_fence_after();
                 product_k<DP, BN>(leader, tmem + d, x, tile(i), id, ks);
+                if (KV)                   // d == 0: XE1, else XE2
+                    product_plain(leader, tmem + d, desc_plain(xe + (d ? 0 : XE_REGION), d ? 2 * XE_REGION : XE_REGION),
+                                  desc_plain(ye + i / 2 % (Cf::SLOTS / 2) * Cf::STAT, 128), id_dp);
                 commit(leader, bar);
             };
             bool ok = warp_wait(x_full, 0, abort_flag) && wait_y(0);
@@ -681,22 +734,21 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             stat[tid] = d;
             warp_arrive(stat_ready);
             ok = warp_wait(stat_ready, 0, abort_flag);
-            for (int x = 0; x < Cf::WG; ++x) ds0 += stat[row + x * 128];
-            ds0 *= -p.scale;
+            float delta = 0.f;
+            for (int x = 0; x < Cf::WG; ++x) delta += stat[row + x * 128];
+            ds0 = -delta * p.scale;
             if (ok && w == 0) {           // for the KV kernel
-                float* out = stat_tile(p, b, hx, (r0 + row) / 64) + row % 64;
-                out[0] = lse2;
-                out[64] = ds0;
+                alignas(16) typename Half16<DT>::T v[8];
+                three_parts<DT>(lse2 * p.lse_part, v);
+                three_parts<DT>(delta * -0.0625f, v + 3);
+                v[6] = v[7] = Half16<DT>::from_f(0.f);
+                uint4* out = reinterpret_cast<uint4*>(stat_tile(p, b, hx, (r0 + row) / 64) + row % 64 / 8 * 256 + row % 8 * 16);
+                out[0] = *reinterpret_cast<const uint4*>(v);
+                out[8] = make_uint4(0, 0, 0, 0);
             }
         }
         int y0 = first * BN;
         for (int i = 0; ok && i < nblk; ++i) {
-            const float *c_lse = stat + i % (Cf::SLOTS / 2) * Cf::STAT + w * CW / 64 * STAT_TILE + w * CW % 64,
-                        *c_ds = c_lse + 64;
-            if (KV) {                     // the block's statistics came with Y1
-                ok = warp_wait(full + 2 * i % Cf::SLOTS, (2 * i / Cf::SLOTS) & 1, abort_flag);
-                if (!ok) break;
-            }
             ok = warp_wait(s_full, i & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
@@ -712,8 +764,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const bool mask = __any_sync(~0u, lo > 0 || hi < CW);
 #pragma unroll
             for (int c = 0; c < CW; c += 2) {
-                const F2 sub = KV ? *reinterpret_cast<const F2*>(c_lse + c) : F2{lse2, lse2};
-                const F2 e = fma2({pr[c], pr[c + 1]}, {p.scale2, p.scale2}, sub);
+                const F2 v = {pr[c], pr[c + 1]}, k = {p.scale2, p.scale2};
+                const F2 e = KV ? mul2(v, k) : fma2(v, k, {lse2, lse2});
                 pr[c] = ex2(e.x);
                 pr[c + 1] = ex2(e.y);
             }
@@ -747,8 +799,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             float* dp = reinterpret_cast<float*>(dv);
 #pragma unroll
             for (int c = 0; c < CW; c += 2) {
-                const F2 sub = KV ? *reinterpret_cast<const F2*>(c_ds + c) : F2{ds0, ds0};
-                const F2 e = mul2({pr[c], pr[c + 1]}, fma2({dp[c], dp[c + 1]}, {p.scale, p.scale}, sub));
+                const F2 v = {dp[c], dp[c + 1]}, k = {p.scale, p.scale};
+                const F2 e = mul2({pr[c], pr[c + 1]}, KV ? mul2(v, k) : fma2(v, k, {ds0, ds0}));
                 dp[c] = e.x;
                 dp[c + 1] = e.y;
             }
@@ -831,6 +883,11 @@ static void set_scale(Params* p, float scale) {
     p->scale = scale;
     p->neg = scale < 0.f;
     p->scale2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);
+    int a;
+    frexpf(fabsf(scale), &a);                // |scale| in [2^(a-1), 2^a)
+    a = a < -15 ? -15 : a > 2 ? 2 : a;
+    p->lse_unit = ldexpf(1.f, -a);
+    p->lse_part = 1.f / (p->scale2 * p->lse_unit);
 }
 
 // A tensor map over a [batch, token, head, D] view with boxes of 64 columns x `rows` tokens.
@@ -920,7 +977,7 @@ extern "C" long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int n
                                                    int nSk, int nHeadDim, int bBackward) {
     const int st = attn::check_sizes(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim);
     if (st != OM_OK) return st;
-    return bBackward ? (long long)nBatch * nHeads * attn::stat_tiles(nSq) * attn::STAT_TILE * 4 : 0;
+    return bBackward ? (long long)nBatch * nHeads * attn::stat_tiles(nSq) * attn::STAT_TILE : 0;
 }
 
 extern "C" int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut,
@@ -959,6 +1016,7 @@ extern "C" int omCudaAttentionBackward(const void* pGradOut, const void* pQ, con
     if (st != OM_OK) return st;
     if (nDtype != OM_DTYPE_BF16 && nDtype != OM_DTYPE_F16) return OM_ERR_UNSUPPORTED;
     if (!(fabsf(fScale) < INFINITY)) return OM_ERR_INVALID;
+    if (fabsf(fScale) < 0x1p-20f) return OM_ERR_UNSUPPORTED;    // lse / |scale| leaves 16-bit range
     attn::Params p = {};
     if (!pStrides || !attn::view(&p.q, pQ, pStrides, nBatch, nSq, nHeads) ||
         !attn::view(&p.k, pK, pStrides + 3, nBatch, nSk, nKvHeads) ||
@@ -972,7 +1030,7 @@ extern "C" int omCudaAttentionBackward(const void* pGradOut, const void* pQ, con
     if (nBatch == 0) return OM_OK;
     if (nSq > 0 && (!pLse || !pWorkspace || reinterpret_cast<uintptr_t>(pWorkspace) % 16))
         return OM_ERR_INVALID;
-    p.lse = const_cast<float*>(pLse); p.stat = static_cast<float*>(pWorkspace);
+    p.lse = const_cast<float*>(pLse); p.stat = static_cast<uint8_t*>(pWorkspace);
     p.qlens = pQLens; p.kvlens = pKvLens;
     p.B = nBatch; p.H = nHeads; p.Hkv = nKvHeads; p.Sq = nSq; p.Sk = nSk; p.D = nHeadDim;
     p.causal = bCausal != 0; p.err = c->err_word;
