@@ -234,7 +234,10 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int row) {
 //   S's columns) -> O += P V (TMEM, fp32).
 // O is rescaled only when a row's maximum has grown by more than 2^8 since its last reference
 // maximum: P stays below 2^8, in range of both types, and the factor cancels in O / l.
-// TMEM: S_t at t * 128 columns, O_t behind the S tiles.
+// Score tile n = NT j + t (block j, query tile t) lies in TMEM buffer n % NB. With heads up to 64
+// there is room for a third buffer, so that a tile's next scores are there when its probabilities
+// are done (without it a softmax warp waited about 900 of 2900 clocks a block for them).
+// TMEM: NB score tiles, then the O tiles.
 template <int DP, int NT>
 struct FwdCfg {
     static constexpr int TILE = DP / 64 * PANEL;
@@ -242,7 +245,9 @@ struct FwdCfg {
     static constexpr int SMEM = (NT + SLOTS) * TILE + 1024 + 1024;
     static constexpr int THREADS = NT * 128 + 64;
     static constexpr int TMEM_COLS = NT * 256;
-    static constexpr int O_COL = NT * 128, O_STEP = 128;
+    static constexpr int NB = NT == 2 && DP == 64 ? 3 : NT;
+    static constexpr int O_COL = NB * 128, O_STEP = DP;
+    static_assert(O_COL + NT * O_STEP <= TMEM_COLS, "TMEM");
 };
 enum : unsigned int { ERR_LOAD = ERRBIT_TC_PRODUCER, ERR_MMA = ERRBIT_TC_MMA,
                       ERR_MATH = ERRBIT_TC_EPILOGUE, ERR_DRAIN = ERRBIT_TC_DRAIN };
@@ -260,8 +265,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     uint64_t* o_full = bars + 1;
     uint64_t* drain = bars + 2;
     uint64_t* s_full = bars + 3;
-    uint64_t* p_full = s_full + NT;
-    uint64_t* full = p_full + NT;
+    uint64_t* p_full = s_full + Cf::NB;
+    uint64_t* pv_done = p_full + Cf::NB;
+    uint64_t* full = pv_done + NT;
     uint64_t* empty = full + Cf::SLOTS;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -282,7 +288,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         mbar_init(q_full, 1);
         mbar_init(o_full, 1);
         mbar_init(drain, 1);
-        for (int t = 0; t < NT; ++t) { mbar_init(s_full + t, 1); mbar_init(p_full + t, 4); }
+        for (int i = 0; i < Cf::NB; ++i) { mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); }
+        for (int t = 0; t < NT; ++t) mbar_init(pv_done + t, 1);
         for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -324,32 +331,31 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             const uint32_t id_s = idesc_f16(DT == OM_DTYPE_F16, 128, false, p.neg);
             const uint32_t id_o = idesc_f16(DT == OM_DTYPE_F16, ks * 16, true, false);
             const uint32_t q_tile = smem_u32(smem);
-            auto qk = [&](int t, int i) {
-                const uint32_t kt = kv_base + (i % Cf::SLOTS) * Cf::TILE;
-                product_k<DP, 128>(leader, tmem + t * 128, q_tile + t * Cf::TILE, kt, id_s, ks);
-                commit(leader, s_full + t);
-            };
             auto wait_kv = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
-            bool ok = warp_wait(q_full, 0, abort_flag) && wait_kv(0);
-            if (ok) {
+            const int total = NT * nblk;
+            auto scores = [&](int n) {    // score tile n, and K's slot back behind the block's last
+                const int j = n / NT, t = n % NT;
+                if (t == 0 && !wait_kv(2 * j)) return false;
                 tc_fence_after();
-                for (int t = 0; t < NT; ++t) qk(t, 0);
-                commit(leader, empty + 0);
-            }
-            for (int j = 0; ok && j < nblk; ++j) {
-                const bool more = j + 1 < nblk;
-                ok = wait_kv(2 * j + 1) && (!more || wait_kv(2 * j + 2));
-                const uint32_t vt = kv_base + ((2 * j + 1) % Cf::SLOTS) * Cf::TILE;
-                for (int t = 0; ok && t < NT; ++t) {
-                    ok = warp_wait(p_full + t, j & 1, abort_flag);
-                    if (!ok) break;
-                    tc_fence_after();
-                    product_mn<128, 128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + t * 128, vt, id_o, j > 0);
-                    if (more) qk(t, 2 * j + 2);
-                }
+                product_k<DP, 128>(leader, tmem + n % Cf::NB * 128, q_tile + t * Cf::TILE,
+                                   kv_base + 2 * j % Cf::SLOTS * Cf::TILE, id_s, ks);
+                commit(leader, s_full + n % Cf::NB);
+                if (t == NT - 1) commit(leader, empty + 2 * j % Cf::SLOTS);
+                return true;
+            };
+            bool ok = warp_wait(q_full, 0, abort_flag);
+            for (int n = 0; ok && n < Cf::NB && n < total; ++n) ok = scores(n);
+            for (int n = 0; ok && n < total; ++n) {
+                const int j = n / NT, t = n % NT;
+                ok = (t > 0 || wait_kv(2 * j + 1)) && warp_wait(p_full + n % Cf::NB, n / Cf::NB & 1, abort_flag);
                 if (!ok) break;
-                commit(leader, empty + (2 * j + 1) % Cf::SLOTS);
-                commit(leader, more ? empty + (2 * j + 2) % Cf::SLOTS : o_full);
+                tc_fence_after();
+                product_mn<128, 128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + n % Cf::NB * 128,
+                                     kv_base + (2 * j + 1) % Cf::SLOTS * Cf::TILE, id_o, j > 0);
+                commit(leader, pv_done + t);
+                if (t == NT - 1) commit(leader, j + 1 < nblk ? empty + (2 * j + 1) % Cf::SLOTS : o_full);
+                // behind the product that read the buffer's probabilities
+                if (n + Cf::NB < total) ok = scores(n + Cf::NB);
             }
             if (!ok) {                    // no MMA may run on when the CTA ends
                 *abort_flag = 1;
@@ -361,14 +367,15 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     } else {
         const int t = warp / 4, row = (warp % 4) * 32 + lane;
         const int i = q0 + t * 128 + row;
-        const uint32_t s_addr = tmem + t * 128 + ((uint32_t)(warp % 4) << 21);
         const uint32_t o_addr = tmem + Cf::O_COL + t * Cf::O_STEP + ((uint32_t)(warp % 4) << 21);
         int row_end = i < ql ? kl : 0;
         if (p.causal) row_end = min(row_end, i + kl - ql + 1);
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < nblk; ++j) {
-            ok = warp_wait(s_full + t, j & 1, abort_flag);
+            const int n = j * NT + t, buf = n % Cf::NB;
+            const uint32_t s_addr = tmem + buf * 128 + ((uint32_t)(warp % 4) << 21);
+            ok = warp_wait(s_full + buf, n / Cf::NB & 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
             uint32_t sv[128];
@@ -413,7 +420,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             }
             sum[0] = add2(sum[0], sum[1]);
             l += sum[0].x + sum[0].y;
-            if (grow)                     // S_j is complete, so every product issued before it is
+            if (grow) {                   // behind the last product that added to O
+                ok = warp_wait(pv_done + t, (j - 1) & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
                 for (int c = 0; c < p.D; c += 32) {
                     uint32_t o[32];
                     tmem_ld32_issue(o_addr + c, o);
@@ -422,6 +432,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
                     tmem_st32(o_addr + c, o);
                 }
+            }
             // keys past the sequence's length may hold anything
             if (t == 0 && j == nblk - 1 && kl - j * 128 < 128) {
                 const int iv = 2 * j + 1;
@@ -431,7 +442,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             }
             tmem_st_wait();
             tc_fence_before();
-            warp_arrive(p_full + t);
+            warp_arrive(p_full + buf);
         }
         if (ok && nblk > 0) ok = warp_wait(o_full, 0, abort_flag);
         if (!ok) {
