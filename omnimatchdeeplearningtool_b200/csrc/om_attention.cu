@@ -331,31 +331,42 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             const uint32_t id_s = idesc_f16(DT == OM_DTYPE_F16, 128, false, p.neg);
             const uint32_t id_o = idesc_f16(DT == OM_DTYPE_F16, ks * 16, true, false);
             const uint32_t q_tile = smem_u32(smem);
-            auto wait_kv = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
-            const int total = NT * nblk;
-            auto scores = [&](int n) {    // score tile n, and K's slot back behind the block's last
-                const int j = n / NT, t = n % NT;
-                if (t == 0 && !wait_kv(2 * j)) return false;
+            // Running places: block, slot and TMEM buffer of the scores to issue next (s...) and of
+            // the probabilities to take next (p...)
+            struct { int tile, slot, buf; uint32_t slot_ph, buf_ph; } sn = {0, 0, 0, 0, 0}, pn = {0, 1, 0, 0, 0};
+            auto step = [&](auto& at) {
+                if (++at.buf == Cf::NB) { at.buf = 0; at.buf_ph ^= 1; }
+                if (++at.tile == NT) {
+                    at.tile = 0;
+                    at.slot += 2;
+                    if (at.slot >= Cf::SLOTS) { at.slot -= Cf::SLOTS; at.slot_ph ^= 1; }
+                }
+            };
+            auto scores = [&]() {         // one score tile, and K's slot back behind the block's last
+                if (sn.tile == 0 && !warp_wait(full + sn.slot, sn.slot_ph, abort_flag)) return false;
                 tc_fence_after();
-                product_k<DP, 128>(leader, tmem + n % Cf::NB * 128, q_tile + t * Cf::TILE,
-                                   kv_base + 2 * j % Cf::SLOTS * Cf::TILE, id_s, ks);
-                commit(leader, s_full + n % Cf::NB);
-                if (t == NT - 1) commit(leader, empty + 2 * j % Cf::SLOTS);
+                product_k<DP, 128>(leader, tmem + sn.buf * 128, q_tile + sn.tile * Cf::TILE, kv_base + sn.slot * Cf::TILE,
+                                   id_s, ks);
+                commit(leader, s_full + sn.buf);
+                if (sn.tile == NT - 1) commit(leader, empty + sn.slot);
+                step(sn);
                 return true;
             };
+            const int total = NT * nblk;
             bool ok = warp_wait(q_full, 0, abort_flag);
-            for (int n = 0; ok && n < Cf::NB && n < total; ++n) ok = scores(n);
+            for (int n = 0; ok && n < Cf::NB && n < total; ++n) ok = scores();
             for (int n = 0; ok && n < total; ++n) {
-                const int j = n / NT, t = n % NT;
-                ok = (t > 0 || wait_kv(2 * j + 1)) && warp_wait(p_full + n % Cf::NB, n / Cf::NB & 1, abort_flag);
+                ok = (pn.tile > 0 || warp_wait(full + pn.slot, pn.slot_ph, abort_flag)) &&
+                     warp_wait(p_full + pn.buf, pn.buf_ph, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                product_mn<128, 128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + n % Cf::NB * 128,
-                                     kv_base + (2 * j + 1) % Cf::SLOTS * Cf::TILE, id_o, j > 0);
-                commit(leader, pv_done + t);
-                if (t == NT - 1) commit(leader, j + 1 < nblk ? empty + (2 * j + 1) % Cf::SLOTS : o_full);
+                product_mn<128, 128>(leader, tmem + Cf::O_COL + pn.tile * Cf::O_STEP, tmem + pn.buf * 128,
+                                     kv_base + pn.slot * Cf::TILE, id_o, n >= NT);
+                commit(leader, pv_done + pn.tile);
+                if (pn.tile == NT - 1) commit(leader, n + 1 < total ? empty + pn.slot : o_full);
+                step(pn);
                 // behind the product that read the buffer's probabilities
-                if (n + Cf::NB < total) ok = scores(n + Cf::NB);
+                if (n + Cf::NB < total) ok = scores();
             }
             if (!ok) {                    // no MMA may run on when the CTA ends
                 *abort_flag = 1;
