@@ -25,6 +25,9 @@ struct Params {
     float scale2;      // |scale| * log2(e), not 0 (masked scores stay minus infinity)
     bool neg;          // scale < 0: the score products negate Q
     unsigned int* err;
+    int splits;        // parts of the streamed axis, each CTA one of them (1: no partial results)
+    float* part;       // partial results: fp32 rows [split][batch][head][token][D]
+    float* part_lse;   // forward: the parts' log2(sum exp) [split][batch][head][token]
 };
 
 template <int DT>
@@ -227,6 +230,31 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int row) {
     fence_async_smem();
 }
 
+// Columns c .. c + 31 of one row from the accumulators o (zeros unless `any`), times f: to a row of
+// partial results, or rounded to the output row; nothing for a row that is not there.
+template <int DT, class T>
+__device__ __forceinline__ void store_chunk(const uint32_t (&o)[32], bool any, float f, bool partial, T* out, float* part,
+                                            int c, int D) {
+    const int n8 = min(32, D - c) / 8;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+        float v[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) v[y] = any ? __uint_as_float(o[x * 8 + y]) * f : 0.f;
+        if (x >= n8) continue;
+        if (partial) {
+            if (part) {
+                reinterpret_cast<float4*>(part + c)[2 * x] = make_float4(v[0], v[1], v[2], v[3]);
+                reinterpret_cast<float4*>(part + c)[2 * x + 1] = make_float4(v[4], v[5], v[6], v[7]);
+            }
+        } else if (out) {
+            reinterpret_cast<uint4*>(out + c)[x] = make_uint4(pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3]),
+                                                              pack16<DT>(v[4], v[5]), pack16<DT>(v[6], v[7]));
+        }
+    }
+}
+constexpr float LN2 = 0.6931471805599453f;
+
 // ---------------------------------------------------------------- forward
 // One CTA: NT tiles of 128 queries of one (batch, head), over the key blocks of 128. A softmax
 // warpgroup per tile (thread = query row), a TMA warp and an MMA warp. Per tile and block:
@@ -276,13 +304,16 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     constexpr int W_LOAD = NT * 4, W_MMA = NT * 4 + 1;
     // causal: heads fastest and the longest rows first, so that the last CTAs to start are short
     const int tiles = (p.Sq + NT * 128 - 1) / (NT * 128), heads = p.B * p.H;
-    const int bh = p.causal ? blockIdx.x % heads : blockIdx.x / tiles;
+    const int split = blockIdx.x % p.splits, cta = blockIdx.x / p.splits;
+    const int bh = p.causal ? cta % heads : cta / tiles;
     const int h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hkv);
-    const int q0 = (p.causal ? tiles - 1 - blockIdx.x / heads : blockIdx.x % tiles) * (NT * 128);
+    const int q0 = (p.causal ? tiles - 1 - cta / heads : cta % tiles) * (NT * 128);
     const int ql = len_of(p.qlens, b, p.Sq), kl = len_of(p.kvlens, b, p.Sk);
     int end = q0 < ql ? kl : 0;
     if (p.causal) end = min(end, min(q0 + NT * 128, ql) - 1 + kl - ql + 1);
-    const int nblk = uniform(end > 0 ? (end + 127) / 128 : 0);
+    // this part's key blocks: blk0 .. blk0 + nblk - 1
+    const int all = end > 0 ? (end + 127) / 128 : 0, share = (all + p.splits - 1) / p.splits;
+    const int blk0 = split * share, nblk = uniform(max(0, min(all - blk0, share)));
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
@@ -315,7 +346,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 const int slot = i % Cf::SLOTS;
                 if (!mbar_wait(empty + slot, ((i / Cf::SLOTS) & 1) ^ 1, abort_flag)) { err = ERR_LOAD; break; }
                 mbar_expect_tx(full + slot, Cf::TILE);
-                load_tile<DP>((NT + slot) * Cf::TILE, smem, i & 1 ? &mv : &mk, full + slot, (i / 2) * 128, hk, b);
+                load_tile<DP>((NT + slot) * Cf::TILE, smem, i & 1 ? &mv : &mk, full + slot, (blk0 + i / 2) * 128, hk, b);
             }
             if (err || *abort_flag) {     // every load issued has to land before the CTA ends
                 *abort_flag = 1;
@@ -394,7 +425,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_addr + c * 32, sv + c * 32);
             tmem_ld_wait<128>(sv);
             float* s = reinterpret_cast<float*>(sv);
-            const int seen = row_end - j * 128;      // columns of this block that the row sees
+            const int seen = row_end - (blk0 + j) * 128;      // columns of this block that the row sees
             if (__any_sync(~0u, seen < 128)) {
 #pragma unroll
                 for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
@@ -445,11 +476,11 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 }
             }
             // keys past the sequence's length may hold anything
-            if (t == 0 && j == nblk - 1 && kl - j * 128 < 128) {
+            if (t == 0 && kl - (blk0 + j) * 128 < 128) {
                 const int iv = 2 * j + 1;
                 ok = warp_wait(full + iv % Cf::SLOTS, (iv / Cf::SLOTS) & 1, abort_flag);
                 if (!ok) break;
-                zero_tail<DP>(smem + (NT + iv % Cf::SLOTS) * Cf::TILE, kl - j * 128, row);
+                zero_tail<DP>(smem + (NT + iv % Cf::SLOTS) * Cf::TILE, kl - (blk0 + j) * 128, row);
             }
             tmem_st_wait();
             tc_fence_before();
@@ -462,29 +493,24 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         } else {
             tc_fence_after();
             const float inv = l > 0.f ? 1.f / l : 0.f;
+            const long long at = ((long long)b * p.H + h) * p.Sq + i;
             auto* out = i < p.Sq ? row_out<DT>(p.o, b, i, h) : nullptr;
+            float* part = i < p.Sq && p.splits > 1 ? p.part + ((long long)split * heads * p.Sq + at) * p.D : nullptr;
             for (int c = 0; c < p.D; c += 32) {
                 uint32_t o[32];
                 if (nblk > 0) {
                     tmem_ld32_issue(o_addr + c, o);
                     tmem_ld_wait<32>(o);
                 }
-                const int n8 = min(32, p.D - c) / 8;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        w[y] = nblk > 0 ? pack16<DT>(__uint_as_float(o[x * 8 + 2 * y]) * inv,
-                                                     __uint_as_float(o[x * 8 + 2 * y + 1]) * inv)
-                                        : 0u;
-                    if (out && x < n8)
-                        reinterpret_cast<uint4*>(out + c)[x] = make_uint4(w[0], w[1], w[2], w[3]);
-                }
+                store_chunk<DT>(o, nblk > 0, inv, p.splits > 1, out, part, c, p.D);
             }
-            if (p.lse && i < p.Sq)
-                p.lse[((long long)b * p.H + h) * p.Sq + i] =
-                    l > 0.f ? (m * p.scale2 + log2f(l)) * 0.6931471805599453f : -INFINITY;
+            if (i < p.Sq) {
+                const float lse2 = l > 0.f ? m * p.scale2 + log2f(l) : -INFINITY;
+                if (p.splits > 1)
+                    p.part_lse[(long long)split * heads * p.Sq + at] = lse2;
+                else if (p.lse)
+                    p.lse[at] = lse2 * LN2;
+            }
         }
     }
     if (err) atomicOr(p.err, err);
@@ -596,8 +622,9 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     const int rep = p.H / p.Hkv, heads = KV ? p.Hkv : p.H;
     // causal: heads fastest and the tiles with the longest rows (first columns) first
     const int tiles = ((KV ? p.Sk : p.Sq) + 127) / 128, bhs = p.B * heads;
-    const int bh = p.causal ? blockIdx.x % bhs : blockIdx.x / tiles;
-    const int tile_x = p.causal ? blockIdx.x / bhs : blockIdx.x % tiles;
+    const int split = blockIdx.x % p.splits, cta = blockIdx.x / p.splits;
+    const int bh = p.causal ? cta % bhs : cta / tiles;
+    const int tile_x = p.causal ? cta / bhs : cta % tiles;
     const int hx = bh % heads, b = bh / heads;                   // head of the kept tiles
     const int hy0 = KV ? hx * rep : hx / rep;                    // first head of the streamed ones
     const int r0 = (p.causal && !KV ? tiles - 1 - tile_x : tile_x) * 128;
@@ -614,6 +641,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         if (p.causal) end = min(end, min(r0 + 128, ql) + kl - ql);
         per = end > 0 ? (end + BN - 1) / BN : 0;
     }
+    // this part's share of them
+    const int share = (per + p.splits - 1) / p.splits;
+    first += split * share;
+    per = max(0, min(per - split * share, share));
     const int nblk = uniform(KV ? per * rep : per);
 
     if (threadIdx.x == 0) {
@@ -759,7 +790,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             float delta = 0.f;
             for (int x = 0; x < Cf::WG; ++x) delta += stat[row + x * 128];
             ds0 = -delta * p.scale;
-            if (ok && w == 0) {           // for the KV kernel
+            if (ok && w == 0 && split == 0) {   // for the KV kernel
                 alignas(16) typename Half16<DT>::T v[8];
                 three_parts<DT>(lse2 * p.lse_part, v);
                 three_parts<DT>(delta * -0.0625f, v + 3);
@@ -850,6 +881,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             const int rows = KV ? p.Sk : p.Sq;
             const View& view = !KV ? p.dq : w < HALF ? p.dk : p.dv;
             auto* out = r < rows ? row_out<DT>(view, b, r, hx) : nullptr;
+            // partial dV behind all of dK's
+            float* part = r < rows && p.splits > 1
+                              ? p.part + ((((KV && w >= HALF ? p.splits : 0) + (long long)split) * bhs + bh) * rows + r) * p.D
+                              : nullptr;
             const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w / HALF * DP : 0);
             for (int c = (KV ? w % HALF : w) * 32; c < p.D; c += (KV ? HALF : Cf::WG) * 32) {
                 uint32_t o[32];
@@ -857,16 +892,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                     tmem_ld32_issue(acc + c, o);
                     tmem_ld_wait<32>(o);
                 }
-                const int n8 = min(32, p.D - c) / 8;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    uint32_t v[4];
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        v[q] = nblk > 0 ? pack16<DT>(__uint_as_float(o[x * 8 + 2 * q]), __uint_as_float(o[x * 8 + 2 * q + 1]))
-                                        : 0u;
-                    if (out && x < n8) reinterpret_cast<uint4*>(out + c)[x] = make_uint4(v[0], v[1], v[2], v[3]);
-                }
+                store_chunk<DT>(o, nblk > 0, 1.f, p.splits > 1, out, part, c, p.D);
             }
         }
     }
@@ -877,6 +903,76 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Cf::TMEM_COLS));
     }
+}
+
+// ---------------------------------------------------------------- joining parts
+// One warp per row of [batch][head][token]: the parts in order. LSE: each weighted by 2^(its
+// log2 sum - the largest), their sum of weights into lse; else their sum.
+template <int DT, bool LSE>
+__global__ void __launch_bounds__(256) join_kernel(const Params p, const View out, const float* part, int T, int H) {
+    const int lane = threadIdx.x % 32;
+    const long long row = blockIdx.x * 8LL + threadIdx.x / 32, rows = (long long)p.B * H * T;
+    if (row >= rows) return;
+    const int t = (int)(row % T), h = (int)(row / T % H), b = (int)(row / T / H);
+    float top = -INFINITY, total = 0.f;
+    if (LSE) {
+        for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_lse[s * rows + row]);
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    }
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < p.splits; ++s) {
+        float w = 1.f;
+        if (LSE) {
+            const float l = p.part_lse[s * rows + row];
+            if (l == -INFINITY) continue;         // saw no key
+            w = exp2f(l - top);
+            total += w;
+        }
+        if (lane * 4 < p.D) {
+            const float4 v = *reinterpret_cast<const float4*>(part + (s * rows + row) * p.D + lane * 4);
+            acc = make_float4(fmaf(w, v.x, acc.x), fmaf(w, v.y, acc.y), fmaf(w, v.z, acc.z), fmaf(w, v.w, acc.w));
+        }
+    }
+    const float f = !LSE ? 1.f : total > 0.f ? 1.f / total : 0.f;
+    if (lane * 4 < p.D)
+        *reinterpret_cast<uint2*>(row_out<DT>(out, b, t, h) + lane * 4) =
+            make_uint2(pack16<DT>(acc.x * f, acc.y * f), pack16<DT>(acc.z * f, acc.w * f));
+    if (LSE && lane == 0 && p.lse) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
+}
+template <int DT, bool LSE>
+static int join(DeviceCtx* c, const Params& p, const View& out, const float* part, int T, int H) {
+    const long long blocks = ((long long)p.B * H * T + 7) / 8;
+    if (blocks > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
+    join_kernel<DT, LSE><<<(unsigned)blocks, 256, 0, c->compute>>>(p, out, part, T, H);
+    return after_launch(c);
+}
+
+// Parts of a streamed axis of `blocks` blocks for `ctas` tiles: as many as the places of CTAs on the
+// GPU's 148 SMs allow, each of two blocks at least. With half of the places filled or more there is
+// one part: joining costs another launch and the partial rows.
+static int parts(long long ctas, int blocks, int places) {
+    if (ctas <= 0 || ctas * 2 > places) return 1;
+    const long long n = places / ctas;
+    return (int)(n < blocks / 2 ? n : blocks / 2 < 1 ? 1 : blocks / 2);
+}
+// The split of each kernel of a problem and the workspace it takes.
+struct Plan {
+    int nt, fwd, dq, dkv;                 // query tiles of a forward CTA; parts
+    long long fwd_bytes, bwd_bytes, dq_at, dkv_at;
+};
+static Plan plan(int B, int H, int Hkv, int Sq, int Sk, int D) {
+    Plan n;
+    const long long qt = (Sq + 127) / 128, kt = (Sk + 127) / 128, bh = (long long)B * H, bhk = (long long)B * Hkv;
+    n.nt = Sq <= 128 ? 1 : 2;
+    n.fwd = parts((qt + n.nt - 1) / n.nt * bh, (int)kt, n.nt == 1 ? 296 : 148);
+    n.fwd_bytes = n.fwd > 1 ? n.fwd * bh * Sq * (D + 1) * 4 : 0;
+    const int places = D <= 64 ? 296 : 148, bn = D <= 64 ? 64 : 128;
+    n.dq = parts(qt * bh, (Sk + bn - 1) / bn, places);
+    n.dkv = parts(kt * bhk, (Sq + bn - 1) / bn, places);
+    n.dq_at = bh * stat_tiles(Sq) * STAT_TILE;
+    n.dkv_at = n.dq_at + (n.dq > 1 ? n.dq * bh * Sq * D * 4 : 0);
+    n.bwd_bytes = n.dkv_at + (n.dkv > 1 ? 2 * n.dkv * bhk * Sk * D * 4 : 0);
+    return n;
 }
 
 static int check_sizes(int nBatch, int nHeads, int nKvHeads, int nSq, int nSk, int nHeadDim) {
@@ -943,15 +1039,24 @@ static int launch_fwd(DeviceCtx* c, const Params& p) {
     if (st == OM_OK && p.Sk > 0) st = encode(&mk, p.k, p.B, p.Sk, p.Hkv, p.D, DT);
     if (st == OM_OK && p.Sk > 0) st = encode(&mv, p.v, p.B, p.Sk, p.Hkv, p.D, DT);
     if (st != OM_OK) return st;
-    const long long grid = (long long)((p.Sq + NT * 128 - 1) / (NT * 128)) * p.B * p.H;
+    const long long grid = (long long)((p.Sq + NT * 128 - 1) / (NT * 128)) * p.B * p.H * p.splits;
     if (grid > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
     kern<<<(unsigned)grid, Cf::THREADS, Cf::SMEM, c->compute>>>(mq, mk, mv, p);
     return after_launch(c);
 }
 template <int DT>
-static int forward(DeviceCtx* c, const Params& p) {
-    if (p.D <= 64) return p.Sq <= 128 ? launch_fwd<64, 1, DT>(c, p) : launch_fwd<64, 2, DT>(c, p);
-    return p.Sq <= 128 ? launch_fwd<128, 1, DT>(c, p) : launch_fwd<128, 2, DT>(c, p);
+static int forward(DeviceCtx* c, Params p, void* workspace) {
+    const Plan n = plan(p.B, p.H, p.Hkv, p.Sq, p.Sk, p.D);
+    p.splits = n.fwd;
+    p.part = static_cast<float*>(workspace);
+    p.part_lse = p.part + (long long)n.fwd * p.B * p.H * p.Sq * p.D;
+    if (n.fwd > 1 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16)) return OM_ERR_INVALID;
+    int st;
+    if (p.D <= 64)
+        st = n.nt == 1 ? launch_fwd<64, 1, DT>(c, p) : launch_fwd<64, 2, DT>(c, p);
+    else
+        st = n.nt == 1 ? launch_fwd<128, 1, DT>(c, p) : launch_fwd<128, 2, DT>(c, p);
+    return st == OM_OK && n.fwd > 1 ? join<DT, true>(c, p, p.o, p.part, p.Sq, p.H) : st;
 }
 
 // x1, x2: maps of the kept tiles (128 rows), y1, y2: of the streamed ones (BN rows)
@@ -965,13 +1070,13 @@ static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2
         OMB_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::SMEM));
         attr_set[c->device] = true;
     }
-    const long long n = (long long)(((KV ? p.Sk : p.Sq) + 127) / 128) * p.B * (KV ? p.Hkv : p.H);
+    const long long n = (long long)(((KV ? p.Sk : p.Sq) + 127) / 128) * p.B * (KV ? p.Hkv : p.H) * p.splits;
     if (n > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
     kern<<<(unsigned)n, Cf::THREADS, Cf::SMEM, c->compute>>>(x1, x2, y1, y2, p);
     return after_launch(c);
 }
 template <int DP, int DT>
-static int backward(DeviceCtx* c, const Params& p) {
+static int backward(DeviceCtx* c, Params p) {
     constexpr int BN = BwdCfg<DP>::BN;
     CUtensorMap m[2][4] = {};             // Q, K, V, dO; boxes of 128 and of BN rows
     const View* view[4] = {&p.q, &p.k, &p.v, &p.dout};
@@ -983,10 +1088,22 @@ static int backward(DeviceCtx* c, const Params& p) {
             if (st != OM_OK) return st;
         }
     }
-    // dQ first: it leaves the queries' statistics for dK and dV
+    const Plan n = plan(p.B, p.H, p.Hkv, p.Sq, p.Sk, p.D);
     int st = OM_OK;
-    if (p.Sq > 0) st = launch_bwd<DP, false, DT>(c, m[0][0], m[0][3], m[1][1], m[1][2], p);
-    if (st == OM_OK && p.Sk > 0) st = launch_bwd<DP, true, DT>(c, m[0][1], m[0][2], m[1][0], m[1][3], p);
+    if (p.Sq > 0) {                       // dQ first: it leaves the queries' statistics for dK and dV
+        p.splits = n.dq;
+        p.part = reinterpret_cast<float*>(p.stat + n.dq_at);
+        st = launch_bwd<DP, false, DT>(c, m[0][0], m[0][3], m[1][1], m[1][2], p);
+        if (st == OM_OK && n.dq > 1) st = join<DT, false>(c, p, p.dq, p.part, p.Sq, p.H);
+    }
+    if (st == OM_OK && p.Sk > 0) {
+        p.splits = n.dkv;
+        p.part = reinterpret_cast<float*>(p.stat + n.dkv_at);
+        st = launch_bwd<DP, true, DT>(c, m[0][1], m[0][2], m[1][0], m[1][3], p);
+        if (st == OM_OK && n.dkv > 1) st = join<DT, false>(c, p, p.dk, p.part, p.Sk, p.Hkv);
+        if (st == OM_OK && n.dkv > 1)
+            st = join<DT, false>(c, p, p.dv, p.part + (long long)n.dkv * p.B * p.Hkv * p.Sk * p.D, p.Sk, p.Hkv);
+    }
     return st;
 }
 
@@ -999,7 +1116,8 @@ extern "C" long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int n
                                                    int nSk, int nHeadDim, int bBackward) {
     const int st = attn::check_sizes(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim);
     if (st != OM_OK) return st;
-    return bBackward ? (long long)nBatch * nHeads * attn::stat_tiles(nSq) * attn::STAT_TILE : 0;
+    const attn::Plan n = attn::plan(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim);
+    return bBackward ? n.bwd_bytes : n.fwd_bytes;
 }
 
 extern "C" int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut,
@@ -1023,7 +1141,8 @@ extern "C" int omCudaAttention(const void* pQ, const void* pK, const void* pV, v
     p.B = nBatch; p.H = nHeads; p.Hkv = nKvHeads; p.Sq = nSq; p.Sk = nSk; p.D = nHeadDim;
     p.causal = bCausal != 0; p.err = c->err_word;
     attn::set_scale(&p, fScale);
-    return nDtype == OM_DTYPE_BF16 ? attn::forward<OM_DTYPE_BF16>(c, p) : attn::forward<OM_DTYPE_F16>(c, p);
+    return nDtype == OM_DTYPE_BF16 ? attn::forward<OM_DTYPE_BF16>(c, p, pWorkspace)
+                                    : attn::forward<OM_DTYPE_F16>(c, p, pWorkspace);
 }
 
 extern "C" int omCudaAttentionBackward(const void* pGradOut, const void* pQ, const void* pK,
