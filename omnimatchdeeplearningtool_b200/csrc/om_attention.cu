@@ -906,44 +906,53 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
 }
 
 // ---------------------------------------------------------------- joining parts
-// One warp per row of [batch][head][token]: the parts in order. LSE: each weighted by 2^(its
+// One warp per row of [batch][head][token]: the parts in a fixed order. LSE: each weighted by 2^(its
 // log2 sum - the largest), their sum of weights into lse; else their sum.
 template <int DT, bool LSE>
-__global__ void __launch_bounds__(256) join_kernel(const Params p, const View out, const float* part, int T, int H) {
+__global__ void __launch_bounds__(128) join_kernel(const Params p, const View out, const float* part, int T, int H) {
     const int lane = threadIdx.x % 32;
-    const long long row = blockIdx.x * 8LL + threadIdx.x / 32, rows = (long long)p.B * H * T;
+    const long long row = blockIdx.x * 4LL + threadIdx.x / 32, rows = (long long)p.B * H * T;
     if (row >= rows) return;
     const int t = (int)(row % T), h = (int)(row / T % H), b = (int)(row / T / H);
+    // lanes: `wide` float4 columns x 32 / wide parts at a time
+    const int cols = p.D / 4, wide = cols <= 2 ? 2 : cols <= 4 ? 4 : cols <= 8 ? 8 : cols <= 16 ? 16 : 32;
+    const int col = lane % wide, first = lane / wide, step = 32 / wide;
     float top = -INFINITY, total = 0.f;
     if (LSE) {
         for (int s = lane; s < p.splits; s += 32) top = fmaxf(top, p.part_lse[s * rows + row]);
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < p.splits; ++s) {
+#pragma unroll 4
+    for (int s = first; s < p.splits; s += step) {
         float w = 1.f;
-        if (LSE) {
+        if (LSE) {                                // 0 where the part saw no key; its row is zeros
             const float l = p.part_lse[s * rows + row];
-            if (l == -INFINITY) continue;         // saw no key
-            w = exp2f(l - top);
+            w = l == -INFINITY ? 0.f : exp2f(l - top);
             total += w;
         }
-        if (lane * 4 < p.D) {
-            const float4 v = *reinterpret_cast<const float4*>(part + (s * rows + row) * p.D + lane * 4);
-            acc = make_float4(fmaf(w, v.x, acc.x), fmaf(w, v.y, acc.y), fmaf(w, v.z, acc.z), fmaf(w, v.w, acc.w));
-        }
+        const float4 v = col < cols ? *reinterpret_cast<const float4*>(part + (s * rows + row) * p.D + col * 4)
+                                    : make_float4(0.f, 0.f, 0.f, 0.f);
+        acc = make_float4(fmaf(w, v.x, acc.x), fmaf(w, v.y, acc.y), fmaf(w, v.z, acc.z), fmaf(w, v.w, acc.w));
+    }
+    for (int o = 16; o >= wide; o >>= 1) {
+        acc.x += __shfl_xor_sync(~0u, acc.x, o);
+        acc.y += __shfl_xor_sync(~0u, acc.y, o);
+        acc.z += __shfl_xor_sync(~0u, acc.z, o);
+        acc.w += __shfl_xor_sync(~0u, acc.w, o);
+        if (LSE) total += __shfl_xor_sync(~0u, total, o);
     }
     const float f = !LSE ? 1.f : total > 0.f ? 1.f / total : 0.f;
-    if (lane * 4 < p.D)
+    if (lane < cols)
         *reinterpret_cast<uint2*>(row_out<DT>(out, b, t, h) + lane * 4) =
             make_uint2(pack16<DT>(acc.x * f, acc.y * f), pack16<DT>(acc.z * f, acc.w * f));
     if (LSE && lane == 0 && p.lse) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
 }
 template <int DT, bool LSE>
 static int join(DeviceCtx* c, const Params& p, const View& out, const float* part, int T, int H) {
-    const long long blocks = ((long long)p.B * H * T + 7) / 8;
+    const long long blocks = ((long long)p.B * H * T + 3) / 4;
     if (blocks > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-    join_kernel<DT, LSE><<<(unsigned)blocks, 256, 0, c->compute>>>(p, out, part, T, H);
+    join_kernel<DT, LSE><<<(unsigned)blocks, 128, 0, c->compute>>>(p, out, part, T, H);
     return after_launch(c);
 }
 
