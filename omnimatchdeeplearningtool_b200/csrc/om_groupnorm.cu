@@ -547,20 +547,20 @@ __global__ void gn_params_kernel(const float* ws, float* dgamma, float* dbeta, i
 __device__ __forceinline__ long long partial_at(const Params& p, int n, int value, int chunk, int c) {
     return (((long long)n * 2 + value) * p.nchunk + chunk) * p.Cs + c;
 }
-template <int DT, int ACT, bool BWD>
-__global__ void __launch_bounds__(T) gn_partial_kernel(const Params p) {
+template <int DT, int ACT, bool BWD, int GV>
+__global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_partial_kernel(const Params p) {
     extern __shared__ uint4 sm[];
     float* red = reinterpret_cast<float*>(sm);
     float* sums = red + T * 16;
     const Part t = part_of(p, blockIdx.z, blockIdx.y, blockIdx.x);
     if constexpr (BWD) {
-        BwdAffine<8> f;
-        bwd_affine_of<8>(p, t, f);
+        BwdAffine<GV> f;
+        bwd_affine_of<GV>(p, t, f);
         float a[8] = {}, b[8] = {};
-#pragma unroll 4
+#pragma unroll 2
         for (int r = t.first; r < t.end; r += t.step) {
             float dz[8], xh[8];
-            bwd_terms<DT, ACT, 8>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
+            bwd_terms<DT, ACT, GV>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 a[i] += dz[i];
@@ -667,20 +667,20 @@ __global__ void __launch_bounds__(T) gn_combine_kernel(const Params p, float* st
     }
 }
 // The last chunks first: they are the ones that the partial pass left in L2.
-template <int DT, int ACT, bool BWD>
-__global__ void __launch_bounds__(T) gn_apply_kernel(const Params p, const float* stat) {
+template <int DT, int ACT, bool BWD, int GV>
+__global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_apply_kernel(const Params p, const float* stat) {
     const Part t = part_of(p, gridDim.z - 1 - blockIdx.z, gridDim.y - 1 - blockIdx.y, gridDim.x - 1 - blockIdx.x);
     const float* s = stat + 2 * (long long)t.n * p.G;
     if constexpr (BWD) {
-        BwdAffine<8> f;
-        bwd_affine_of<8>(p, t, f);
-        float m1[8], m2[8];
-        bwd_means_of<8>(p, t, f, s, 0, m1, m2);
-#pragma unroll 4
+        BwdAffine<GV> f;
+        bwd_affine_of<GV>(p, t, f);
+        float m1[GV], m2[GV];
+        bwd_means_of<GV>(p, t, f, s, 0, m1, m2);
+#pragma unroll 2
         for (int r = t.first; r < t.end; r += t.step) {
             float dz[8], xh[8];
-            bwd_terms<DT, ACT, 8>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
-            store<DT>(p.out, at(p, t, r), bwd_out<DT, 8>(dz, xh, f, m1, m2));
+            bwd_terms<DT, ACT, GV>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
+            store<DT>(p.out, at(p, t, r), bwd_out<DT, GV>(dz, xh, f, m1, m2));
         }
     } else {
         Affine<DT> f;
@@ -787,11 +787,16 @@ static int launch(DeviceCtx* c, Params p, size_t smem) {
         float* stat = chan + (BWD ? 2LL * p.N * p.C : 0);
         p.ws = stat + 2LL * p.N * p.G;
         const dim3 grid(p.nchunk, p.nslab, p.N);
-        gn_partial_kernel<DT, ACT, BWD><<<grid, T, smem, c->compute>>>(p);
+        const int gv = BWD ? entries(p.cpg) : 8;
+        (gv == 1   ? gn_partial_kernel<DT, ACT, BWD, BWD ? 1 : 8>
+         : gv == 2 ? gn_partial_kernel<DT, ACT, BWD, BWD ? 2 : 8>
+                   : gn_partial_kernel<DT, ACT, BWD, 8>)<<<grid, T, smem, c->compute>>>(p);
         if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
         gn_combine_kernel<BWD><<<dim3(p.G, p.N), T, 0, c->compute>>>(p, stat, chan);
         if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
-        gn_apply_kernel<DT, ACT, BWD><<<grid, T, 0, c->compute>>>(p, stat);
+        (gv == 1   ? gn_apply_kernel<DT, ACT, BWD, BWD ? 1 : 8>
+         : gv == 2 ? gn_apply_kernel<DT, ACT, BWD, BWD ? 2 : 8>
+                   : gn_apply_kernel<DT, ACT, BWD, 8>)<<<grid, T, 0, c->compute>>>(p, stat);
         if (after_launch(c) != OM_OK) return OM_ERR_CUDA;
         p.ws = chan;
     }
