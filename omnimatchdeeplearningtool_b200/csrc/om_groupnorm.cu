@@ -17,6 +17,7 @@
 #include <cooperative_groups.h>
 
 #include "om_common.cuh"
+#include "om_f2.cuh"
 
 namespace omb {
 namespace gn {
@@ -39,34 +40,39 @@ template <> struct Elem<OM_DTYPE_F16> { using T = __half; static constexpr int V
 template <int DT> struct Vec { uint4 q[Elem<DT>::V16]; };
 
 template <int DT>
-__device__ __forceinline__ void unpack(const Vec<DT>& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack(const Vec<DT>& v, F2 (&f)[4]) {
     if constexpr (DT == OM_DTYPE_F32) {
         const float* s = reinterpret_cast<const float*>(&v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = s[i];
+        for (int i = 0; i < 4; ++i) f[i] = {s[2 * i], s[2 * i + 1]};
     } else {
         const auto* s = reinterpret_cast<const typename Half16<DT>::T2*>(&v);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 u = Half16<DT>::unpack(s[i]);
-            f[2 * i] = u.x;
-            f[2 * i + 1] = u.y;
+            f[i] = {u.x, u.y};
         }
     }
 }
 template <int DT>
-__device__ __forceinline__ Vec<DT> pack(const float (&f)[8]) {
+__device__ __forceinline__ Vec<DT> pack(const F2 (&f)[4]) {
     Vec<DT> v;
     if constexpr (DT == OM_DTYPE_F32) {
         float* d = reinterpret_cast<float*>(&v);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] = f[i];
+        for (int i = 0; i < 4; ++i) { d[2 * i] = f[i].x; d[2 * i + 1] = f[i].y; }
     } else {
         auto* d = reinterpret_cast<typename Half16<DT>::T2*>(&v);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = Half16<DT>::pack(f[2 * i], f[2 * i + 1]);
+        for (int i = 0; i < 4; ++i) d[i] = Half16<DT>::pack(f[i].x, f[i].y);
     }
     return v;
+}
+// channels past nval (stored padding) as zeros, whatever they hold
+__device__ __forceinline__ void cut(F2 (&f)[4], int nval) {
+    if (nval < 8)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = {2 * i < nval ? f[i].x : 0.f, 2 * i + 1 < nval ? f[i].y : 0.f};
 }
 template <int DT>
 __device__ __forceinline__ Vec<DT> load(const void* base, long long elem) {
@@ -101,26 +107,30 @@ __device__ __forceinline__ Vec<DT> own(const uint4* sm, int s) {
     return v;
 }
 // sigmoid(z) = 1 / (1 + 2^(-z log2 e)): an overflowing power gives 0
-__device__ __forceinline__ float sigmoid(float z) {
-    float e, s;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
+__device__ __forceinline__ F2 sigmoid(F2 z) {
+    F2 e = mul2(z, {-1.4426950408889634f, -1.4426950408889634f}), s;
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(e.y));
+    e = add2(e, {1.f, 1.f});
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s.y) : "f"(e.y));
     return s;
 }
 template <int ACT>
-__device__ __forceinline__ float act_fwd(float z) {
-    if (ACT == OM_ACT_SILU) return z * sigmoid(z);
-    return apply_act(z, ACT);
+__device__ __forceinline__ F2 act_fwd(F2 z) {
+    if (ACT == OM_ACT_SILU) return mul2(z, sigmoid(z));
+    return {apply_act(z.x, ACT), apply_act(z.y, ACT)};
 }
 // dz = dy * act'(z)
 template <int ACT>
-__device__ __forceinline__ float act_bwd(float dy, float z) {
-    if (ACT == OM_ACT_SILU) {
-        const float s = sigmoid(z);
-        return dy * s * fmaf(z, 1.f - s, 1.f);
+__device__ __forceinline__ F2 act_bwd(F2 dy, F2 z) {
+    if (ACT == OM_ACT_SILU) {             // s (1 + z (1 - s))
+        const F2 s = sigmoid(z), zs = mul2(z, s);
+        return mul2(dy, mul2(s, add2(fma2(zs, {-1.f, -1.f}, z), {1.f, 1.f})));
     }
-    if (ACT == OM_ACT_RELU) return z > 0.f ? dy : 0.f;
-    if (ACT == OM_ACT_RELU6) return z > 0.f && z < 6.f ? dy : 0.f;
+    if (ACT == OM_ACT_RELU) return {z.x > 0.f ? dy.x : 0.f, z.y > 0.f ? dy.y : 0.f};
+    if (ACT == OM_ACT_RELU6)
+        return {z.x > 0.f && z.x < 6.f ? dy.x : 0.f, z.y > 0.f && z.y < 6.f ? dy.y : 0.f};
     return dy;
 }
 
@@ -210,28 +220,48 @@ struct Stats {
         for (int g = 0; g < GV; ++g) mean[g] = m2[g] = 0.f;
     }
     template <int B>
-    __device__ __forceinline__ void add(const float (&v)[B][8]) {
-        constexpr int PER = 8 / GV;
-        constexpr float cnt = B * PER;
+    __device__ __forceinline__ void add(const F2 (&v)[B][4]) {
+        constexpr float cnt = B * (8 / GV);
         const float w = __fdividef(cnt, n + cnt), k = n * w;
-#pragma unroll
-        for (int g = 0; g < GV; ++g) {
-            float s = 0.f, q = 0.f;
-#pragma unroll
-            for (int j = 0; j < B; ++j)
-#pragma unroll
-                for (int i = 0; i < PER; ++i) s += v[j][g * PER + i];
-            const float m = s * (1.f / cnt);
-#pragma unroll
-            for (int j = 0; j < B; ++j)
-#pragma unroll
-                for (int i = 0; i < PER; ++i) {
-                    const float e = v[j][g * PER + i] - m;
-                    q = fmaf(e, e, q);
-                }
+        auto merge = [&](int g, float m, float q) {
             const float d = m - mean[g];
             mean[g] = fmaf(d, w, mean[g]);
             m2[g] += fmaf(d * d, k, q);
+        };
+        if constexpr (GV == 8) {              // both halves of a pair are entries of their own
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                F2 s = v[0][i], q = {0.f, 0.f};
+#pragma unroll
+                for (int j = 1; j < B; ++j) s = add2(s, v[j][i]);
+                const F2 m = mul2(s, {1.f / cnt, 1.f / cnt}), nm = {-m.x, -m.y};
+#pragma unroll
+                for (int j = 0; j < B; ++j) {
+                    const F2 e = add2(v[j][i], nm);
+                    q = fma2(e, e, q);
+                }
+                merge(2 * i, m.x, q.x);
+                merge(2 * i + 1, m.y, q.y);
+            }
+        } else {
+            constexpr int PAIRS = 4 / GV;
+#pragma unroll
+            for (int g = 0; g < GV; ++g) {
+                F2 s = {0.f, 0.f}, q = {0.f, 0.f};
+#pragma unroll
+                for (int j = 0; j < B; ++j)
+#pragma unroll
+                    for (int i = 0; i < PAIRS; ++i) s = add2(s, v[j][g * PAIRS + i]);
+                const float m = (s.x + s.y) * (1.f / cnt);
+#pragma unroll
+                for (int j = 0; j < B; ++j)
+#pragma unroll
+                    for (int i = 0; i < PAIRS; ++i) {
+                        const F2 e = add2(v[j][g * PAIRS + i], {-m, -m});
+                        q = fma2(e, e, q);
+                    }
+                merge(g, m, q.x + q.y);
+            }
         }
         n += cnt;
     }
@@ -265,36 +295,37 @@ __device__ void block_stats(const Params& p, const Stats<GV>& st, float count, f
 // into the shift (its rounding, 2^-24 of mean * scale, is far below the output's). Padding: 0.
 template <int DT>
 struct Affine {
-    float mean[DT == OM_DTYPE_F32 ? 8 : 1], scale[8], shift[8];
+    F2 minus_mean[DT == OM_DTYPE_F32 ? 4 : 1], scale[4], shift[4];
 };
+__device__ __forceinline__ float& half_of(F2* f, int i) { return i % 2 ? f[i / 2].y : f[i / 2].x; }
 template <int DT, class MeanOf, class RstdOf>
 __device__ __forceinline__ void affine_of(const Params& p, const Part& t, Affine<DT>& f, MeanOf mean_of, RstdOf rstd_of) {
     int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);     // group of the channel, channels left in it
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        float m = 0.f;
-        f.scale[i] = f.shift[i] = 0.f;
+        float m = 0.f, scale = 0.f, shift = 0.f;
         if (i < t.nval) {
             const int c = t.c0 + i;
             m = mean_of(g);
-            f.scale[i] = rstd_of(g) * (p.gamma ? p.gamma[c] : 1.f);
-            f.shift[i] = p.beta ? p.beta[c] : 0.f;
-            if (DT != OM_DTYPE_F32) f.shift[i] = fmaf(-m, f.scale[i], f.shift[i]);
+            scale = rstd_of(g) * (p.gamma ? p.gamma[c] : 1.f);
+            shift = p.beta ? p.beta[c] : 0.f;
+            if (DT != OM_DTYPE_F32) shift = fmaf(-m, scale, shift);
         }
-        if (DT == OM_DTYPE_F32) f.mean[i] = m;
+        half_of(f.scale, i) = scale;
+        half_of(f.shift, i) = shift;
+        if (DT == OM_DTYPE_F32) half_of(f.minus_mean, i) = -m;
         if (--left == 0) { ++g; left = p.cpg; }
     }
 }
 template <int DT, int ACT>
 __device__ __forceinline__ Vec<DT> apply(const Vec<DT>& v, const Affine<DT>& f, int nval) {
-    float x[8];
+    F2 x[4];
     unpack<DT>(v, x);
-    if (nval < 8)
+    cut(x, nval);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i < nval ? x[i] : 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = act_fwd<ACT>(fmaf(DT == OM_DTYPE_F32 ? x[i] - f.mean[i] : x[i], f.scale[i], f.shift[i]));
+    for (int i = 0; i < 4; ++i)
+        x[i] = act_fwd<ACT>(fma2(DT == OM_DTYPE_F32 ? add2(x[i], f.minus_mean[DT == OM_DTYPE_F32 ? i : 0]) : x[i],
+                                 f.scale[i], f.shift[i]));
     return pack<DT>(x);
 }
 
@@ -326,13 +357,13 @@ __global__ void __launch_bounds__(T, 4) gn_fwd_unit_kernel(const Params p) {
     st.clear();
     auto take = [&](int s, int end) {
         for (; s + 3 < end; s += 4) {
-            float v[4][8];
+            F2 v[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) unpack<DT>(own<DT>(sm, s + j), v[j]);
             st.template add<4>(v);
         }
         for (; s < end; ++s) {
-            float v[1][8];
+            F2 v[1][4];
             unpack<DT>(own<DT>(sm, s), v[0]);
             st.template add<1>(v);
         }
@@ -360,18 +391,24 @@ __global__ void __launch_bounds__(T, 4) gn_fwd_unit_kernel(const Params p) {
     }
     if (p.cluster > 1) cl.sync(); else __syncthreads();
     for (int g = threadIdx.x; g < ng; g += T) {
-        float m = 0.f, q = 0.f;
-        for (int k = 0; k < p.cluster; ++k) {
-            const float cnt = (float)max(0, min((k + 1) * p.rows, p.HW) - k * p.rows);
-            m += cnt * cl.map_shared_rank(group, k)[2 * g];
-        }
+        // all CTAs' values are on their way before the first is used (one by one their latencies
+        // added up to a sixth of the kernel)
+        float mk[MAX_CLUSTER], qk[MAX_CLUSTER], m = 0.f, q = 0.f;
+#pragma unroll
+        for (int k = 0; k < MAX_CLUSTER; ++k)
+            if (k < p.cluster) {
+                const float* o = cl.map_shared_rank(group, k);
+                mk[k] = o[2 * g];
+                qk[k] = o[2 * g + 1];
+            }
+        auto pixels = [&](int k) { return (float)max(0, min((k + 1) * p.rows, p.HW) - k * p.rows); };
+#pragma unroll
+        for (int k = 0; k < MAX_CLUSTER; ++k)
+            if (k < p.cluster) m = fmaf(pixels(k), mk[k], m);
         m /= (float)p.HW;
-        for (int k = 0; k < p.cluster; ++k) {
-            const float cnt = (float)max(0, min((k + 1) * p.rows, p.HW) - k * p.rows);
-            const float* o = cl.map_shared_rank(group, k);
-            const float d = o[2 * g] - m;
-            q += o[2 * g + 1] + cnt * (float)p.cpg * d * d;
-        }
+#pragma unroll
+        for (int k = 0; k < MAX_CLUSTER; ++k)
+            if (k < p.cluster) q += fmaf(pixels(k) * (float)p.cpg * (mk[k] - m), mk[k] - m, qk[k]);
         const float rs = 1.f / sqrtf(q / ((float)p.HW * (float)p.cpg) + p.eps);
         total[2 * g] = m;
         total[2 * g + 1] = rs;
@@ -392,8 +429,14 @@ __global__ void __launch_bounds__(T, 4) gn_fwd_unit_kernel(const Params p) {
 // i belongs to entry i * GV / 8).
 template <int GV>
 struct BwdAffine {
-    float mean[GV], rstd[GV], gamma[8], beta[8];
+    float minus_mean[GV], rstd[GV];
+    F2 gamma[4], beta[4];
 };
+// the pair i of a vector from values per entry
+template <int GV>
+__device__ __forceinline__ F2 pair_of(const float (&v)[GV], int i) {
+    return {v[2 * i * GV / 8], v[(2 * i + 1) * GV / 8]};
+}
 template <int GV>
 __device__ __forceinline__ void bwd_affine_of(const Params& p, const Part& t, BwdAffine<GV>& f) {
     int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);
@@ -401,15 +444,15 @@ __device__ __forceinline__ void bwd_affine_of(const Params& p, const Part& t, Bw
     for (int i = 0; i < 8; ++i) {
         const bool in = i < t.nval;
         if (i % (8 / GV) == 0) {
-            f.mean[i * GV / 8] = in ? p.mean[(long long)t.n * p.G + g] : 0.f;
+            f.minus_mean[i * GV / 8] = in ? -p.mean[(long long)t.n * p.G + g] : 0.f;
             f.rstd[i * GV / 8] = in ? p.rstd[(long long)t.n * p.G + g] : 0.f;
         }
-        f.gamma[i] = !in ? 0.f : p.gamma ? p.gamma[t.c0 + i] : 1.f;
-        f.beta[i] = in && p.beta ? p.beta[t.c0 + i] : 0.f;
+        half_of(f.gamma, i) = !in ? 0.f : p.gamma ? p.gamma[t.c0 + i] : 1.f;
+        half_of(f.beta, i) = in && p.beta ? p.beta[t.c0 + i] : 0.f;
         if (--left == 0) { ++g; left = p.cpg; }
     }
 }
-// rstd times the means of t and t xh, from pairs of means per group starting at group g0
+// minus rstd times the means of t and t xh, from pairs of means per group starting at group g0
 template <int GV>
 __device__ __forceinline__ void bwd_means_of(const Params& p, const Part& t, const BwdAffine<GV>& f, const float* pairs,
                                              int g0, float (&m1)[GV], float (&m2)[GV]) {
@@ -417,8 +460,8 @@ __device__ __forceinline__ void bwd_means_of(const Params& p, const Part& t, con
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         if (i % (8 / GV) == 0) {
-            m1[i * GV / 8] = i < t.nval ? f.rstd[i * GV / 8] * pairs[2 * (g - g0)] : 0.f;
-            m2[i * GV / 8] = i < t.nval ? f.rstd[i * GV / 8] * pairs[2 * (g - g0) + 1] : 0.f;
+            m1[i * GV / 8] = i < t.nval ? -f.rstd[i * GV / 8] * pairs[2 * (g - g0)] : 0.f;
+            m2[i * GV / 8] = i < t.nval ? -f.rstd[i * GV / 8] * pairs[2 * (g - g0) + 1] : 0.f;
         }
         if (--left == 0) { ++g; left = p.cpg; }
     }
@@ -426,29 +469,37 @@ __device__ __forceinline__ void bwd_means_of(const Params& p, const Part& t, con
 // dz and xh of 8 channels of one pixel (0 for padding, whatever it holds)
 template <int DT, int ACT, int GV>
 __device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy, const BwdAffine<GV>& f, int nval,
-                                          float (&dz)[8], float (&xh)[8]) {
+                                          F2 (&dz)[4], F2 (&xh)[4]) {
     unpack<DT>(vx, xh);
     unpack<DT>(vdy, dz);
-    if (nval < 8)
+    cut(xh, nval);
+    cut(dz, nval);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            xh[i] = i < nval ? xh[i] : 0.f;
-            dz[i] = i < nval ? dz[i] : 0.f;
-        }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        xh[i] = (xh[i] - f.mean[i * GV / 8]) * f.rstd[i * GV / 8];
-        dz[i] = act_bwd<ACT>(dz[i], fmaf(xh[i], f.gamma[i], f.beta[i]));
+    for (int i = 0; i < 4; ++i) {
+        xh[i] = mul2(add2(xh[i], pair_of<GV>(f.minus_mean, i)), pair_of<GV>(f.rstd, i));
+        dz[i] = act_bwd<ACT>(dz[i], fma2(xh[i], f.gamma[i], f.beta[i]));
     }
 }
-// dx = rstd (gamma dz - mean(t) - xh mean(t xh)), m1 and m2 with their rstd
-template <int DT, int GV>
-__device__ __forceinline__ Vec<DT> bwd_out(const float (&dz)[8], const float (&xh)[8], const BwdAffine<GV>& f,
-                                           const float (&m1)[GV], const float (&m2)[GV]) {
-    float d[8];
+// the sums that a thread keeps of them: dz, and dz xh
+__device__ __forceinline__ void bwd_add(const F2 (&dz)[4], const F2 (&xh)[4], F2 (&a)[4], F2 (&b)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        d[i] = fmaf(dz[i] * f.gamma[i], f.rstd[i * GV / 8], -fmaf(xh[i], m2[i * GV / 8], m1[i * GV / 8]));
+    for (int i = 0; i < 4; ++i) {
+        a[i] = add2(a[i], dz[i]);
+        b[i] = fma2(dz[i], xh[i], b[i]);
+    }
+}
+__device__ __forceinline__ void flat(const F2 (&v)[4], float (&f)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[2 * i] = v[i].x; f[2 * i + 1] = v[i].y; }
+}
+// dx = rstd (gamma dz - mean(t) - xh mean(t xh)); m1 and m2: minus the means, with their rstd
+template <int DT, int GV>
+__device__ __forceinline__ Vec<DT> bwd_out(const F2 (&dz)[4], const F2 (&xh)[4], const BwdAffine<GV>& f,
+                                           const float (&m1)[GV], const float (&m2)[GV]) {
+    F2 d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        d[i] = fma2(mul2(dz[i], f.gamma[i]), pair_of<GV>(f.rstd, i), fma2(xh[i], pair_of<GV>(m2, i), pair_of<GV>(m1, i)));
     return pack<DT>(d);
 }
 
@@ -478,28 +529,30 @@ __global__ void __launch_bounds__(T, GV == 8 ? 2 : 3) gn_bwd_unit_kernel(const P
     }
     BwdAffine<GV> f;
     bwd_affine_of<GV>(p, t, f);
-    float a[8] = {}, b[8] = {};
+    F2 a2[4] = {}, b2[4] = {};
     auto take = [&](int s, int end) {
         for (; s < end; ++s) {
-            float dz[8], xh[8];
+            F2 dz[4], xh[4];
             bwd_terms<DT, ACT, GV>(own<DT>(sm, s), own<DT>(sm_dy, s), f, t.nval, dz, xh);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                a[i] += dz[i];
-                b[i] = fmaf(dz[i], xh[i], b[i]);
-            }
+            bwd_add(dz, xh, a2, b2);
         }
     };
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     take(0, half);
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     take(half, mine_rows);
+    float a[8], b[8];
+    flat(a2, a);
+    flat(b2, b);
     reduce_columns<8>(p, a, b, red, sums);
     if (p.cluster > 1) cl.sync();
     const int c_lo = slab * p.vc * 8, nc = max(0, min(p.C - c_lo, p.vc * 8));
     for (int c = threadIdx.x; c < p.vc * 16; c += T) {
-        float v = 0.f;
-        for (int k = 0; k < p.cluster; ++k) v += cl.map_shared_rank(sums, k)[c];
+        float vk[MAX_CLUSTER], v = 0.f;     // on their way together
+#pragma unroll
+        for (int k = 0; k < MAX_CLUSTER; ++k) vk[k] = k < p.cluster ? cl.map_shared_rank(sums, k)[c] : 0.f;
+#pragma unroll
+        for (int k = 0; k < MAX_CLUSTER; ++k) v += vk[k];
         total[c] = v;
         if (rank == 0 && p.ws && c % (p.vc * 8) < nc)
             p.ws[((long long)(c / (p.vc * 8)) * p.N + n) * p.C + c_lo + c % (p.vc * 8)] = v;
@@ -522,7 +575,7 @@ __global__ void __launch_bounds__(T, GV == 8 ? 2 : 3) gn_bwd_unit_kernel(const P
     bwd_means_of<GV>(p, t, f, means, c_lo / p.cpg, m1, m2);
     long long e = at(p, t, t.first);
     for (int s = 0; s < mine_rows; ++s, e += step) {
-        float dz[8], xh[8];
+        F2 dz[4], xh[4];
         bwd_terms<DT, ACT, GV>(own<DT>(sm, s), own<DT>(sm_dy, s), f, t.nval, dz, xh);
         store<DT>(p.out, e, bwd_out<DT, GV>(dz, xh, f, m1, m2));
     }
@@ -556,17 +609,16 @@ __global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_partial_kernel(const Pa
     if constexpr (BWD) {
         BwdAffine<GV> f;
         bwd_affine_of<GV>(p, t, f);
-        float a[8] = {}, b[8] = {};
+        F2 a2[4] = {}, b2[4] = {};
 #pragma unroll 2
         for (int r = t.first; r < t.end; r += t.step) {
-            float dz[8], xh[8];
+            F2 dz[4], xh[4];
             bwd_terms<DT, ACT, GV>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                a[i] += dz[i];
-                b[i] = fmaf(dz[i], xh[i], b[i]);
-            }
+            bwd_add(dz, xh, a2, b2);
         }
+        float a[8], b[8];
+        flat(a2, a);
+        flat(b2, b);
         reduce_columns<8>(p, a, b, red, sums);
     } else {
         Stats<8> st;
@@ -574,7 +626,7 @@ __global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_partial_kernel(const Pa
         int r = t.first;
         for (; r + 3 * t.step < t.end; r += 4 * t.step) {
             Vec<DT> q[4];
-            float v[4][8];
+            F2 v[4][4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) q[j] = load<DT>(p.x, at(p, t, r + j * t.step));
 #pragma unroll
@@ -582,7 +634,7 @@ __global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_partial_kernel(const Pa
             st.template add<4>(v);
         }
         for (; r < t.end; r += t.step) {
-            float v[1][8];
+            F2 v[1][4];
             unpack<DT>(load<DT>(p.x, at(p, t, r)), v[0]);
             st.template add<1>(v);
         }
@@ -678,7 +730,7 @@ __global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_apply_kernel(const Para
         bwd_means_of<GV>(p, t, f, s, 0, m1, m2);
 #pragma unroll 2
         for (int r = t.first; r < t.end; r += t.step) {
-            float dz[8], xh[8];
+            F2 dz[4], xh[4];
             bwd_terms<DT, ACT, GV>(load<DT>(p.x, at(p, t, r)), load<DT>(p.dy, at(p, t, r)), f, t.nval, dz, xh);
             store<DT>(p.out, at(p, t, r), bwd_out<DT, GV>(dz, xh, f, m1, m2));
         }
