@@ -208,28 +208,35 @@ __device__ __forceinline__ void zero_tail(uint8_t* tile, int first, int row) {
     fence_async_smem();
 }
 
-// Columns c .. c + 31 of one row from the accumulators o (zeros unless `any`), times f: to a row of
-// partial results, or rounded to the output row; nothing for a row that is not there.
-template <int DT, class T>
-__device__ __forceinline__ void store_chunk(const uint32_t (&o)[32], bool any, float f, bool partial, T* out, float* part,
-                                            int c, int D) {
+// Columns c .. c + 31 of row `row` from the accumulators o (zeros unless `any`), times f: rounded into
+// the 128-row tile at `tile` (panels of 64 columns with the 128-byte swizzle, for a TMA store: stored
+// from the registers, 16 bytes to each of 32 rows at a time, the epilogue took 2400 to 4200 clocks of
+// a CTA), or in fp32 to a row of partial results, when it is there.
+template <int DT>
+__device__ __forceinline__ void store_chunk(const uint32_t (&o)[32], bool any, float f, bool partial, uint8_t* tile, int row,
+                                            float* part, int c, int D) {
     const int n8 = min(32, D - c) / 8;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
         float v[8];
 #pragma unroll
         for (int y = 0; y < 8; ++y) v[y] = any ? __uint_as_float(o[x * 8 + y]) * f : 0.f;
-        if (x >= n8) continue;
-        if (partial) {
-            if (part) {
-                reinterpret_cast<float4*>(part + c)[2 * x] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(part + c)[2 * x + 1] = make_float4(v[4], v[5], v[6], v[7]);
-            }
-        } else if (out) {
-            reinterpret_cast<uint4*>(out + c)[x] = make_uint4(pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3]),
-                                                              pack16<DT>(v[4], v[5]), pack16<DT>(v[6], v[7]));
+        if (!partial) {
+            *reinterpret_cast<uint4*>(tile + c / 64 * PANEL + row * 128 + (((c % 64 / 8 + x) ^ (row & 7)) << 4)) =
+                make_uint4(pack16<DT>(v[0], v[1]), pack16<DT>(v[2], v[3]), pack16<DT>(v[4], v[5]), pack16<DT>(v[6], v[7]));
+        } else if (part && x < n8) {
+            reinterpret_cast<float4*>(part + c)[2 * x] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(part + c)[2 * x + 1] = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
+}
+// A tile's panels to rows t0 .. of one batch entry and head; what lies past the tensor is dropped.
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, const uint8_t* tile, int D, int t0, int h, int b) {
+    for (int c = 0; c < D; c += 64)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+                reinterpret_cast<uint64_t>(map)), "r"(smem_u32(tile + c / 64 * PANEL)), "r"(c), "r"(t0), "r"(h), "r"(b)
+            : "memory");
 }
 constexpr float LN2 = 0.6931471805599453f;
 
@@ -261,7 +268,7 @@ enum : unsigned int { ERR_LOAD = ERRBIT_TC_PRODUCER, ERR_MMA = ERRBIT_TC_MMA,
 template <int DP, int NT, int DT>
 __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                const __grid_constant__ CUtensorMap mv, const Params p) {
+                const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Params p) {
     using Cf = FwdCfg<DP, NT>;
     using H16 = Half16<DT>;
     extern __shared__ uint8_t smem_raw[];
@@ -273,7 +280,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     uint64_t* s_full = bars + 3;
     uint64_t* p_full = s_full + Cf::NB;
     uint64_t* pv_done = p_full + Cf::NB;
-    uint64_t* full = pv_done + NT;
+    uint64_t* out_ready = pv_done + NT;
+    uint64_t* full = out_ready + NT;
     uint64_t* empty = full + Cf::SLOTS;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
@@ -298,7 +306,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         mbar_init(o_full, 1);
         mbar_init(drain, 1);
         for (int i = 0; i < Cf::NB; ++i) { mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); }
-        for (int t = 0; t < NT; ++t) mbar_init(pv_done + t, 1);
+        for (int t = 0; t < NT; ++t) { mbar_init(pv_done + t, 1); mbar_init(out_ready + t, 4); }
         for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -472,7 +480,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             tc_fence_after();
             const float inv = l > 0.f ? 1.f / l : 0.f;
             const long long at = ((long long)b * p.H + h) * p.Sq + i;
-            auto* out = i < p.Sq ? row_out<DT>(p.o, b, i, h) : nullptr;
+            uint8_t* tile = smem + t * Cf::TILE;      // Q's, which every product has read
             float* part = i < p.Sq && p.splits > 1 ? p.part + ((long long)split * heads * p.Sq + at) * p.D : nullptr;
             for (int c = 0; c < p.D; c += 32) {
                 uint32_t o[32];
@@ -480,7 +488,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     tmem_ld32_issue(o_addr + c, o);
                     tmem_ld_wait<32>(o);
                 }
-                store_chunk<DT>(o, nblk > 0, inv, p.splits > 1, out, part, c, p.D);
+                store_chunk<DT>(o, nblk > 0, inv, p.splits > 1, tile, row, part, c, p.D);
             }
             if (i < p.Sq) {
                 const float lse2 = l > 0.f ? m * p.scale2 + log2f(l) : -INFINITY;
@@ -488,6 +496,19 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     p.part_lse[(long long)split * heads * p.Sq + at] = lse2;
                 else if (p.lse)
                     p.lse[at] = lse2 * LN2;
+            }
+            if (p.splits == 1) {
+                fence_async_smem();
+                warp_arrive(out_ready + t);
+                if (warp % 4 == 0) {
+                    if (!warp_wait(out_ready + t, 0, abort_flag)) {
+                        err = ERR_MATH;
+                    } else if (lane == 0 && q0 + t * 128 < p.Sq) {
+                        store_tile(&mo, tile, p.D, q0 + t * 128, h, b);
+                        bulk_commit();
+                        bulk_wait_read<0>();
+                    }
+                }
             }
         }
     }
@@ -582,14 +603,14 @@ template <int DP, bool KV, int DT>
 __global__ void __launch_bounds__(BwdCfg<DP>::THREADS, BwdCfg<DP>::OCC)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__ CUtensorMap mx2,
                 const __grid_constant__ CUtensorMap my1, const __grid_constant__ CUtensorMap my2,
-                const Params p) {
+                const __grid_constant__ CUtensorMap mo1, const __grid_constant__ CUtensorMap mo2, const Params p) {
     using Cf = BwdCfg<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* stat = reinterpret_cast<float*>(smem + Cf::STAT_OFF);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BAR_OFF);
     uint64_t *x_full = bars, *s_full = bars + 1, *dp_full = bars + 2, *acc_full = bars + 3, *drain = bars + 4,
-             *p_ready = bars + 5, *ds_ready = bars + 6, *stat_ready = bars + 7;
+             *p_ready = bars + 5, *ds_ready = bars + 6, *out_ready = bars + 7;
     uint64_t* full = bars + 8;
     uint64_t* empty = full + Cf::SLOTS;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
@@ -635,6 +656,36 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                          smem_u32(tmem_holder)), "r"(Cf::TMEM_COLS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // dQ: a thread's part of its row's delta, 8 elements of dO . O at a time, and the row's lse,
+    // fetched while the barriers and TMEM are set up
+    float delta_part = 0.f, lse_in = 0.f;
+    if (!KV && warp < W_LOAD) {
+        const int w = warp / 4, r = r0 + (warp % 4) * 32 + lane;
+        if (r < ql) {
+            const auto* go = attn::row<DT>(p.dout, b, r, hx);
+            const auto* o = attn::row<DT>(p.o, b, r, hx);
+            constexpr int N = DP / 8 / Cf::WG;
+            uint4 u[N], v[N];
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+                if ((w + x * Cf::WG) * 8 < p.D) {
+                    u[x] = __ldg(reinterpret_cast<const uint4*>(go) + w + x * Cf::WG);
+                    v[x] = __ldg(reinterpret_cast<const uint4*>(o) + w + x * Cf::WG);
+                }
+            lse_in = __ldg(p.lse + ((long long)b * p.H + hx) * p.Sq + r);
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+                if ((w + x * Cf::WG) * 8 < p.D) {
+                    const auto* a2 = reinterpret_cast<const typename Half16<DT>::T2*>(&u[x]);
+                    const auto* b2 = reinterpret_cast<const typename Half16<DT>::T2*>(&v[x]);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const float2 f = Half16<DT>::unpack(a2[y]), g = Half16<DT>::unpack(b2[y]);
+                        delta_part += f.x * g.x + f.y * g.y;
+                    }
+                }
+        }
     }
     if (KV) {                             // the constant operands, 8 columns of a row at a time
         for (int i = threadIdx.x; i < XE_BYTES / 16; i += Cf::THREADS) {
@@ -746,25 +797,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         } else {
             row_hi = r < ql ? kl : 0;
             if (p.causal) row_hi = min(row_hi, r + kl - ql + 1);
-            float d = 0.f;
-            if (row_hi > 0) {                 // a part of dO . O, 8 elements at a time
-                const auto* go = attn::row<DT>(p.dout, b, r, hx);
-                const auto* o = attn::row<DT>(p.o, b, r, hx);
-                for (int c = w; c < p.D / 8; c += Cf::WG) {
-                    const uint4 u = reinterpret_cast<const uint4*>(go)[c], v = reinterpret_cast<const uint4*>(o)[c];
-                    const auto* a2 = reinterpret_cast<const typename Half16<DT>::T2*>(&u);
-                    const auto* b2 = reinterpret_cast<const typename Half16<DT>::T2*>(&v);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const float2 f = Half16<DT>::unpack(a2[x]), g = Half16<DT>::unpack(b2[x]);
-                        d += f.x * g.x + f.y * g.y;
-                    }
-                }
-                lse2 = -p.lse[((long long)b * p.H + hx) * p.Sq + r] * LOG2E;
-            }
-            stat[tid] = d;
-            warp_arrive(stat_ready);
-            ok = warp_wait(stat_ready, 0, abort_flag);
+            if (row_hi > 0) lse2 = -lse_in * LOG2E;
+            stat[tid] = row_hi > 0 ? delta_part : 0.f;
+            warp_arrive(out_ready);               // its first phase: the parts of delta
+            ok = warp_wait(out_ready, 0, abort_flag);
             float delta = 0.f;
             for (int x = 0; x < Cf::WG; ++x) delta += stat[row + x * 128];
             ds0 = -delta * p.scale;
@@ -857,8 +893,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             // the warpgroups take alternate 32 columns; KV: the first half of them dK, the others dV
             constexpr int HALF = Cf::WG / 2;
             const int rows = KV ? p.Sk : p.Sq;
-            const View& view = !KV ? p.dq : w < HALF ? p.dk : p.dv;
-            auto* out = r < rows ? row_out<DT>(view, b, r, hx) : nullptr;
+            uint8_t* tile = smem + (KV && w >= HALF ? Cf::TILE : 0);   // X's, which every product has read
             // partial dV behind all of dK's
             float* part = r < rows && p.splits > 1
                               ? p.part + ((((KV && w >= HALF ? p.splits : 0) + (long long)split) * bhs + bh) * rows + r) * p.D
@@ -870,7 +905,21 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                     tmem_ld32_issue(acc + c, o);
                     tmem_ld_wait<32>(o);
                 }
-                store_chunk<DT>(o, nblk > 0, 1.f, p.splits > 1, out, part, c, p.D);
+                store_chunk<DT>(o, nblk > 0, 1.f, p.splits > 1, tile, row, part, c, p.D);
+            }
+            if (p.splits == 1) {
+                fence_async_smem();
+                warp_arrive(out_ready);
+                if (warp == 0) {
+                    if (!warp_wait(out_ready, KV ? 0 : 1, abort_flag)) {
+                        err = ERR_MATH;
+                    } else if (lane == 0) {
+                        store_tile(&mo1, smem, p.D, r0, hx, b);
+                        if (KV) store_tile(&mo2, smem + Cf::TILE, p.D, r0, hx, b);
+                        bulk_commit();
+                        bulk_wait_read<0>();
+                    }
+                }
             }
         }
     }
@@ -1021,14 +1070,15 @@ static int launch_fwd(DeviceCtx* c, const Params& p) {
         OMB_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::SMEM));
         attr_set[c->device] = true;
     }
-    CUtensorMap mq = {}, mk = {}, mv = {};
+    CUtensorMap mq = {}, mk = {}, mv = {}, mo = {};
     int st = encode(&mq, p.q, p.B, p.Sq, p.H, p.D, DT);
     if (st == OM_OK && p.Sk > 0) st = encode(&mk, p.k, p.B, p.Sk, p.Hkv, p.D, DT);
     if (st == OM_OK && p.Sk > 0) st = encode(&mv, p.v, p.B, p.Sk, p.Hkv, p.D, DT);
+    if (st == OM_OK && p.splits == 1) st = encode(&mo, p.o, p.B, p.Sq, p.H, p.D, DT);
     if (st != OM_OK) return st;
     const long long grid = (long long)((p.Sq + NT * 128 - 1) / (NT * 128)) * p.B * p.H * p.splits;
     if (grid > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-    kern<<<(unsigned)grid, Cf::THREADS, Cf::SMEM, c->compute>>>(mq, mk, mv, p);
+    kern<<<(unsigned)grid, Cf::THREADS, Cf::SMEM, c->compute>>>(mq, mk, mv, mo, p);
     return after_launch(c);
 }
 template <int DT>
@@ -1051,6 +1101,13 @@ template <int DP, bool KV, int DT>
 static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& y1,
                       const CUtensorMap& y2, const Params& p) {
     using Cf = BwdCfg<DP>;
+    CUtensorMap o1 = {}, o2 = {};         // dQ, or dK and dV
+    if (p.splits == 1) {
+        const int T = KV ? p.Sk : p.Sq, H = KV ? p.Hkv : p.H;
+        int st = encode(&o1, KV ? p.dk : p.dq, p.B, T, H, p.D, DT);
+        if (st == OM_OK && KV) st = encode(&o2, p.dv, p.B, T, H, p.D, DT);
+        if (st != OM_OK) return st;
+    }
     auto kern = attn_bwd_kernel<DP, KV, DT>;
     static bool attr_set[64] = {false};
     if (!attr_set[c->device]) {
@@ -1059,7 +1116,7 @@ static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2
     }
     const long long n = (long long)(((KV ? p.Sk : p.Sq) + 127) / 128) * p.B * (KV ? p.Hkv : p.H) * p.splits;
     if (n > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-    kern<<<(unsigned)n, Cf::THREADS, Cf::SMEM, c->compute>>>(x1, x2, y1, y2, p);
+    kern<<<(unsigned)n, Cf::THREADS, Cf::SMEM, c->compute>>>(x1, x2, y1, y2, o1, o2, p);
     return after_launch(c);
 }
 template <int DP, int DT>
