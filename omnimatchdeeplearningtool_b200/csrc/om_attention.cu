@@ -640,11 +640,10 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         if (p.causal) end = min(end, min(r0 + 128, ql) + kl - ql);
         per = end > 0 ? (end + BN - 1) / BN : 0;
     }
-    // this part's share of them
-    const int share = (per + p.splits - 1) / p.splits;
-    first += split * share;
-    per = max(0, min(per - split * share, share));
-    const int nblk = uniform(KV ? per * rep : per);
+    // this part's share of them, from the it0-th on (KV: head by head)
+    const int all = KV ? per * rep : per, share = (all + p.splits - 1) / p.splits, it0 = split * share;
+    const int nblk = uniform(max(0, min(all - it0, share)));
+    const int y_start = per > 0 ? first + it0 % per : 0, hy_start = hy0 + (per > 0 ? it0 / per : 0);
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8; ++i) mbar_init(bars + i, i < 5 ? 1 : Cf::WG * 4);
@@ -703,6 +702,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_holder);
+    if (!KV) pdl_launch_dependents();     // the KV kernel may set up where this one's CTAs have left
     unsigned int err = 0;
 
     if (warp == W_LOAD) {
@@ -710,11 +710,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             mbar_expect_tx(x_full, 2 * Cf::TILE);
             load_tile<DP>(0, smem, &mx1, x_full, r0, hx, b);
             load_tile<DP>(Cf::TILE, smem, &mx2, x_full, r0, hx, b);
-            int i = 0, y = first, hy = hy0;
+            int i = 0, y = y_start, hy = hy_start;
             for (; i < 2 * nblk; ++i) {   // Y1 (KV: and its queries' statistics), Y2 of each block in turn
                 const int slot = i % Cf::SLOTS;
                 if (!mbar_wait(empty + slot, ((i / Cf::SLOTS) & 1) ^ 1, abort_flag)) { err = ERR_LOAD; break; }
                 mbar_expect_tx(full + slot, Cf::Y_TILE + (KV && !(i & 1) ? Cf::STAT : 0));
+                if (KV && i == 0) pdl_wait();     // the dQ kernel's statistics
                 if (KV && !(i & 1))
                     bulk_load(smem + Cf::STAT_OFF + slot / 2 * Cf::STAT, stat_tile(p, b, hy, y * (BN / 64)), Cf::STAT,
                               full + slot);
@@ -814,7 +815,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 out[8] = make_uint4(0, 0, 0, 0);
             }
         }
-        int y0 = first * BN;
+        int y0 = y_start * BN;
         for (int i = 0; ok && i < nblk; ++i) {
             ok = warp_wait(s_full, i & 1, abort_flag);
             if (!ok) break;
@@ -924,6 +925,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         }
     }
     if (err) atomicOr(p.err, err);
+    if (KV && nblk == 0) pdl_wait();      // so that this kernel's end means the dQ kernel's end too
     tc_fence_before();
     __syncthreads();
     if (warp == W_MMA) {
@@ -936,10 +938,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
 // One warp per row of [batch][head][token]: the parts in a fixed order. LSE: each weighted by 2^(its
 // log2 sum - the largest), their sum of weights into lse; else their sum.
 template <int DT, bool LSE>
-__global__ void __launch_bounds__(128) join_kernel(const Params p, const View out, const float* part, int T, int H) {
+__global__ void __launch_bounds__(128) join_kernel(const Params p, const View out0, const View out1, int T, int H) {
     const int lane = threadIdx.x % 32;
     const long long row = blockIdx.x * 4LL + threadIdx.x / 32, rows = (long long)p.B * H * T;
     if (row >= rows) return;
+    const View& out = blockIdx.y ? out1 : out0;
+    const float* part = p.part + (blockIdx.y ? p.splits * rows * p.D : 0);
     const int t = (int)(row % T), h = (int)(row / T % H), b = (int)(row / T / H);
     // lanes: `wide` float4 columns x 32 / wide parts at a time
     const int cols = p.D / 4, wide = cols <= 2 ? 2 : cols <= 4 ? 4 : cols <= 8 ? 8 : cols <= 16 ? 16 : 32;
@@ -976,35 +980,43 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p, const View ou
     if (LSE && lane == 0 && p.lse) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
 }
 template <int DT, bool LSE>
-static int join(DeviceCtx* c, const Params& p, const View& out, const float* part, int T, int H) {
+static int join(DeviceCtx* c, const Params& p, const View& out, int T, int H, const View* second = nullptr) {
     const long long blocks = ((long long)p.B * H * T + 3) / 4;
     if (blocks > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-    join_kernel<DT, LSE><<<(unsigned)blocks, 128, 0, c->compute>>>(p, out, part, T, H);
+    join_kernel<DT, LSE><<<dim3((unsigned)blocks, second ? 2 : 1), 128, 0, c->compute>>>(p, out, second ? *second : out, T, H);
     return after_launch(c);
 }
 
-// Parts of a streamed axis of `blocks` blocks for `ctas` tiles: as many as the places of CTAs on the
-// GPU's 148 SMs allow, each of two blocks at least. With half of the places filled or more there is
-// one part: joining costs another launch and the partial rows.
-static int parts(long long ctas, int blocks, int places) {
-    if (ctas <= 0 || ctas * 2 > places) return 1;
-    const long long n = places / ctas;
-    return (int)(n < blocks / 2 ? n : blocks / 2 < 1 ? 1 : blocks / 2);
+// Parts of the streamed axis for `ctas` tiles of `blocks` blocks each (causal: half of that on the
+// average), on `places` of CTAs, 148 SMs times the CTAs that an SM holds: the count with the least
+// estimated time, in blocks: the longest part or the even share of all of them, each part with about
+// 4 blocks' time for its start and end; joining costs about 3 (another launch) and grows with the
+// parts. Parts of two blocks at least. (84 tiles of 28 causal blocks: 3 parts, 62 -> 32 us; 16 tiles
+// of 32 blocks: 16 parts, 55 -> 18 us.)
+static int parts(long long ctas, int blocks, int places, bool causal) {
+    int best = 1;
+    float least = INFINITY;
+    for (int n = 1; n <= 64 && (n == 1 || n * 2 <= blocks); ++n) {
+        const float mean = (causal ? 0.5f : 1.f) * blocks / n + 4.f, rounds = (float)(ctas * n) / places;
+        const float t = fmaxf((float)blocks / n + 4.f, (causal ? rounds : ceilf(rounds)) * mean) + (n > 1 ? 3.f + 0.1f * n : 0.f);
+        if (t < least) { least = t; best = n; }
+    }
+    return best;
 }
 // The split of each kernel of a problem and the workspace it takes.
 struct Plan {
     int nt, fwd, dq, dkv;                 // query tiles of a forward CTA; parts
     long long fwd_bytes, bwd_bytes, dq_at, dkv_at;
 };
-static Plan plan(int B, int H, int Hkv, int Sq, int Sk, int D) {
+static Plan plan(int B, int H, int Hkv, int Sq, int Sk, int D, bool causal) {
     Plan n;
     const long long qt = (Sq + 127) / 128, kt = (Sk + 127) / 128, bh = (long long)B * H, bhk = (long long)B * Hkv;
     n.nt = Sq <= 128 ? 1 : 2;
-    n.fwd = parts((qt + n.nt - 1) / n.nt * bh, (int)kt, n.nt == 1 ? 296 : 148);
+    n.fwd = parts((qt + n.nt - 1) / n.nt * bh, (int)kt, n.nt == 1 ? 296 : 148, causal);
     n.fwd_bytes = n.fwd > 1 ? n.fwd * bh * Sq * (D + 1) * 4 : 0;
     const int places = D <= 64 ? 296 : 148, bn = D <= 64 ? 64 : 128;
-    n.dq = parts(qt * bh, (Sk + bn - 1) / bn, places);
-    n.dkv = parts(kt * bhk, (Sq + bn - 1) / bn, places);
+    n.dq = parts(qt * bh, (Sk + bn - 1) / bn, places, causal);
+    n.dkv = parts(kt * bhk, (Sq + bn - 1) / bn * (H / Hkv), places, causal);
     n.dq_at = bh * stat_tiles(Sq) * STAT_TILE;
     n.dkv_at = n.dq_at + (n.dq > 1 ? n.dq * bh * Sq * D * 4 : 0);
     n.bwd_bytes = n.dkv_at + (n.dkv > 1 ? 2 * n.dkv * bhk * Sk * D * 4 : 0);
@@ -1083,7 +1095,7 @@ static int launch_fwd(DeviceCtx* c, const Params& p) {
 }
 template <int DT>
 static int forward(DeviceCtx* c, Params p, void* workspace) {
-    const Plan n = plan(p.B, p.H, p.Hkv, p.Sq, p.Sk, p.D);
+    const Plan n = plan(p.B, p.H, p.Hkv, p.Sq, p.Sk, p.D, p.causal);
     p.splits = n.fwd;
     p.part = static_cast<float*>(workspace);
     p.part_lse = p.part + (long long)n.fwd * p.B * p.H * p.Sq * p.D;
@@ -1093,13 +1105,13 @@ static int forward(DeviceCtx* c, Params p, void* workspace) {
         st = n.nt == 1 ? launch_fwd<64, 1, DT>(c, p) : launch_fwd<64, 2, DT>(c, p);
     else
         st = n.nt == 1 ? launch_fwd<128, 1, DT>(c, p) : launch_fwd<128, 2, DT>(c, p);
-    return st == OM_OK && n.fwd > 1 ? join<DT, true>(c, p, p.o, p.part, p.Sq, p.H) : st;
+    return st == OM_OK && n.fwd > 1 ? join<DT, true>(c, p, p.o, p.Sq, p.H) : st;
 }
 
 // x1, x2: maps of the kept tiles (128 rows), y1, y2: of the streamed ones (BN rows)
 template <int DP, bool KV, int DT>
 static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& y1,
-                      const CUtensorMap& y2, const Params& p) {
+                      const CUtensorMap& y2, const Params& p, bool after_dq = false) {
     using Cf = BwdCfg<DP>;
     CUtensorMap o1 = {}, o2 = {};         // dQ, or dK and dV
     if (p.splits == 1) {
@@ -1116,7 +1128,17 @@ static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2
     }
     const long long n = (long long)(((KV ? p.Sk : p.Sq) + 127) / 128) * p.B * (KV ? p.Hkv : p.H) * p.splits;
     if (n > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-    kern<<<(unsigned)n, Cf::THREADS, Cf::SMEM, c->compute>>>(x1, x2, y1, y2, o1, o2, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)n);
+    cfg.blockDim = dim3(Cf::THREADS);
+    cfg.dynamicSmemBytes = Cf::SMEM;
+    cfg.stream = c->compute;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = KV && after_dq ? 1 : 0;    // it may set up while the dQ kernel ends
+    OMB_CHECK(cudaLaunchKernelEx(&cfg, kern, x1, x2, y1, y2, o1, o2, p));
     return after_launch(c);
 }
 template <int DP, int DT>
@@ -1132,21 +1154,19 @@ static int backward(DeviceCtx* c, Params p) {
             if (st != OM_OK) return st;
         }
     }
-    const Plan n = plan(p.B, p.H, p.Hkv, p.Sq, p.Sk, p.D);
+    const Plan n = plan(p.B, p.H, p.Hkv, p.Sq, p.Sk, p.D, p.causal);
     int st = OM_OK;
     if (p.Sq > 0) {                       // dQ first: it leaves the queries' statistics for dK and dV
         p.splits = n.dq;
         p.part = reinterpret_cast<float*>(p.stat + n.dq_at);
         st = launch_bwd<DP, false, DT>(c, m[0][0], m[0][3], m[1][1], m[1][2], p);
-        if (st == OM_OK && n.dq > 1) st = join<DT, false>(c, p, p.dq, p.part, p.Sq, p.H);
+        if (st == OM_OK && n.dq > 1) st = join<DT, false>(c, p, p.dq, p.Sq, p.H);
     }
     if (st == OM_OK && p.Sk > 0) {
         p.splits = n.dkv;
         p.part = reinterpret_cast<float*>(p.stat + n.dkv_at);
-        st = launch_bwd<DP, true, DT>(c, m[0][1], m[0][2], m[1][0], m[1][3], p);
-        if (st == OM_OK && n.dkv > 1) st = join<DT, false>(c, p, p.dk, p.part, p.Sk, p.Hkv);
-        if (st == OM_OK && n.dkv > 1)
-            st = join<DT, false>(c, p, p.dv, p.part + (long long)n.dkv * p.B * p.Hkv * p.Sk * p.D, p.Sk, p.Hkv);
+        st = launch_bwd<DP, true, DT>(c, m[0][1], m[0][2], m[1][0], m[1][3], p, p.Sq > 0);
+        if (st == OM_OK && n.dkv > 1) st = join<DT, false>(c, p, p.dk, p.Sk, p.Hkv, &p.dv);
     }
     return st;
 }
@@ -1160,8 +1180,10 @@ extern "C" long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int n
                                                    int nSk, int nHeadDim, int bBackward) {
     const int st = attn::check_sizes(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim);
     if (st != OM_OK) return st;
-    const attn::Plan n = attn::plan(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim);
-    return bBackward ? n.bwd_bytes : n.fwd_bytes;
+    const attn::Plan a = attn::plan(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim, false);
+    const attn::Plan b = attn::plan(nBatch, nHeads, nKvHeads, nSq, nSk, nHeadDim, true);
+    return bBackward ? (a.bwd_bytes > b.bwd_bytes ? a.bwd_bytes : b.bwd_bytes)
+                     : (a.fwd_bytes > b.fwd_bytes ? a.fwd_bytes : b.fwd_bytes);
 }
 
 extern "C" int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut,
