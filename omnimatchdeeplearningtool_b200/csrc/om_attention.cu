@@ -10,6 +10,23 @@ namespace attn {
 
 using namespace omb::tc;
 
+// Division of 0 <= n < 2^31 by a divisor known on the host: n * mul / 2^(32 + shift)
+// (Granlund and Montgomery, 1994)
+struct Div {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ int operator()(int n) const {
+        return d == 1 ? n : (int)(__umulhi((uint32_t)n, mul) >> shift);
+    }
+};
+static Div div_by(uint32_t d) {
+    Div r = {d, 0, 0};
+    if (d <= 1) return r;
+    int l = 0;
+    while ((1ull << l) < d) ++l;              // 2^(l-1) < d <= 2^l
+    r.shift = l - 1;                          // mul = ceil(2^(31 + l) / d) < 2^32
+    r.mul = (uint32_t)(((1ull << (31 + l)) + d - 1) / d);
+    return r;
+}
 struct View {          // a [batch, token, head, D] tensor: element strides, D contiguous
     void* p;
     long long sb, st, sh;
@@ -26,6 +43,8 @@ struct Params {
     float scale2;      // |scale| * log2(e), not 0 (masked scores stay minus infinity)
     bool neg;          // scale < 0: the score products negate Q
     unsigned int* err;
+    int items;         // the forward's tiles times parts, and the divisions that find an item's place
+    Div by_splits, by_fast, by_heads;   // by_fast: tiles of a head, causal: heads
     int splits;        // parts of the streamed axis, each CTA one of them (1: no partial results)
     float* part;       // partial results: fp32 rows [split][batch][head][token][D]
     float* part_lse;   // forward: the parts' log2(sum exp) [split][batch][head][token]
@@ -241,72 +260,111 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* map, const uint8_t
 constexpr float LN2 = 0.6931471805599453f;
 
 // ---------------------------------------------------------------- forward
-// One CTA: NT tiles of 128 queries of one (batch, head), over the key blocks of 128. A softmax
-// warpgroup per tile (thread = query row), a TMA warp and an MMA warp. Per tile and block:
+// One item of work: NT tiles of 128 queries of one (batch, head) over the key blocks of 128 (or one
+// part of them). A CTA stays on its SM and takes every gridDim.x-th item: a softmax warpgroup per
+// tile (thread = query row), a TMA warp and an MMA warp, each running ahead of the others as far as
+// the buffers go, so that an item's loads and first scores come beside the last one's end (with a
+// CTA per item the time between two CTAs of an SM, about 2.9 us with their set-up, was a third of
+// the 54 us that 768 heads of 197 tokens took).
+// Per tile and block:
 //   S = Q K^T (TMEM, fp32) -> running maximum, P = exp(S - m), row sums -> P (TMEM, 16-bit, over
 //   S's columns) -> O += P V (TMEM, fp32).
 // O is rescaled only when a row's maximum has grown by more than 2^8 since its last reference
 // maximum: P stays below 2^8, in range of both types, and the factor cancels in O / l.
-// Score tile n = NT j + t (block j, query tile t) lies in TMEM buffer n % NB. With heads up to 64
-// there is room for a third buffer, so that a tile's next scores are there when its probabilities
-// are done (without it a softmax warp waited about 900 of 2900 clocks a block for them).
+// Score tile n = NT j + t (block j, query tile t) lies in TMEM buffer n % NB, counted over all items.
+// With heads up to 64 there is room for a third buffer, so that a tile's next scores are there when
+// its probabilities are done (without it a softmax warp waited about 900 of 2900 clocks a block for
+// them).
 // TMEM: NB score tiles, then the O tiles.
 template <int DP, int NT>
 struct FwdCfg {
     static constexpr int TILE = DP / 64 * PANEL;
-    static constexpr int SLOTS = NT == 2 ? (DP == 128 ? 4 : 8) : (DP == 128 ? 2 : 5);
-    static constexpr int SMEM = (NT + SLOTS) * TILE + 1024 + 1024;
-    static constexpr int THREADS = NT * 128 + 64;
+    static constexpr int SLOTS = NT == 2 ? (DP == 128 ? 4 : 6) : (DP == 128 ? 2 : 4);
+    // the output's staging tiles: Q's with long heads, which shared memory then holds no others beside
+    static constexpr bool OWN_STAGE = DP == 64;
+    static constexpr int KV_OFF = NT * TILE, STAGE_OFF = OWN_STAGE ? KV_OFF + SLOTS * TILE : 0;
+    static constexpr int BAR_OFF = KV_OFF + (SLOTS + (OWN_STAGE ? NT : 0)) * TILE;
+    static constexpr int SMEM = BAR_OFF + 512;
+    static constexpr int THREADS = NT * 128 + 64, OCC = NT == 1 ? 2 : 1;
     static constexpr int TMEM_COLS = NT * 256;
     static constexpr int NB = NT == 2 && DP == 64 ? 3 : NT;
     static constexpr int O_COL = NB * 128, O_STEP = DP;
-    static_assert(O_COL + NT * O_STEP <= TMEM_COLS, "TMEM");
+    static_assert(O_COL + NT * O_STEP <= TMEM_COLS && (SMEM + 1024) * OCC <= 228 * 1024, "on-chip memory");
 };
 enum : unsigned int { ERR_LOAD = ERRBIT_TC_PRODUCER, ERR_MMA = ERRBIT_TC_MMA,
                       ERR_MATH = ERRBIT_TC_EPILOGUE, ERR_DRAIN = ERRBIT_TC_DRAIN };
+
+struct FwdPlace { int b, h, q0, split; };
+struct FwdRange { int ql, kl, blk0, nblk; };
+// The r-th item of a CTA, in turns from the first and from the last CTA (long items come first), or
+// one past the end.
+__device__ __forceinline__ int fwd_at(int r) {
+    return r * gridDim.x + (r % 2 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+}
+template <int NT>
+__device__ __forceinline__ FwdPlace fwd_place(const Params& p, int at) {
+    // causal: heads fastest and the longest rows first, so that the last items are short
+    const int i = p.by_splits(at), hi = p.by_fast(i), lo = i - hi * (int)p.by_fast.d;
+    const int bh = p.causal ? lo : hi, tile = p.causal ? (p.Sq + NT * 128 - 1) / (NT * 128) - 1 - hi : lo;
+    const int b = p.by_heads(bh);
+    return {b, bh - b * p.H, tile * (NT * 128), at - i * p.splits};
+}
+template <int NT>
+__device__ __forceinline__ FwdRange fwd_range(const Params& p, const FwdPlace& w) {
+    FwdRange r;
+    r.ql = len_of(p.qlens, w.b, p.Sq);
+    r.kl = len_of(p.kvlens, w.b, p.Sk);
+    int end = w.q0 < r.ql ? r.kl : 0;
+    if (p.causal) end = min(end, min(w.q0 + NT * 128, r.ql) + r.kl - r.ql);
+    // this part's key blocks: blk0 .. blk0 + nblk - 1
+    const int all = end > 0 ? (end + 127) / 128 : 0, share = p.by_splits(all + p.splits - 1);
+    r.blk0 = w.split * share;
+    r.nblk = uniform(max(0, min(all - r.blk0, share)));
+    return r;
+}
 
 template <int DP, int NT, int DT>
 __global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Params p) {
     using Cf = FwdCfg<DP, NT>;
-    using H16 = Half16<DT>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + (NT + Cf::SLOTS) * Cf::TILE);
-    uint64_t* q_full = bars;
-    uint64_t* o_full = bars + 1;
-    uint64_t* drain = bars + 2;
-    uint64_t* s_full = bars + 3;
+    // aligned by its declaration, so that every address below is a constant (rounded up at run time,
+    // the barriers' pointers took the registers that the scores need)
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) % 1024) {
+        if (threadIdx.x == 0) atomicOr(p.err, ERR_LOAD);
+        return;
+    }
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BAR_OFF);
+    // q_full and q_empty pass once an item, with key blocks or without, and every role takes part:
+    // so no role is ever two phases of a barrier ahead of another
+    uint64_t *q_full = bars, *q_empty = bars + 1, *drain = bars + 2;
+    uint64_t* s_full = bars + 3;                 // per score buffer
     uint64_t* p_full = s_full + Cf::NB;
-    uint64_t* pv_done = p_full + Cf::NB;
-    uint64_t* out_ready = pv_done + NT;
-    uint64_t* full = out_ready + NT;
+    uint64_t* pv_done = p_full + Cf::NB;         // per tile: O has a block's product
+    uint64_t* o_free = pv_done + NT;             // ... and has been read by the item's epilogue
+    uint64_t* out_ready = o_free + NT;           // the staging tile is written
+    uint64_t* stage_free = out_ready + NT;       // ... and stored
+    uint64_t* full = stage_free + NT;
     uint64_t* empty = full + Cf::SLOTS;
     uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(empty + Cf::SLOTS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
-    const int warp = uniform(threadIdx.x / 32), lane = threadIdx.x % 32;
+    const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
     constexpr int W_LOAD = NT * 4, W_MMA = NT * 4 + 1;
-    // causal: heads fastest and the longest rows first, so that the last CTAs to start are short
-    const int tiles = (p.Sq + NT * 128 - 1) / (NT * 128), heads = p.B * p.H;
-    const int split = blockIdx.x % p.splits, cta = blockIdx.x / p.splits;
-    const int bh = p.causal ? cta % heads : cta / tiles;
-    const int h = bh % p.H, b = bh / p.H, hk = h / (p.H / p.Hkv);
-    const int q0 = (p.causal ? tiles - 1 - cta / heads : cta % tiles) * (NT * 128);
-    const int ql = len_of(p.qlens, b, p.Sq), kl = len_of(p.kvlens, b, p.Sk);
-    int end = q0 < ql ? kl : 0;
-    if (p.causal) end = min(end, min(q0 + NT * 128, ql) - 1 + kl - ql + 1);
-    // this part's key blocks: blk0 .. blk0 + nblk - 1
-    const int all = end > 0 ? (end + 127) / 128 : 0, share = (all + p.splits - 1) / p.splits;
-    const int blk0 = split * share, nblk = uniform(max(0, min(all - blk0, share)));
+    const int items = p.items;
 
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
-        mbar_init(o_full, 1);
+        mbar_init(q_empty, 1 + NT);
         mbar_init(drain, 1);
         for (int i = 0; i < Cf::NB; ++i) { mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); }
-        for (int t = 0; t < NT; ++t) { mbar_init(pv_done + t, 1); mbar_init(out_ready + t, 4); }
+        for (int t = 0; t < NT; ++t) {
+            mbar_init(pv_done + t, 1);
+            mbar_init(o_free + t, 4);
+            mbar_init(out_ready + t, 4);
+            mbar_init(stage_free + t, 1);
+        }
         for (int i = 0; i < Cf::SLOTS; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -320,196 +378,300 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_holder);
-    const uint32_t kv_base = smem_u32(smem) + NT * Cf::TILE;
     unsigned int err = 0;
 
     if (warp == W_LOAD) {
-        if (lane == 0 && nblk > 0) {
-            mbar_expect_tx(q_full, NT * Cf::TILE);
-            for (int t = 0; t < NT; ++t) load_tile<DP>(t * Cf::TILE, smem, &mq, q_full, q0 + t * 128, h, b);
-            int i = 0;
-            for (; i < 2 * nblk; ++i) {   // K_0, V_0, K_1, V_1, ...
-                const int slot = i % Cf::SLOTS;
-                if (!mbar_wait(empty + slot, ((i / Cf::SLOTS) & 1) ^ 1, abort_flag)) { err = ERR_LOAD; break; }
-                mbar_expect_tx(full + slot, Cf::TILE);
-                load_tile<DP>((NT + slot) * Cf::TILE, smem, i & 1 ? &mv : &mk, full + slot, (blk0 + i / 2) * 128, hk, b);
+        int slot = 0, issued = 0, queries = 0;   // queries: phases of q_full so far
+        uint32_t slot_ph = 1, item_ph = 1;
+        bool ok = true;
+        for (int turn = 0; ok && turn * (int)gridDim.x < items; ++turn) {
+            const int at = fwd_at(turn);
+            if (at >= items) continue;
+            const FwdPlace w = fwd_place<NT>(p, at);
+            const FwdRange r = fwd_range<NT>(p, w);
+            ok = warp_wait(q_empty, item_ph, abort_flag);
+            if (!ok) break;
+            item_ph ^= 1;
+            if (lane == 0 && r.nblk > 0) {
+                mbar_expect_tx(q_full, NT * Cf::TILE);
+                for (int t = 0; t < NT; ++t) load_tile<DP>(t * Cf::TILE, smem, &mq, q_full, w.q0 + t * 128, w.h, w.b);
+            } else if (lane == 0) {
+                mbar_arrive(q_full);
             }
-            if (err || *abort_flag) {     // every load issued has to land before the CTA ends
-                *abort_flag = 1;
-                if (!mbar_wait_drain(q_full, 0)) err |= ERR_DRAIN;
-                for (int j = max(0, i - Cf::SLOTS); j < i; ++j)
-                    if (!mbar_wait_drain(full + j % Cf::SLOTS, (j / Cf::SLOTS) & 1)) err |= ERR_DRAIN;
+            ++queries;
+            const int hk = w.h / (p.H / p.Hkv);
+            for (int i = 0; i < 2 * r.nblk; ++i) {   // K, V of each block
+                ok = warp_wait(empty + slot, slot_ph, abort_flag);
+                if (!ok) break;
+                if (lane == 0) {
+                    mbar_expect_tx(full + slot, Cf::TILE);
+                    load_tile<DP>(Cf::KV_OFF + slot * Cf::TILE, smem, i & 1 ? &mv : &mk, full + slot,
+                                  (r.blk0 + i / 2) * 128, hk, w.b);
+                }
+                ++issued;
+                if (++slot == Cf::SLOTS) { slot = 0; slot_ph ^= 1; }
             }
         }
+        if (!ok || *abort_flag) {                // every load issued has to land before the CTA ends
+            *abort_flag = 1;
+            err = ok ? 0 : ERR_LOAD;
+            if (queries > 0 && !mbar_wait_drain(q_full, (queries - 1) & 1)) err |= ERR_DRAIN;
+            for (int j = max(0, issued - Cf::SLOTS); j < issued; ++j)
+                if (!mbar_wait_drain(full + j % Cf::SLOTS, (j / Cf::SLOTS) & 1)) err |= ERR_DRAIN;
+        }
     } else if (warp == W_MMA) {
-        if (nblk > 0) {
-            const uint32_t leader = elect();
-            const int ks = (p.D + 15) / 16;
-            const uint32_t id_s = idesc_f16(DT == OM_DTYPE_F16, 128, false, p.neg);
-            const uint32_t id_o = idesc_f16(DT == OM_DTYPE_F16, ks * 16, true, false);
-            const uint32_t q_tile = smem_u32(smem);
-            // Running places: block, slot and TMEM buffer of the scores to issue next (s...) and of
-            // the probabilities to take next (p...)
-            struct { int tile, slot, buf; uint32_t slot_ph, buf_ph; } sn = {0, 0, 0, 0, 0}, pn = {0, 1, 0, 0, 0};
-            auto step = [&](auto& at) {
-                if (++at.buf == Cf::NB) { at.buf = 0; at.buf_ph ^= 1; }
-                if (++at.tile == NT) {
-                    at.tile = 0;
-                    at.slot += 2;
-                    if (at.slot >= Cf::SLOTS) { at.slot -= Cf::SLOTS; at.slot_ph ^= 1; }
-                }
-            };
-            auto scores = [&]() {         // one score tile, and K's slot back behind the block's last
-                if (sn.tile == 0 && !warp_wait(full + sn.slot, sn.slot_ph, abort_flag)) return false;
-                tc_fence_after();
-                product_k<DP, 128>(leader, tmem + sn.buf * 128, q_tile + sn.tile * Cf::TILE, kv_base + sn.slot * Cf::TILE,
-                                   id_s, ks);
-                commit(leader, s_full + sn.buf);
-                if (sn.tile == NT - 1) commit(leader, empty + sn.slot);
-                step(sn);
-                return true;
-            };
-            const int total = NT * nblk;
-            bool ok = warp_wait(q_full, 0, abort_flag);
-            for (int n = 0; ok && n < Cf::NB && n < total; ++n) ok = scores();
+        const uint32_t leader = elect();
+        const int ks = (p.D + 15) / 16;
+        const uint32_t id_s = idesc_f16(DT == OM_DTYPE_F16, 128, false, p.neg);
+        const uint32_t id_o = idesc_f16(DT == OM_DTYPE_F16, ks * 16, true, false);
+        const uint32_t q_tile = smem_u32(smem), kv_base = q_tile + Cf::KV_OFF;
+        // Running places: slot and TMEM buffer of the scores to issue next (sn) and of the
+        // probabilities to take next (pn), counted over all items
+        struct { int tile, slot, buf; uint32_t slot_ph, buf_ph; } sn = {0, 0, 0, 0, 0}, pn = {0, 1, 0, 0, 0};
+        auto step = [&](auto& at) {
+            if (++at.buf == Cf::NB) { at.buf = 0; at.buf_ph ^= 1; }
+            if (++at.tile == NT) {
+                at.tile = 0;
+                at.slot += 2;
+                if (at.slot >= Cf::SLOTS) { at.slot -= Cf::SLOTS; at.slot_ph ^= 1; }
+            }
+        };
+        auto scores = [&]() {             // one score tile, and K's slot back behind the block's last
+            if (sn.tile == 0 && !warp_wait(full + sn.slot, sn.slot_ph, abort_flag)) return false;
+            tc_fence_after();
+            product_k<DP, 128>(leader, tmem + sn.buf * 128, q_tile + sn.tile * Cf::TILE, kv_base + sn.slot * Cf::TILE,
+                               id_s, ks);
+            commit(leader, s_full + sn.buf);
+            if (sn.tile == NT - 1) commit(leader, empty + sn.slot);
+            step(sn);
+            return true;
+        };
+        uint32_t q_ph = 0, o_ph = 1;      // o_ph: the first item finds O free
+        bool ok = true;
+        for (int turn = 0; ok && turn * (int)gridDim.x < items; ++turn) {
+            const int at = fwd_at(turn);
+            if (at >= items) continue;
+            const FwdRange r = fwd_range<NT>(p, fwd_place<NT>(p, at));
+            const int total = NT * r.nblk;
+            ok = warp_wait(q_full, q_ph, abort_flag);
+            if (!ok) break;
+            q_ph ^= 1;
+            if (total == 0) {
+                if (leader) mbar_arrive(q_empty);
+                continue;
+            }
+            int issued = 0;
+            for (; ok && issued < Cf::NB && issued < total; ++issued) ok = scores();
+            if (ok && issued == total) commit(leader, q_empty);
             for (int n = 0; ok && n < total; ++n) {
-                ok = (pn.tile > 0 || warp_wait(full + pn.slot, pn.slot_ph, abort_flag)) &&
+                const int t = pn.tile;
+                ok = (t > 0 || warp_wait(full + pn.slot, pn.slot_ph, abort_flag)) &&
+                     (n >= NT || warp_wait(o_free + t, o_ph, abort_flag)) &&
                      warp_wait(p_full + pn.buf, pn.buf_ph, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                product_mn<128, 128>(leader, tmem + Cf::O_COL + pn.tile * Cf::O_STEP, tmem + pn.buf * 128,
+                product_mn<128, 128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + pn.buf * 128,
                                      kv_base + pn.slot * Cf::TILE, id_o, n >= NT);
-                commit(leader, pv_done + pn.tile);
-                if (pn.tile == NT - 1) commit(leader, n + 1 < total ? empty + pn.slot : o_full);
+                commit(leader, pv_done + t);
+                if (t == NT - 1) commit(leader, empty + pn.slot);
                 step(pn);
-                // behind the product that read the buffer's probabilities
-                if (n + Cf::NB < total) ok = scores();
+                if (issued < total) {     // behind the product that read the buffer's probabilities
+                    ok = scores();
+                    if (ok && ++issued == total) commit(leader, q_empty);
+                }
             }
-            if (!ok) {                    // no MMA may run on when the CTA ends
-                *abort_flag = 1;
-                err = ERR_MMA;
-                commit(leader, drain);
-                if (!mbar_wait_drain(drain, 0)) err |= ERR_DRAIN;
-            }
+            o_ph ^= 1;
+        }
+        if (!ok) {                        // no MMA may run on when the CTA ends
+            *abort_flag = 1;
+            err = ERR_MMA;
+            commit(leader, drain);
+            if (!mbar_wait_drain(drain, 0)) err |= ERR_DRAIN;
         }
     } else {
         const int t = warp / 4, row = (warp % 4) * 32 + lane;
-        const int i = q0 + t * 128 + row;
-        const uint32_t o_addr = tmem + Cf::O_COL + t * Cf::O_STEP + ((uint32_t)(warp % 4) << 21);
-        int row_end = i < ql ? kl : 0;
-        if (p.causal) row_end = min(row_end, i + kl - ql + 1);
-        float m = -INFINITY, l = 0.f;
+        const uint32_t lanes = (uint32_t)(warp % 4) << 21;
+        const uint32_t o_addr = tmem + Cf::O_COL + t * Cf::O_STEP + lanes;
+        uint8_t* stage = smem + Cf::STAGE_OFF + t * Cf::TILE;
+        int buf = t, vslot = 1;           // running places, as the MMA warp's
+        uint32_t buf_ph = 0, v_ph = 0, pv_ph = 1, out_ph = 0;
         bool ok = true;
-        for (int j = 0; j < nblk; ++j) {
-            const int n = j * NT + t, buf = n % Cf::NB;
-            const uint32_t s_addr = tmem + buf * 128 + ((uint32_t)(warp % 4) << 21);
-            ok = warp_wait(s_full + buf, n / Cf::NB & 1, abort_flag);
+        for (int turn = 0; ok && turn * (int)gridDim.x < items; ++turn) {
+            const int at = fwd_at(turn);
+            if (at >= items) continue;
+            int row_end, kl_left, nblk;       // from the part's first key block on
+            {
+                const FwdPlace w = fwd_place<NT>(p, at);
+                const FwdRange r = fwd_range<NT>(p, w);
+                const int i = w.q0 + t * 128 + row;
+                row_end = i < r.ql ? r.kl : 0;
+                if (p.causal) row_end = min(row_end, i + r.kl - r.ql + 1);
+                row_end -= r.blk0 * 128;
+                kl_left = r.kl - r.blk0 * 128;
+                nblk = r.nblk;
+            }
+            float m = -INFINITY, l = 0.f;
+            // this warpgroup's part in q_empty: here with staging tiles of their own, else at the end
+            auto seen_item = [&]() {
+                if (Cf::OWN_STAGE && warp % 4 == 0) {
+                    if (lane == 0) mbar_arrive(q_empty);
+                    __syncwarp();
+                }
+            };
+            if (nblk == 0) {
+                ok = warp_wait(q_full, out_ph, abort_flag);
+                if (!ok) break;
+                seen_item();
+            }
+            for (int j = 0; j < nblk; ++j) {
+                const uint32_t s_addr = tmem + buf * 128 + lanes;
+                ok = warp_wait(s_full + buf, buf_ph, abort_flag);
+                if (!ok) break;
+                if (j == 0) seen_item();
+                tc_fence_after();
+                // The scores are read twice, 64 columns for the maximum and then 32 at a time for the
+                // exponentials: held in registers over both they spilled, which cost more.
+                const int seen = row_end - j * 128;              // columns of this block that the row sees
+                const int least = -uniform(-seen);               // ... that every row of the warp sees
+                auto hide = [&](float* s, int c) {               // columns c .. c + 31
+                    if (least < c + 32)
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) s[x] = c + x < seen ? s[x] : -INFINITY;
+                };
+                float m_new = m;
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    uint32_t v[64];
+                    tmem_ld32_issue(s_addr + c, v);
+                    tmem_ld32_issue(s_addr + c + 32, v + 32);
+                    tmem_ld_wait<64>(v);
+                    float* s = reinterpret_cast<float*>(v);
+                    hide(s, c);
+                    hide(s + 32, c + 32);
+                    float mx[4] = {m_new, s[0], s[1], s[2]};
+#pragma unroll
+                    for (int x = 3; x < 63; x += 2) mx[x / 2 % 4] = max3(mx[x / 2 % 4], s[x], s[x + 1]);
+                    m_new = max3(fmaxf(mx[0], s[63]), mx[1], fmaxf(mx[2], mx[3]));
+                }
+                uint32_t v[2][32];
+                tmem_ld32_issue(s_addr, v[0]);
+                // the reference maximum moves when a row's maximum has grown by more than 2^8
+                const bool grow = j > 0 && __any_sync(~0u, (m_new - m) * p.scale2 > 8.f);
+                float f = 1.f;
+                if (j == 0) {
+                    m = m_new;
+                } else if (grow) {
+                    f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale2);
+                    l *= f;
+                    m = m_new;
+                }
+                const float sub = m == -INFINITY ? 0.f : -m * p.scale2;
+                const F2 sc = {p.scale2, p.scale2}, sb = {sub, sub};
+                F2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    tmem_ld_wait<32>(v[c % 2]);
+                    if (c < 3) tmem_ld32_issue(s_addr + c * 32 + 32, v[(c + 1) % 2]);
+                    float* s = reinterpret_cast<float*>(v[c % 2]);
+                    hide(s, c * 32);
+                    uint32_t w[16];
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        F2 e = fma2({s[2 * x], s[2 * x + 1]}, sc, sb);
+                        e.x = ex2(e.x);
+                        e.y = ex2(e.y);
+                        sum[x % 2] = add2(sum[x % 2], e);
+                        w[x] = pack16<DT>(e.x, e.y);
+                    }
+                    tmem_st16(s_addr + c * 16, w);
+                }
+                sum[0] = add2(sum[0], sum[1]);
+                l += sum[0].x + sum[0].y;
+                if (grow) {               // behind the last product that added to O
+                    ok = warp_wait(pv_done + t, pv_ph, abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
+                    for (int c = 0; c < p.D; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32_issue(o_addr + c, o);
+                        tmem_ld_wait<32>(o);
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                        tmem_st32(o_addr + c, o);
+                    }
+                }
+                // keys past the sequence's length may hold anything
+                if (t == 0 && kl_left - j * 128 < 128) {
+                    ok = warp_wait(full + vslot, v_ph, abort_flag);
+                    if (!ok) break;
+                    zero_tail<DP>(smem + Cf::KV_OFF + vslot * Cf::TILE, kl_left - j * 128, row);
+                }
+                tmem_st_wait();
+                tc_fence_before();
+                warp_arrive(p_full + buf);
+                buf += NT;
+                if (buf >= Cf::NB) { buf -= Cf::NB; buf_ph ^= 1; }
+                vslot += 2;
+                if (vslot >= Cf::SLOTS) { vslot -= Cf::SLOTS; v_ph ^= 1; }
+                pv_ph ^= 1;               // the phase of this block's product, the next block's last one
+            }
+            if (ok && nblk > 0) ok = warp_wait(pv_done + t, pv_ph, abort_flag);
+            // the last item's output has left the staging tile
+            if (ok && p.splits == 1) ok = warp_wait(stage_free + t, out_ph ^ 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
-            uint32_t sv[128];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_addr + c * 32, sv + c * 32);
-            tmem_ld_wait<128>(sv);
-            float* s = reinterpret_cast<float*>(sv);
-            const int seen = row_end - (blk0 + j) * 128;      // columns of this block that the row sees
-            if (__any_sync(~0u, seen < 128)) {
-#pragma unroll
-                for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
-            }
-            float mx[4] = {m, s[0], s[1], s[2]};
-#pragma unroll
-            for (int c = 3; c < 127; c += 2) mx[c / 2 % 4] = max3(mx[c / 2 % 4], s[c], s[c + 1]);
-            const float m_new = max3(fmaxf(mx[0], s[127]), mx[1], fmaxf(mx[2], mx[3]));
-            // the reference maximum moves when a row's maximum has grown by more than 2^8
-            const bool grow = j > 0 && __any_sync(~0u, (m_new - m) * p.scale2 > 8.f);
-            float f = 1.f;
-            if (j == 0) {
-                m = m_new;
-            } else if (grow) {
-                f = m == -INFINITY ? 0.f : ex2((m - m_new) * p.scale2);
-                l *= f;
-                m = m_new;
-            }
-            const float sub = m == -INFINITY ? 0.f : -m * p.scale2;
-            const F2 sc = {p.scale2, p.scale2}, sb = {sub, sub};
-            F2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t w[16];
-#pragma unroll
-                for (int x = 0; x < 16; ++x) {
-                    F2 e = fma2({s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]}, sc, sb);
-                    e.x = ex2(e.x);
-                    e.y = ex2(e.y);
-                    sum[x % 2] = add2(sum[x % 2], e);
-                    w[x] = pack16<DT>(e.x, e.y);
-                }
-                tmem_st16(s_addr + c * 16, w);
-            }
-            sum[0] = add2(sum[0], sum[1]);
-            l += sum[0].x + sum[0].y;
-            if (grow) {                   // behind the last product that added to O
-                ok = warp_wait(pv_done + t, (j - 1) & 1, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-                for (int c = 0; c < p.D; c += 32) {
-                    uint32_t o[32];
-                    tmem_ld32_issue(o_addr + c, o);
-                    tmem_ld_wait<32>(o);
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-                    tmem_st32(o_addr + c, o);
-                }
-            }
-            // keys past the sequence's length may hold anything
-            if (t == 0 && kl - (blk0 + j) * 128 < 128) {
-                const int iv = 2 * j + 1;
-                ok = warp_wait(full + iv % Cf::SLOTS, (iv / Cf::SLOTS) & 1, abort_flag);
-                if (!ok) break;
-                zero_tail<DP>(smem + (NT + iv % Cf::SLOTS) * Cf::TILE, kl - (blk0 + j) * 128, row);
-            }
-            tmem_st_wait();
-            tc_fence_before();
-            warp_arrive(p_full + buf);
-        }
-        if (ok && nblk > 0) ok = warp_wait(o_full, 0, abort_flag);
-        if (!ok) {
-            *abort_flag = 1;
-            err = ERR_MATH;
-        } else {
-            tc_fence_after();
+            int again = at;               // worked out again rather than held through the blocks
+            asm volatile("" : "+r"(again));
+            const FwdPlace w = fwd_place<NT>(p, again);
+            const int i = w.q0 + t * 128 + row;
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            const long long at = ((long long)b * p.H + h) * p.Sq + i;
-            uint8_t* tile = smem + t * Cf::TILE;      // Q's, which every product has read
-            float* part = i < p.Sq && p.splits > 1 ? p.part + ((long long)split * heads * p.Sq + at) * p.D : nullptr;
+            const long long rows = (long long)p.B * p.H * p.Sq, to = ((long long)w.b * p.H + w.h) * p.Sq + i;
+            float* part = i < p.Sq && p.splits > 1 ? p.part + (w.split * rows + to) * p.D : nullptr;
             for (int c = 0; c < p.D; c += 32) {
                 uint32_t o[32];
                 if (nblk > 0) {
                     tmem_ld32_issue(o_addr + c, o);
                     tmem_ld_wait<32>(o);
                 }
-                store_chunk<DT>(o, nblk > 0, inv, p.splits > 1, tile, row, part, c, p.D);
+                store_chunk<DT>(o, nblk > 0, inv, p.splits > 1, stage, row, part, c, p.D);
+            }
+            if (nblk > 0) {
+                tc_fence_before();
+                warp_arrive(o_free + t);
             }
             if (i < p.Sq) {
                 const float lse2 = l > 0.f ? m * p.scale2 + log2f(l) : -INFINITY;
                 if (p.splits > 1)
-                    p.part_lse[(long long)split * heads * p.Sq + at] = lse2;
+                    p.part_lse[w.split * rows + to] = lse2;
                 else if (p.lse)
-                    p.lse[at] = lse2 * LN2;
+                    p.lse[to] = lse2 * LN2;
             }
             if (p.splits == 1) {
                 fence_async_smem();
                 warp_arrive(out_ready + t);
                 if (warp % 4 == 0) {
-                    if (!warp_wait(out_ready + t, 0, abort_flag)) {
-                        err = ERR_MATH;
-                    } else if (lane == 0 && q0 + t * 128 < p.Sq) {
-                        store_tile(&mo, tile, p.D, q0 + t * 128, h, b);
-                        bulk_commit();
-                        bulk_wait_read<0>();
+                    ok = warp_wait(out_ready + t, out_ph, abort_flag);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        if (w.q0 + t * 128 < p.Sq) {
+                            store_tile(&mo, stage, p.D, w.q0 + t * 128, w.h, w.b);
+                            bulk_commit();
+                            bulk_wait_read<0>();
+                        }
+                        mbar_arrive(stage_free + t);
+                        if (!Cf::OWN_STAGE) mbar_arrive(q_empty);
                     }
+                    __syncwarp();
                 }
+            } else if (!Cf::OWN_STAGE) {
+                if (warp % 4 == 0 && lane == 0) mbar_arrive(q_empty);
+                __syncwarp();
             }
+            out_ph ^= 1;
+        }
+        if (!ok) {
+            *abort_flag = 1;
+            err = ERR_MATH;
         }
     }
     if (err) atomicOr(p.err, err);
@@ -594,7 +756,7 @@ struct BwdCfg {
     static constexpr int STAT_OFF = Y_OFF + SLOTS * Y_TILE;
     static constexpr int XE_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT, WG * 128 * 4);
     static constexpr int BAR_OFF = XE_OFF + XE_BYTES;
-    static constexpr int SMEM = BAR_OFF + 512 + 1024;
+    static constexpr int SMEM = BAR_OFF + 512;
     static constexpr int DP_COL = BN, ACC = 2 * BN, TMEM_COLS = 2 * BN + 2 * DP;
     static_assert(TMEM_COLS * OCC <= 512 && (SMEM + 1024) * OCC <= 228 * 1024, "on-chip memory");
 };
@@ -605,8 +767,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 const __grid_constant__ CUtensorMap my1, const __grid_constant__ CUtensorMap my2,
                 const __grid_constant__ CUtensorMap mo1, const __grid_constant__ CUtensorMap mo2, const Params p) {
     using Cf = BwdCfg<DP>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    // aligned by its declaration, so that every address below is a constant (rounded up at run time,
+    // the barriers' pointers took the registers that the scores need)
+    extern __shared__ __align__(1024) uint8_t smem[];
+    if (smem_u32(smem) % 1024) {
+        if (threadIdx.x == 0) atomicOr(p.err, ERR_LOAD);
+        return;
+    }
     float* stat = reinterpret_cast<float*>(smem + Cf::STAT_OFF);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BAR_OFF);
     uint64_t *x_full = bars, *s_full = bars + 1, *dp_full = bars + 2, *acc_full = bars + 3, *drain = bars + 4,
@@ -830,12 +997,15 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             }
             const int lo = row_lo - y0 - w * CW, hi = row_hi - y0 - w * CW;
             const bool mask = __any_sync(~0u, lo > 0 || hi < CW);
+            const bool some = __any_sync(~0u, max(lo, 0) < min(hi, CW));
+            if (some) {
 #pragma unroll
-            for (int c = 0; c < CW; c += 2) {
-                const F2 v = {pr[c], pr[c + 1]}, k = {p.scale2, p.scale2};
-                const F2 e = KV ? mul2(v, k) : fma2(v, k, {lse2, lse2});
-                pr[c] = ex2(e.x);
-                pr[c + 1] = ex2(e.y);
+                for (int c = 0; c < CW; c += 2) {
+                    const F2 v = {pr[c], pr[c + 1]}, k = {p.scale2, p.scale2};
+                    const F2 e = KV ? mul2(v, k) : fma2(v, k, {lse2, lse2});
+                    pr[c] = ex2(e.x);
+                    pr[c + 1] = ex2(e.y);
+                }
             }
             if (mask) {
 #pragma unroll
@@ -1088,9 +1258,16 @@ static int launch_fwd(DeviceCtx* c, const Params& p) {
     if (st == OM_OK && p.Sk > 0) st = encode(&mv, p.v, p.B, p.Sk, p.Hkv, p.D, DT);
     if (st == OM_OK && p.splits == 1) st = encode(&mo, p.o, p.B, p.Sq, p.H, p.D, DT);
     if (st != OM_OK) return st;
-    const long long grid = (long long)((p.Sq + NT * 128 - 1) / (NT * 128)) * p.B * p.H * p.splits;
-    if (grid > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-    kern<<<(unsigned)grid, Cf::THREADS, Cf::SMEM, c->compute>>>(mq, mk, mv, mo, p);
+    const long long items = (long long)((p.Sq + NT * 128 - 1) / (NT * 128)) * p.B * p.H * p.splits;
+    if (items > 0x7FFF0000) return OM_ERR_UNSUPPORTED;
+    const int tiles = (p.Sq + NT * 128 - 1) / (NT * 128);
+    Params q = p;
+    q.items = (int)items;
+    q.by_splits = div_by(p.splits);
+    q.by_fast = div_by(p.causal ? p.B * p.H : tiles);
+    q.by_heads = div_by(p.H);
+    const int places = c->num_sms * Cf::OCC, grid = q.items < places ? q.items : places;
+    kern<<<grid, Cf::THREADS, Cf::SMEM, c->compute>>>(mq, mk, mv, mo, q);
     return after_launch(c);
 }
 template <int DT>
