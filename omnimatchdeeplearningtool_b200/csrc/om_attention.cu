@@ -529,32 +529,20 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 if (!ok) break;
                 if (j == 0) seen_item();
                 tc_fence_after();
-                // The scores are read twice, 64 columns for the maximum and then 32 at a time for the
-                // exponentials: held in registers over both they spilled, which cost more.
                 const int seen = row_end - j * 128;              // columns of this block that the row sees
-                const int least = -uniform(-seen);               // ... that every row of the warp sees
-                auto hide = [&](float* s, int c) {               // columns c .. c + 31
-                    if (least < c + 32)
+                uint32_t sv[128];
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) s[x] = c + x < seen ? s[x] : -INFINITY;
-                };
-                float m_new = m;
+                for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_addr + c * 32, sv + c * 32);
+                tmem_ld_wait<128>(sv);
+                float* s = reinterpret_cast<float*>(sv);
+                if (__any_sync(~0u, seen < 128)) {
 #pragma unroll
-                for (int c = 0; c < 128; c += 64) {
-                    uint32_t v[64];
-                    tmem_ld32_issue(s_addr + c, v);
-                    tmem_ld32_issue(s_addr + c + 32, v + 32);
-                    tmem_ld_wait<64>(v);
-                    float* s = reinterpret_cast<float*>(v);
-                    hide(s, c);
-                    hide(s + 32, c + 32);
-                    float mx[4] = {m_new, s[0], s[1], s[2]};
-#pragma unroll
-                    for (int x = 3; x < 63; x += 2) mx[x / 2 % 4] = max3(mx[x / 2 % 4], s[x], s[x + 1]);
-                    m_new = max3(fmaxf(mx[0], s[63]), mx[1], fmaxf(mx[2], mx[3]));
+                    for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
                 }
-                uint32_t v[2][32];
-                tmem_ld32_issue(s_addr, v[0]);
+                float mx[4] = {m, s[0], s[1], s[2]};
+#pragma unroll
+                for (int c = 3; c < 127; c += 2) mx[c / 2 % 4] = max3(mx[c / 2 % 4], s[c], s[c + 1]);
+                const float m_new = max3(fmaxf(mx[0], s[127]), mx[1], fmaxf(mx[2], mx[3]));
                 // the reference maximum moves when a row's maximum has grown by more than 2^8
                 const bool grow = j > 0 && __any_sync(~0u, (m_new - m) * p.scale2 > 8.f);
                 float f = 1.f;
@@ -570,14 +558,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 F2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    tmem_ld_wait<32>(v[c % 2]);
-                    if (c < 3) tmem_ld32_issue(s_addr + c * 32 + 32, v[(c + 1) % 2]);
-                    float* s = reinterpret_cast<float*>(v[c % 2]);
-                    hide(s, c * 32);
                     uint32_t w[16];
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
-                        F2 e = fma2({s[2 * x], s[2 * x + 1]}, sc, sb);
+                        F2 e = fma2({s[c * 32 + 2 * x], s[c * 32 + 2 * x + 1]}, sc, sb);
                         e.x = ex2(e.x);
                         e.y = ex2(e.y);
                         sum[x % 2] = add2(sum[x % 2], e);
