@@ -438,6 +438,21 @@ def test_attention_rising_scores(gpu):
     c.check()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_more_tiles_than_the_gpu_holds(gpu, d, causal):
+    """Many more (batch, head, tile) items than places on the GPU, runs of empty entries among them."""
+    rng = np.random.Generator(np.random.PCG64(d))
+    b = 70
+    qlens = [int(x) for x in rng.integers(0, 161, b)]
+    klens = [int(x) for x in rng.integers(0, 301, b)]
+    for i in range(10, 40):
+        klens[i] = 0
+    for i in range(45, 60):
+        qlens[i] = 0
+    _Case(b, 9, 3, 160, 300, d, F16, causal=causal, qlens=qlens, klens=klens, garbage=True).check()
+
+
 def test_attention_packed_projection(gpu):
     """Q, K, V and their gradients as thirds of one [b, s, 3, h, d] tensor, in place."""
     from omnimatchdeeplearningtool_b200._lib import call
