@@ -342,7 +342,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     uint64_t* s_full = bars + 3;                 // per score buffer
     uint64_t* p_full = s_full + Cf::NB;
     uint64_t* pv_done = p_full + Cf::NB;         // per tile: O has a block's product
-    uint64_t* o_free = pv_done + NT;             // ... and has been read by the item's epilogue
+    uint64_t* o_full = pv_done + NT;             // ... and the item's last one
+    uint64_t* o_free = o_full + NT;              // ... and has been read by the item's epilogue
     uint64_t* out_ready = o_free + NT;           // the staging tile is written
     uint64_t* stage_free = out_ready + NT;       // ... and stored
     uint64_t* full = stage_free + NT;
@@ -361,6 +362,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         for (int i = 0; i < Cf::NB; ++i) { mbar_init(s_full + i, 1); mbar_init(p_full + i, 4); }
         for (int t = 0; t < NT; ++t) {
             mbar_init(pv_done + t, 1);
+            mbar_init(o_full + t, 1);
             mbar_init(o_free + t, 4);
             mbar_init(out_ready + t, 4);
             mbar_init(stage_free + t, 1);
@@ -473,6 +475,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 product_mn<128, 128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + pn.buf * 128,
                                      kv_base + pn.slot * Cf::TILE, id_o, n >= NT);
                 commit(leader, pv_done + t);
+                if (n >= total - NT) commit(leader, o_full + t);
                 if (t == NT - 1) commit(leader, empty + pn.slot);
                 step(pn);
                 if (issued < total) {     // behind the product that read the buffer's probabilities
@@ -494,7 +497,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         const uint32_t o_addr = tmem + Cf::O_COL + t * Cf::O_STEP + lanes;
         uint8_t* stage = smem + Cf::STAGE_OFF + t * Cf::TILE;
         int buf = t, vslot = 1;           // running places, as the MMA warp's
-        uint32_t buf_ph = 0, v_ph = 0, pv_ph = 1, out_ph = 0;
+        uint32_t buf_ph = 0, v_ph = 0, pv_ph = 1, o_ph = 0, out_ph = 0;
         bool ok = true;
         for (int turn = 0; ok && turn * (int)gridDim.x < items; ++turn) {
             const int at = fwd_at(turn);
@@ -571,7 +574,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 }
                 sum[0] = add2(sum[0], sum[1]);
                 l += sum[0].x + sum[0].y;
-                if (grow) {               // behind the last product that added to O
+                // behind the last product that added to O; the one before that was complete before S of
+                // this block was, so the phase is told by its parity
+                if (grow) {
                     ok = warp_wait(pv_done + t, pv_ph, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
@@ -599,7 +604,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 if (vslot >= Cf::SLOTS) { vslot -= Cf::SLOTS; v_ph ^= 1; }
                 pv_ph ^= 1;               // the phase of this block's product, the next block's last one
             }
-            if (ok && nblk > 0) ok = warp_wait(pv_done + t, pv_ph, abort_flag);
+            // o_full passes once an item and is waited for each time; pv_done's last phase must not
+            // be waited for here, since the one before it may still be open
+            if (ok && nblk > 0) {
+                ok = warp_wait(o_full + t, o_ph, abort_flag);
+                o_ph ^= 1;
+            }
             // the last item's output has left the staging tile
             if (ok && p.splits == 1) ok = warp_wait(stage_free + t, out_ph ^ 1, abort_flag);
             if (!ok) break;

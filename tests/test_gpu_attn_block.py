@@ -453,6 +453,25 @@ def test_attention_more_tiles_than_the_gpu_holds(gpu, d, causal):
     _Case(b, 9, 3, 160, 300, d, F16, causal=causal, qlens=qlens, klens=klens, garbage=True).check()
 
 
+def test_attention_serving_batch(gpu):
+    """A batch whose tiles take every CTA several turns: each entry repeats one of four (so that the
+    device's results can be compared with each other bit for bit), the four against 64 bits."""
+    from omnimatchdeeplearningtool_b200._lib import call
+    b, h, s, d = 64, 12, 197, 64
+    c = _Case(4, h, h, s, s, d, F16)
+    o, lse = c.forward()
+    c.check_forward()
+    st = (ctypes.c_longlong * 12)(*(_strides("bshd", b, s, h, d) * 4))
+    qd, kd, vd = (_dev(np.tile(x, (b // 4, 1, 1, 1)), F16) for x in (c.q, c.k, c.v))
+    for _ in range(3):
+        out, ls = _new(b * s * h * d * 2), _new(b * h * s * 4)
+        call("omCudaAttention", qd.ptr, kd.ptr, vd.ptr, out.ptr, ls.ptr, st, None, None, None, b, h, h, s, s, d,
+             float(c.scale), 0, F16)
+        got = _get(out, (b, s, h, d), F16)
+        assert (got == np.tile(o, (b // 4, 1, 1, 1))).all()
+        assert (ls.to_numpy((b, h, s)) == np.tile(lse, (b // 4, 1, 1))).all()
+
+
 def test_attention_packed_projection(gpu):
     """Q, K, V and their gradients as thirds of one [b, s, 3, h, d] tensor, in place."""
     from omnimatchdeeplearningtool_b200._lib import call
