@@ -260,7 +260,7 @@ __device__ __forceinline__ void store_tile(const CUtensorMap* map, const uint8_t
 constexpr float LN2 = 0.6931471805599453f;
 
 // ---------------------------------------------------------------- forward
-// One item of work: NT tiles of 128 queries of one (batch, head) over the key blocks of 128 (or one
+// One item of work: NT tiles of 128 queries of one (batch, head) over the blocks of KB keys (or one
 // part of them). A CTA stays on its SM and takes every gridDim.x-th item: a softmax warpgroup per
 // tile (thread = query row), a TMA warp and an MMA warp, each running ahead of the others as far as
 // the buffers go, so that an item's loads and first scores come beside the last one's end (with a
@@ -272,23 +272,25 @@ constexpr float LN2 = 0.6931471805599453f;
 // O is rescaled only when a row's maximum has grown by more than 2^8 since its last reference
 // maximum: P stays below 2^8, in range of both types, and the factor cancels in O / l.
 // Score tile n = NT j + t (block j, query tile t) lies in TMEM buffer n % NB, counted over all items.
-// With heads up to 64 there is room for a third buffer, so that a tile's next scores are there when
-// its probabilities are done (without it a softmax warp waited about 900 of 2900 clocks a block for
-// them).
+// There are more buffers than query tiles, so that a tile's next scores are there when its
+// probabilities are done (without, a softmax warp waited about 900 of 2900 clocks a block for them):
+// blocks of KB = 128 keys and three buffers with heads up to 64; longer heads' O fills half of TMEM,
+// so there are four buffers of 64 keys.
 // TMEM: NB score tiles, then the O tiles.
 template <int DP, int NT>
 struct FwdCfg {
-    static constexpr int TILE = DP / 64 * PANEL;
-    static constexpr int SLOTS = NT == 2 ? (DP == 128 ? 4 : 6) : (DP == 128 ? 2 : 4);
+    static constexpr int KB = DP == 128 ? 64 : 128;
+    static constexpr int TILE = DP / 64 * PANEL, KV_TILE = DP / 64 * KB * 128;
+    static constexpr int SLOTS = NT == 2 ? (DP == 128 ? 8 : 6) : 4;
     // the output's staging tiles: Q's with long heads, which shared memory then holds no others beside
     static constexpr bool OWN_STAGE = DP == 64;
-    static constexpr int KV_OFF = NT * TILE, STAGE_OFF = OWN_STAGE ? KV_OFF + SLOTS * TILE : 0;
-    static constexpr int BAR_OFF = KV_OFF + (SLOTS + (OWN_STAGE ? NT : 0)) * TILE;
+    static constexpr int KV_OFF = NT * TILE, STAGE_OFF = OWN_STAGE ? KV_OFF + SLOTS * KV_TILE : 0;
+    static constexpr int BAR_OFF = KV_OFF + SLOTS * KV_TILE + (OWN_STAGE ? NT * TILE : 0);
     static constexpr int SMEM = BAR_OFF + 512;
     static constexpr int THREADS = NT * 128 + 64, OCC = NT == 1 ? 2 : 1;
     static constexpr int TMEM_COLS = NT * 256;
-    static constexpr int NB = NT == 2 && DP == 64 ? 3 : NT;
-    static constexpr int O_COL = NB * 128, O_STEP = DP;
+    static constexpr int NB = DP == 128 ? 2 * NT : NT == 2 ? 3 : 1;
+    static constexpr int O_COL = NB * KB, O_STEP = DP;
     static_assert(O_COL + NT * O_STEP <= TMEM_COLS && (SMEM + 1024) * OCC <= 228 * 1024, "on-chip memory");
 };
 enum : unsigned int { ERR_LOAD = ERRBIT_TC_PRODUCER, ERR_MMA = ERRBIT_TC_MMA,
@@ -309,7 +311,7 @@ __device__ __forceinline__ FwdPlace fwd_place(const Params& p, int at) {
     const int b = p.by_heads(bh);
     return {b, bh - b * p.H, tile * (NT * 128), at - i * p.splits};
 }
-template <int NT>
+template <int NT, int KB>
 __device__ __forceinline__ FwdRange fwd_range(const Params& p, const FwdPlace& w) {
     FwdRange r;
     r.ql = len_of(p.qlens, w.b, p.Sq);
@@ -317,7 +319,7 @@ __device__ __forceinline__ FwdRange fwd_range(const Params& p, const FwdPlace& w
     int end = w.q0 < r.ql ? r.kl : 0;
     if (p.causal) end = min(end, min(w.q0 + NT * 128, r.ql) + r.kl - r.ql);
     // this part's key blocks: blk0 .. blk0 + nblk - 1
-    const int all = end > 0 ? (end + 127) / 128 : 0, share = p.by_splits(all + p.splits - 1);
+    const int all = end > 0 ? (end + KB - 1) / KB : 0, share = p.by_splits(all + p.splits - 1);
     r.blk0 = w.split * share;
     r.nblk = uniform(max(0, min(all - r.blk0, share)));
     return r;
@@ -352,7 +354,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
 
     const int warp = uniform((int)threadIdx.x / 32), lane = threadIdx.x % 32;
-    constexpr int W_LOAD = NT * 4, W_MMA = NT * 4 + 1;
+    constexpr int W_LOAD = NT * 4, W_MMA = NT * 4 + 1, KB = Cf::KB;
     const int items = p.items;
 
     if (threadIdx.x == 0) {
@@ -390,7 +392,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             const int at = fwd_at(turn);
             if (at >= items) continue;
             const FwdPlace w = fwd_place<NT>(p, at);
-            const FwdRange r = fwd_range<NT>(p, w);
+            const FwdRange r = fwd_range<NT, Cf::KB>(p, w);
             ok = warp_wait(q_empty, item_ph, abort_flag);
             if (!ok) break;
             item_ph ^= 1;
@@ -406,9 +408,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 ok = warp_wait(empty + slot, slot_ph, abort_flag);
                 if (!ok) break;
                 if (lane == 0) {
-                    mbar_expect_tx(full + slot, Cf::TILE);
-                    load_tile<DP>(Cf::KV_OFF + slot * Cf::TILE, smem, i & 1 ? &mv : &mk, full + slot,
-                                  (r.blk0 + i / 2) * 128, hk, w.b);
+                    mbar_expect_tx(full + slot, Cf::KV_TILE);
+                    load_tile<DP, KB>(Cf::KV_OFF + slot * Cf::KV_TILE, smem, i & 1 ? &mv : &mk, full + slot,
+                                      (r.blk0 + i / 2) * KB, hk, w.b);
                 }
                 ++issued;
                 if (++slot == Cf::SLOTS) { slot = 0; slot_ph ^= 1; }
@@ -424,7 +426,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     } else if (warp == W_MMA) {
         const uint32_t leader = elect();
         const int ks = (p.D + 15) / 16;
-        const uint32_t id_s = idesc_f16(DT == OM_DTYPE_F16, 128, false, p.neg);
+        const uint32_t id_s = idesc_f16(DT == OM_DTYPE_F16, KB, false, p.neg);
         const uint32_t id_o = idesc_f16(DT == OM_DTYPE_F16, ks * 16, true, false);
         const uint32_t q_tile = smem_u32(smem), kv_base = q_tile + Cf::KV_OFF;
         // Running places: slot and TMEM buffer of the scores to issue next (sn) and of the
@@ -441,7 +443,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         auto scores = [&]() {             // one score tile, and K's slot back behind the block's last
             if (sn.tile == 0 && !warp_wait(full + sn.slot, sn.slot_ph, abort_flag)) return false;
             tc_fence_after();
-            product_k<DP, 128>(leader, tmem + sn.buf * 128, q_tile + sn.tile * Cf::TILE, kv_base + sn.slot * Cf::TILE,
+            product_k<DP, KB>(leader, tmem + sn.buf * KB, q_tile + sn.tile * Cf::TILE, kv_base + sn.slot * Cf::KV_TILE,
                                id_s, ks);
             commit(leader, s_full + sn.buf);
             if (sn.tile == NT - 1) commit(leader, empty + sn.slot);
@@ -453,7 +455,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         for (int turn = 0; ok && turn * (int)gridDim.x < items; ++turn) {
             const int at = fwd_at(turn);
             if (at >= items) continue;
-            const FwdRange r = fwd_range<NT>(p, fwd_place<NT>(p, at));
+            const FwdRange r = fwd_range<NT, Cf::KB>(p, fwd_place<NT>(p, at));
             const int total = NT * r.nblk;
             ok = warp_wait(q_full, q_ph, abort_flag);
             if (!ok) break;
@@ -472,8 +474,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                      warp_wait(p_full + pn.buf, pn.buf_ph, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                product_mn<128, 128>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + pn.buf * 128,
-                                     kv_base + pn.slot * Cf::TILE, id_o, n >= NT);
+                product_mn<KB, KB>(leader, tmem + Cf::O_COL + t * Cf::O_STEP, tmem + pn.buf * KB,
+                                   kv_base + pn.slot * Cf::KV_TILE, id_o, n >= NT);
                 commit(leader, pv_done + t);
                 if (n >= total - NT) commit(leader, o_full + t);
                 if (t == NT - 1) commit(leader, empty + pn.slot);
@@ -505,12 +507,12 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             int row_end, kl_left, nblk;       // from the part's first key block on
             {
                 const FwdPlace w = fwd_place<NT>(p, at);
-                const FwdRange r = fwd_range<NT>(p, w);
+                const FwdRange r = fwd_range<NT, Cf::KB>(p, w);
                 const int i = w.q0 + t * 128 + row;
                 row_end = i < r.ql ? r.kl : 0;
                 if (p.causal) row_end = min(row_end, i + r.kl - r.ql + 1);
-                row_end -= r.blk0 * 128;
-                kl_left = r.kl - r.blk0 * 128;
+                row_end -= r.blk0 * KB;
+                kl_left = r.kl - r.blk0 * KB;
                 nblk = r.nblk;
             }
             float m = -INFINITY, l = 0.f;
@@ -527,25 +529,25 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 seen_item();
             }
             for (int j = 0; j < nblk; ++j) {
-                const uint32_t s_addr = tmem + buf * 128 + lanes;
+                const uint32_t s_addr = tmem + buf * KB + lanes;
                 ok = warp_wait(s_full + buf, buf_ph, abort_flag);
                 if (!ok) break;
                 if (j == 0) seen_item();
                 tc_fence_after();
-                const int seen = row_end - j * 128;              // columns of this block that the row sees
-                uint32_t sv[128];
+                const int seen = row_end - j * KB;              // columns of this block that the row sees
+                uint32_t sv[KB];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld32_issue(s_addr + c * 32, sv + c * 32);
-                tmem_ld_wait<128>(sv);
+                for (int c = 0; c < KB / 32; ++c) tmem_ld32_issue(s_addr + c * 32, sv + c * 32);
+                tmem_ld_wait<KB>(sv);
                 float* s = reinterpret_cast<float*>(sv);
-                if (__any_sync(~0u, seen < 128)) {
+                if (__any_sync(~0u, seen < KB)) {
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) s[c] = c < seen ? s[c] : -INFINITY;
+                    for (int c = 0; c < KB; ++c) s[c] = c < seen ? s[c] : -INFINITY;
                 }
                 float mx[4] = {m, s[0], s[1], s[2]};
 #pragma unroll
-                for (int c = 3; c < 127; c += 2) mx[c / 2 % 4] = max3(mx[c / 2 % 4], s[c], s[c + 1]);
-                const float m_new = max3(fmaxf(mx[0], s[127]), mx[1], fmaxf(mx[2], mx[3]));
+                for (int c = 3; c < KB - 1; c += 2) mx[c / 2 % 4] = max3(mx[c / 2 % 4], s[c], s[c + 1]);
+                const float m_new = max3(fmaxf(mx[0], s[KB - 1]), mx[1], fmaxf(mx[2], mx[3]));
                 // the reference maximum moves when a row's maximum has grown by more than 2^8
                 const bool grow = j > 0 && __any_sync(~0u, (m_new - m) * p.scale2 > 8.f);
                 float f = 1.f;
@@ -560,7 +562,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 const F2 sc = {p.scale2, p.scale2}, sb = {sub, sub};
                 F2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < KB / 32; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int x = 0; x < 16; ++x) {
@@ -590,10 +592,10 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     }
                 }
                 // keys past the sequence's length may hold anything
-                if (t == 0 && kl_left - j * 128 < 128) {
+                if (t == 0 && kl_left - j * KB < KB) {
                     ok = warp_wait(full + vslot, v_ph, abort_flag);
                     if (!ok) break;
-                    zero_tail<DP>(smem + Cf::KV_OFF + vslot * Cf::TILE, kl_left - j * 128, row);
+                    zero_tail<DP, KB>(smem + Cf::KV_OFF + vslot * Cf::KV_TILE, kl_left - j * KB, row);
                 }
                 tmem_st_wait();
                 tc_fence_before();
@@ -1248,8 +1250,8 @@ static int launch_fwd(DeviceCtx* c, const Params& p) {
     }
     CUtensorMap mq = {}, mk = {}, mv = {}, mo = {};
     int st = encode(&mq, p.q, p.B, p.Sq, p.H, p.D, DT);
-    if (st == OM_OK && p.Sk > 0) st = encode(&mk, p.k, p.B, p.Sk, p.Hkv, p.D, DT);
-    if (st == OM_OK && p.Sk > 0) st = encode(&mv, p.v, p.B, p.Sk, p.Hkv, p.D, DT);
+    if (st == OM_OK && p.Sk > 0) st = encode(&mk, p.k, p.B, p.Sk, p.Hkv, p.D, DT, Cf::KB);
+    if (st == OM_OK && p.Sk > 0) st = encode(&mv, p.v, p.B, p.Sk, p.Hkv, p.D, DT, Cf::KB);
     if (st == OM_OK && p.splits == 1) st = encode(&mo, p.o, p.B, p.Sq, p.H, p.D, DT);
     if (st != OM_OK) return st;
     const long long items = (long long)((p.Sq + NT * 128 - 1) / (NT * 128)) * p.B * p.H * p.splits;
