@@ -274,14 +274,16 @@ constexpr float LN2 = 0.6931471805599453f;
 // Score tile n = NT j + t (block j, query tile t) lies in TMEM buffer n % NB, counted over all items.
 // There are more buffers than query tiles, so that a tile's next scores are there when its
 // probabilities are done (without, a softmax warp waited about 900 of 2900 clocks a block for them):
-// blocks of KB = 128 keys and three buffers with heads up to 64; longer heads' O fills half of TMEM,
-// so there are four buffers of 64 keys.
+// blocks of KB = 128 keys and three buffers for two tiles of heads up to 64 (24 heads of 4096 tokens:
+// 154 us, with 64 keys 176 us). Longer heads' O fills half of TMEM, and with one tile two CTAs share
+// an SM, so there are two buffers of 64 keys a tile (768 heads of 64 queries over 2000 keys: 98 us,
+// with one buffer of 128 keys 121 us).
 // TMEM: NB score tiles, then the O tiles.
 template <int DP, int NT>
 struct FwdCfg {
-    static constexpr int KB = DP == 128 ? 64 : 128;
+    static constexpr int KB = DP == 128 || NT == 1 ? 64 : 128;
     static constexpr int TILE = DP / 64 * PANEL, KV_TILE = DP / 64 * KB * 128;
-    static constexpr int SLOTS = NT == 2 ? (DP == 128 ? 8 : 6) : 4;
+    static constexpr int SLOTS = NT == 2 ? (DP == 128 ? 8 : 6) : (DP == 128 ? 4 : 8);
     // the output's staging tiles: Q's with long heads, which shared memory then holds no others beside
     static constexpr bool OWN_STAGE = DP == 64;
     static constexpr int KV_OFF = NT * TILE, STAGE_OFF = OWN_STAGE ? KV_OFF + SLOTS * KV_TILE : 0;
@@ -289,7 +291,7 @@ struct FwdCfg {
     static constexpr int SMEM = BAR_OFF + 512;
     static constexpr int THREADS = NT * 128 + 64, OCC = NT == 1 ? 2 : 1;
     static constexpr int TMEM_COLS = NT * 256;
-    static constexpr int NB = DP == 128 ? 2 * NT : NT == 2 ? 3 : 1;
+    static constexpr int NB = KB == 64 ? 2 * NT : 3;
     static constexpr int O_COL = NB * KB, O_STEP = DP;
     static_assert(O_COL + NT * O_STEP <= TMEM_COLS && (SMEM + 1024) * OCC <= 228 * 1024, "on-chip memory");
 };
