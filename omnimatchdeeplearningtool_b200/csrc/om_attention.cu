@@ -340,8 +340,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
         return;
     }
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Cf::BAR_OFF);
-    // q_full and q_empty pass once an item, with key blocks or without, and every role takes part:
-    // so no role is ever two phases of a barrier ahead of another
+    // q_full and q_empty pass once an item, with key blocks or without. Only warps that arrive on
+    // q_empty wait for q_full, each time: so none is ever two phases of a barrier behind another
     uint64_t *q_full = bars, *q_empty = bars + 1, *drain = bars + 2;
     uint64_t* s_full = bars + 3;                 // per score buffer
     uint64_t* p_full = s_full + Cf::NB;
@@ -525,7 +525,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                     __syncwarp();
                 }
             };
-            if (nblk == 0) {
+            if (nblk == 0 && warp % 4 == 0) {
                 ok = warp_wait(q_full, out_ph, abort_flag);
                 if (!ok) break;
                 seen_item();

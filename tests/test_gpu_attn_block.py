@@ -453,6 +453,19 @@ def test_attention_more_tiles_than_the_gpu_holds(gpu, d, causal):
     _Case(b, 9, 3, 160, 300, d, F16, causal=causal, qlens=qlens, klens=klens, garbage=True).check()
 
 
+@pytest.mark.parametrize("b,h,s,causal,d", [(3, 4, 1100, True, 40), (1, 12, 900, False, 64), (2, 6, 1000, True, 128)])
+def test_attention_parts_in_turns(gpu, b, h, s, causal, d):
+    """Tiles split into parts, several turns a CTA, and parts without keys beside full ones; repeated,
+    as what one warp does ahead of another differs from run to run."""
+    kl = [s, s // 7, s // 3][:b]
+    c = _Case(b, h, h, s, s, d, BF16, causal=causal, klens=kl, garbage=True)
+    o, lse, p, es = c.check_forward()
+    first = c.forward()
+    for _ in range(20):
+        got = c.forward()
+        assert (got[0] == first[0]).all() and (got[1] == first[1]).all()
+
+
 def test_attention_serving_batch(gpu):
     """A batch whose tiles take every CTA several turns: each entry repeats one of four (so that the
     device's results can be compared with each other bit for bit), the four against 64 bits."""
