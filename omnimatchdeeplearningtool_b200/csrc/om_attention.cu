@@ -289,7 +289,14 @@ struct FwdCfg {
     static constexpr int KV_OFF = NT * TILE, STAGE_OFF = OWN_STAGE ? KV_OFF + SLOTS * KV_TILE : 0;
     static constexpr int BAR_OFF = KV_OFF + SLOTS * KV_TILE + (OWN_STAGE ? NT * TILE : 0);
     static constexpr int SMEM = BAR_OFF + 512;
-    static constexpr int THREADS = NT * 128 + 64, OCC = NT == 1 ? 2 : 1;
+    // A row's 128 scores and what goes with them need more than the 168 registers that 320 or 384
+    // threads can have each (114 bytes spilled): the softmax warps take what the other warpgroup,
+    // whose last two warps idle, gives back. 24 heads of 4096 tokens: 154 -> 145 us
+    static constexpr bool MORE_REGS = KB == 128;
+    static constexpr int THREADS = NT * 128 + (MORE_REGS ? 128 : 64), OCC = NT == 1 ? 2 : 1;
+    static constexpr int MATH_REGS = 208, OTHER_REGS = 80;
+    // registers a thread that the launch must have for that split, else the softmax warps would wait
+    static constexpr int LAUNCH_REGS = MORE_REGS ? (NT * 128 * MATH_REGS + 128 * OTHER_REGS + THREADS - 1) / THREADS : 0;
     static constexpr int TMEM_COLS = NT * 256;
     static constexpr int NB = KB == 64 ? 2 * NT : 3;
     static constexpr int O_COL = NB * KB, O_STEP = DP;
@@ -328,7 +335,7 @@ __device__ __forceinline__ FwdRange fwd_range(const Params& p, const FwdPlace& w
 }
 
 template <int DP, int NT, int DT>
-__global__ void __launch_bounds__(NT * 128 + 64, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(FwdCfg<DP, NT>::THREADS, FwdCfg<DP, NT>::OCC)
 attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                 const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mo, const Params p) {
     using Cf = FwdCfg<DP, NT>;
@@ -385,6 +392,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
     tc_fence_after();
     const uint32_t tmem = uniform(*tmem_holder);
     unsigned int err = 0;
+    if (Cf::MORE_REGS && warp >= W_LOAD) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cf::OTHER_REGS));
 
     if (warp == W_LOAD) {
         int slot = 0, issued = 0, queries = 0;   // queries: phases of q_full so far
@@ -495,7 +503,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             commit(leader, drain);
             if (!mbar_wait_drain(drain, 0)) err |= ERR_DRAIN;
         }
-    } else {
+    } else if (warp < W_LOAD) {
+        if (Cf::MORE_REGS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cf::MATH_REGS));
         const int t = warp / 4, row = (warp % 4) * 32 + lane;
         const uint32_t lanes = (uint32_t)(warp % 4) << 21;
         const uint32_t o_addr = tmem + Cf::O_COL + t * Cf::O_STEP + lanes;
@@ -1247,6 +1256,9 @@ static int launch_fwd(DeviceCtx* c, const Params& p) {
     auto kern = attn_fwd_kernel<DP, NT, DT>;
     static bool attr_set[64] = {false};
     if (!attr_set[c->device]) {
+        cudaFuncAttributes fa;
+        OMB_CHECK(cudaFuncGetAttributes(&fa, kern));
+        if (fa.numRegs < Cf::LAUNCH_REGS) return OM_ERR_UNSUPPORTED;   // built with other limits
         OMB_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cf::SMEM));
         attr_set[c->device] = true;
     }
