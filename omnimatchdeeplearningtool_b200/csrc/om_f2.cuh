@@ -1,4 +1,5 @@
-// Pairs of fp32 values and the sm_100 instructions that work on both at once.
+// Pairs of fp32 values and the sm_100 instructions that work on both at once. A product whose only use
+// is a sum may come out fused with it, rounded once: where that matters, use __fmul_rn and __fadd_rn.
 #pragma once
 
 namespace omb {

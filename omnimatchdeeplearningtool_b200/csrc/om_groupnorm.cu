@@ -477,7 +477,13 @@ __device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy,
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         xh[i] = mul2(add2(xh[i], pair_of<GV>(f.minus_mean, i)), pair_of<GV>(f.rstd, i));
-        dz[i] = act_bwd<ACT>(dz[i], fma2(xh[i], f.gamma[i], f.beta[i]));
+        // Where z's sign decides, product and sum are rounded apart, as the formula reads: fused (as the
+        // paired instructions can be), a z that rounds to 0 came out next to 0 and let its gradient through
+        const F2 z = ACT == OM_ACT_RELU || ACT == OM_ACT_RELU6
+                         ? F2{__fadd_rn(__fmul_rn(xh[i].x, f.gamma[i].x), f.beta[i].x),
+                              __fadd_rn(__fmul_rn(xh[i].y, f.gamma[i].y), f.beta[i].y)}
+                         : fma2(xh[i], f.gamma[i], f.beta[i]);
+        dz[i] = act_bwd<ACT>(dz[i], z);
     }
 }
 // the sums that a thread keeps of them: dz, and dz xh

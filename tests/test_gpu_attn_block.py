@@ -114,6 +114,25 @@ def test_group_norm(gpu, shape, dtype, kind):
     assert (np.abs(gb.to_numpy((c,)) - dbet) <= sums + lost + 1e-30).all()
 
 
+@pytest.mark.parametrize("kind", [1, 2])
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_group_norm_backward_at_the_kink(gpu, dtype, kind):
+    """((x - mean) * rstd) * gamma + beta is 0 in fp32 and below 0 without rounding (-2.7e-9): no gradient."""
+    from omnimatchdeeplearningtool_b200._lib import call
+    n, hw, c = 1, 300, 8
+    mean, rstd, gamma, beta = (np.array([v], np.uint32).view(np.float32) for v in
+                               (0xbe7efff0, 0x3f67b984, 0x3f47aba7, 0x3e1933e6))
+    x = np.float32(-0.4609375)
+    assert (x - mean) * rstd * gamma + beta == 0
+    xd, dyd = _dev(np.full((n, hw, c), x), dtype), _dev(np.ones((n, hw, c)), dtype)
+    md, rd, gd, bd = _dev(mean), _dev(rstd), _dev(np.repeat(gamma, c)), _dev(np.repeat(beta, c))
+    dx, dg, db = _new(n * hw * c * 4), _new(c * 4), _new(c * 4)
+    call("omCudaGroupNormActNhwcBackward", dyd.ptr, xd.ptr, md.ptr, rd.ptr, gd.ptr, bd.ptr, dx.ptr, dg.ptr, db.ptr,
+         _gn_ws(n, hw, c, c, 1, dtype, 1).ptr, n, hw, c, c, 1, kind, dtype)
+    assert (_get(dx, (n, hw, c), dtype) == 0).all()
+    assert (dg.to_numpy((c,)) == 0).all() and (db.to_numpy((c,)) == 0).all()
+
+
 def test_group_norm_optional_arguments_in_place_and_repeat(gpu):
     from omnimatchdeeplearningtool_b200._lib import call
     rng = np.random.Generator(np.random.PCG64(5))
