@@ -274,10 +274,10 @@ constexpr float LN2 = 0.6931471805599453f;
 // Score tile n = NT j + t (block j, query tile t) lies in TMEM buffer n % NB, counted over all items.
 // There are more buffers than query tiles, so that a tile's next scores are there when its
 // probabilities are done (without, a softmax warp waited about 900 of 2900 clocks a block for them):
-// blocks of KB = 128 keys and three buffers for two tiles of heads up to 64 (24 heads of 4096 tokens, with 168 registers a thread:
-// 154 us, with 64 keys 176 us). Longer heads' O fills half of TMEM, and with one tile two CTAs share
-// an SM, so there are two buffers of 64 keys a tile (768 heads of 64 queries over 2000 keys: 98 us,
-// with one buffer of 128 keys 121 us).
+// blocks of KB = 128 keys and three buffers for two tiles of heads up to 64 (24 heads of 4096 tokens,
+// with 168 registers a thread: 154 us, with 64 keys 176 us). Longer heads' O fills half of TMEM, and
+// with one tile two CTAs share an SM, so there are two buffers of 64 keys a tile (768 heads of 64
+// queries over 2000 keys: 98 us, with one buffer of 128 keys 121 us).
 // TMEM: NB score tiles, then the O tiles.
 template <int DP, int NT>
 struct FwdCfg {
