@@ -647,7 +647,8 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
                 warp_arrive(o_free + t);
             }
             if (i < p.Sq) {
-                const float lse2 = l > 0.f ? m * p.scale2 + log2f(l) : -INFINITY;
+                // l is relative to the rounded product, as `sub` had it: fused with the sum, it would not be
+                const float lse2 = l > 0.f ? __fadd_rn(__fmul_rn(m, p.scale2), log2f(l)) : -INFINITY;
                 if (p.splits > 1)
                     p.part_lse[w.split * rows + to] = lse2;
                 else if (p.lse)
