@@ -654,8 +654,9 @@ int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut, 
  * pOut is the forward's output. pStrides: 24 element strides, (batch, token, head) of Q, K, V,
  * out, dOut, dQ, dK, dV. dK and dV sum over the query heads that share a key/value head. dQ of
  * queries that see no key or lie past their length, and dK, dV of keys past theirs, are zeros.
- * dQ, dK and dV must not overlap an input. |fScale| below 2^-20 is OM_ERR_UNSUPPORTED (lse and the
- * like enter a product divided by it). */
+ * dQ, dK and dV must not overlap an input. |fScale| below 2^-20 is OM_ERR_UNSUPPORTED (lse enters a
+ * product divided by it). With F16, a query's |lse / fScale| and |sum(dOut * out)| enter dK and dV up
+ * to 2^31 (cut to that beyond, where fp32 scores no longer tell keys apart). */
 int omCudaAttentionBackward(const void* pGradOut, const void* pQ, const void* pK, const void* pV,
                             const void* pOut, const float* pLse, void* pGradQ, void* pGradK,
                             void* pGradV, const long long* pStrides, const int* pQLens,

@@ -38,8 +38,7 @@ struct Params {
     const int *qlens, *kvlens;
     int B, H, Hkv, Sq, Sk, D, causal;
     float scale;
-    float lse_unit;    // the backward's 2^a near 1 / |scale|, and what turns -lse log2(e) into the
-    float lse_part;    // value whose parts are kept: 1 / (scale2 2^a)
+    float inv_scale;   // 1 / |scale|, for the backward
     float scale2;      // |scale| * log2(e), not 0 (masked scores stay minus infinity)
     bool neg;          // scale < 0: the score products negate Q
     unsigned int* err;
@@ -714,13 +713,14 @@ constexpr int BWD_COLS = 32;
 // them one by one (from shared memory 1024 broadcast wavefronts a 128 x 128 tile, more than the
 // products' own operands take: 303 us against 211 us without any arithmetic, 24 heads of 4096
 // tokens x 64). So they enter through the products: one more step of 16 columns, in which the
-// streamed side has -lse / |scale| and -delta and the kept side constants. Each value is three
-// 16-bit parts, h + 2^-11 m + 2^-22 l (24 bits and more), so nothing of fp32 is lost:
+// streamed side has -lse / |scale| and -delta and the kept side constants. Each value is four 16-bit
+// parts of the units U = (2^15, 2^4, 2^-7, 2^-18), so nothing of fp32 is lost:
 //   S^T - lse / |scale| = K Q^T + XE1 YE^T, dP^T - delta = V dO^T + XE2 YE^T,
-//   YE = (parts of -lse / |scale| / 2^a, parts of -delta / 16, 0 ...),
-//   XE1 = 2^a (1, 2^-11, 2^-22, 0 ...), XE2 = 16 (0, 0, 0, 1, 2^-11, 2^-22, 0 ...),
-// with 2^a near 1 / |scale| to keep the parts in range of fp16. Without swizzle, as core matrices of
-// 8 rows x 8 columns (128 bytes); the columns 8..15 are zeros.
+//   YE = (parts of -lse / |scale|, parts of -delta, 0 ...), XE1 = (U, 0 ...), XE2 = (0 0 0 0, U, 0 ...).
+// In fp16 the parts reach from 2^31 down to 2^-42, which covers every lse of scores that fp32 can
+// tell apart (and delta alike); what lies beyond is cut to that, so that no part is ever an infinity
+// or, times the other value's zeros, a NaN in every key's sums. Without swizzle, as core matrices of 8
+// rows x 8 columns (128 bytes); the columns 8..15 are zeros.
 // The dQ kernel leaves YE in the workspace as [batch][head][64 queries][8 rows][2 cores].
 constexpr int STAT_TILE = 2048;                              // bytes of 64 queries
 constexpr int XE_REGION = 128 * 16, XE_BYTES = 3 * XE_REGION;   // XE2's and XE1's first cores, zeros
@@ -739,14 +739,18 @@ __device__ __forceinline__ void product_plain(uint32_t leader, uint32_t d_tmem, 
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
         "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(plain_hi(128)), "r"(plain_hi(256)), "r"(leader));
 }
-// the three parts of a value in the first three elements at `out`
+// the four parts of a value and their units: each part is what the ones before it left, rounded
+__device__ __forceinline__ float part_unit(int i) { return i == 0 ? 0x1p15f : i == 1 ? 0x1p4f : i == 2 ? 0x1p-7f : 0x1p-18f; }
 template <int DT>
-__device__ __forceinline__ void three_parts(float v, typename Half16<DT>::T* out) {
+__device__ __forceinline__ void four_parts(float v, typename Half16<DT>::T* out) {
     using H16 = Half16<DT>;
-    out[0] = H16::from_f(v);
-    const float r = (v - H16::to_f(out[0])) * 2048.f;
-    out[1] = H16::from_f(r);
-    out[2] = H16::from_f((r - H16::to_f(out[1])) * 2048.f);
+    constexpr float MOST = 65504.f * 0x1p15f;
+    if (DT == OM_DTYPE_F16 && fabsf(v) > MOST) v = copysignf(MOST, v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        out[i] = H16::from_f(v * (1.f / part_unit(i)));
+        v -= H16::to_f(out[i]) * part_unit(i);
+    }
 }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
@@ -865,10 +869,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         for (int i = threadIdx.x; i < XE_BYTES / 16; i += Cf::THREADS) {
             alignas(16) typename Half16<DT>::T v[8];
             const int region = i / 128;   // 0: XE2, 1: XE1, 2: zeros
-            for (int c = 0; c < 8; ++c) {
-                const float unit = c % 3 == 0 ? 1.f : c % 3 == 1 ? 1.f / 2048.f : 1.f / 4194304.f;
-                v[c] = Half16<DT>::from_f(region == 0 && c >= 3 && c < 6 ? 16.f * unit : region == 1 && c < 3 ? p.lse_unit * unit : 0.f);
-            }
+            for (int c = 0; c < 8; ++c) v[c] = Half16<DT>::from_f(region + c / 4 == 1 ? part_unit(c % 4) : 0.f);
             reinterpret_cast<uint4*>(smem + Cf::XE_OFF)[i] = *reinterpret_cast<const uint4*>(v);
         }
         fence_async_smem();
@@ -982,9 +983,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             ds0 = -delta * p.scale;
             if (ok && w == 0 && split == 0) {   // for the KV kernel
                 alignas(16) typename Half16<DT>::T v[8];
-                three_parts<DT>(lse2 * p.lse_part, v);
-                three_parts<DT>(delta * -0.0625f, v + 3);
-                v[6] = v[7] = Half16<DT>::from_f(0.f);
+                four_parts<DT>(row_hi > 0 ? -lse_in * p.inv_scale : 0.f, v);
+                four_parts<DT>(-delta, v + 4);
                 uint4* out = reinterpret_cast<uint4*>(stat_tile(p, b, hx, (r0 + row) / 64) + row % 64 / 8 * 256 + row % 8 * 16);
                 out[0] = *reinterpret_cast<const uint4*>(v);
                 out[8] = make_uint4(0, 0, 0, 0);
@@ -1227,11 +1227,7 @@ static void set_scale(Params* p, float scale) {
     p->scale = scale;
     p->neg = scale < 0.f;
     p->scale2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);
-    int a;
-    frexpf(fabsf(scale), &a);                // |scale| in [2^(a-1), 2^a)
-    a = a < -15 ? -15 : a > 2 ? 2 : a;
-    p->lse_unit = ldexpf(1.f, -a);
-    p->lse_part = 1.f / (p->scale2 * p->lse_unit);
+    p->inv_scale = 1.f / fabsf(scale);
 }
 
 // A tensor map over a [batch, token, head, D] view with boxes of 64 columns x `rows` tokens.
@@ -1411,7 +1407,7 @@ extern "C" int omCudaAttentionBackward(const void* pGradOut, const void* pQ, con
     if (st != OM_OK) return st;
     if (nDtype != OM_DTYPE_BF16 && nDtype != OM_DTYPE_F16) return OM_ERR_UNSUPPORTED;
     if (!(fabsf(fScale) < INFINITY)) return OM_ERR_INVALID;
-    if (fabsf(fScale) < 0x1p-20f) return OM_ERR_UNSUPPORTED;    // lse / |scale| leaves 16-bit range
+    if (fabsf(fScale) < 0x1p-20f) return OM_ERR_UNSUPPORTED;    // log(keys) / |scale| nears the parts' range
     attn::Params p = {};
     if (!pStrides || !attn::view(&p.q, pQ, pStrides, nBatch, nSq, nHeads) ||
         !attn::view(&p.k, pK, pStrides + 3, nBatch, nSk, nKvHeads) ||
