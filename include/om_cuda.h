@@ -652,7 +652,9 @@ int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut, 
                     int nHeadDim, float fScale, int bCausal, int nDtype);
 /* The gradients of that call. The probabilities are recomputed from Q, K and the forward's pLse;
  * pOut is the forward's output. pStrides: 24 element strides, (batch, token, head) of Q, K, V,
- * out, dOut, dQ, dK, dV. dK and dV sum over the query heads that share a key/value head. dQ of
+ * out, dOut, dQ, dK, dV. Probabilities (for dV) and score gradients (for dQ and dK) are rounded to
+ * nDtype for their products, with F16 behind powers of two that keep score gradients of any size in
+ * range; the rest is fp32. dK and dV sum over the query heads that share a key/value head. dQ of
  * queries that see no key or lie past their length, and dK, dV of keys past theirs, are zeros.
  * dQ, dK and dV must not overlap an input. |fScale| below 2^-20 is OM_ERR_UNSUPPORTED (lse enters a
  * product divided by it). With F16, a query's |lse / fScale| and |sum(dOut * out)| enter dK and dV up

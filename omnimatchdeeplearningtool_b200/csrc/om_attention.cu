@@ -35,6 +35,8 @@ struct Params {
     View q, k, v, o, dout, dq, dk, dv;
     float* lse;        // [B, H, Sq]
     uint8_t* stat;     // the backward's workspace: see stat_tile
+    float2* qmax;      // ... and, for fp16, what bounds the score gradients: see range_factor
+    float* vmax;
     const int *qlens, *kvlens;
     int B, H, Hkv, Sq, Sk, D, causal;
     float scale;
@@ -696,8 +698,9 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
 // and dO blocks of every query head that shares them. With X1, X2 the kept tiles and Y1, Y2 the
 // streamed ones, per block:
 //   S = X1 Y1^T, dP = X2 Y2^T                     (the transposes of S and dP for KV)
-//   P = exp(S - lse), dS = scale * P o (dP - delta)
+//   P = exp(S - lse), dS = P o (dP - delta)
 //   dQ += dS Y1                                   KV: dV += P Y2, dK += dS Y1
+// and scale enters dQ and dK in fp32 at the end.
 // The thread of a row of S has the row of P^T or dS that the next product takes as its TMEM
 // operand, so P and dS never leave TMEM and nothing is transposed: Y1 and Y2 serve as K-major
 // operands of the first products and as MN-major operands of the others. dQ and dK, dV are
@@ -756,6 +759,62 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                      smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
+// dS is rounded to the type for its product. fp16 holds it only within 2^-14 .. 2^16 at full precision,
+// and gradients come in any size, so there the kept side's row has a factor 2^a for its dS, taken back
+// at the end: |dS| <= |dO_i| |V_j| + |delta_i| (Cauchy-Schwarz; P is 1 at most), and the factor brings
+// the largest such bound of a row into [2^14, 2^15): no dS overflows, and those down to 2^-28 of the
+// bound are normal numbers. (With the scale in dS and no factor, dO of size 1e-3 over 4096 keys left
+// dQ 2 to 4 % off, and dO of size 1e-5 left nothing of it.) dQ's rows take their own |dO_i| and
+// delta_i, and the largest |V_j| of the head from a launch before (vmax, per 128 keys); dK's rows take
+// their own |V_j|, and from the dQ kernel the largest |dO_i| and |delta_i| of the queries that the
+// CTA streams (qmax, squared and not, per 32 queries). bf16 has fp32's range and needs none of it. In
+// fp16 the launch and the bounds cost 6 to 13 us: 32 x 12 heads of 197 tokens 71 -> 79 us, the ragged
+// causal batch 61 -> 67, 24 heads of 4096 tokens 403 -> 416 (bf16, by the multiply that went: 403 -> 386).
+struct Factor { float f, inverse; };
+__device__ __forceinline__ Factor range_factor(float bound) {
+    if (!(bound >= 0x1p-100f && bound <= 0x1p100f)) return {1.f, 1.f};   // no gradient, or not finite
+    const int e = __float_as_int(bound) >> 23;
+    return {__int_as_float((2 * 127 + 14 - e) << 23), __int_as_float((e - 14) << 23)};
+}
+// the largest of the lanes' values, none of which is negative
+__device__ __forceinline__ float warp_max(float v) { return __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(v))); }
+__device__ __forceinline__ float if_finite(float v) { return v < INFINITY ? v : 0.f; }
+template <int DT>
+__device__ __forceinline__ float squares(const uint4& u) {
+    const auto* v = reinterpret_cast<const typename Half16<DT>::T2*>(&u);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = Half16<DT>::unpack(v[i]);
+        s += f.x * f.x + f.y * f.y;
+    }
+    return s;
+}
+// vmax: the largest sum of squares of a value row of 128 keys, rows that are not finite left out. 8 or
+// 16 lanes a row, one 16-byte load each
+template <int DT>
+__global__ void __launch_bounds__(256) value_norms_kernel(const Params p) {
+    __shared__ float sh[8];
+    pdl_launch_dependents();
+    const int tiles = (p.Sk + 127) / 128, t0 = blockIdx.x % tiles * 128, bh = blockIdx.x / tiles;
+    const int b = bh / p.Hkv, h = bh - b * p.Hkv, end = min(len_of(p.kvlens, b, p.Sk), t0 + 128);
+    const int wide = p.D <= 64 ? 8 : 16, col = threadIdx.x % wide * 8;
+    float most = 0.f;
+#pragma unroll 4
+    for (int r = threadIdx.x / wide; r < 128; r += 256 / wide) {
+        float s = 0.f;
+        if (t0 + r < end && col < p.D) s = squares<DT>(__ldg(reinterpret_cast<const uint4*>(row<DT>(p.v, b, t0 + r, h) + col)));
+        for (int o = wide / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
+        most = fmaxf(most, if_finite(s));
+    }
+    most = warp_max(most);
+    if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; ++i) most = fmaxf(most, sh[i]);
+        p.vmax[blockIdx.x] = most;
+    }
+}
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
 template <int DP>
 struct BwdCfg {
@@ -766,7 +825,7 @@ struct BwdCfg {
     static constexpr int Y_OFF = 2 * TILE;
     static constexpr int STAT = BN / 64 * STAT_TILE;         // YE of a block, per pair of slots
     static constexpr int STAT_OFF = Y_OFF + SLOTS * Y_TILE;
-    static constexpr int XE_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT, WG * 128 * 4);
+    static constexpr int XE_OFF = STAT_OFF + max_of(SLOTS / 2 * STAT, WG * 128 * 8);
     static constexpr int BAR_OFF = XE_OFF + XE_BYTES;
     static constexpr int SMEM = BAR_OFF + 512;
     static constexpr int DP_COL = BN, ACC = 2 * BN, TMEM_COLS = 2 * BN + 2 * DP;
@@ -837,7 +896,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
     }
     // dQ: a thread's part of its row's delta, 8 elements of dO . O at a time, and the row's lse,
     // fetched while the barriers and TMEM are set up
-    float delta_part = 0.f, lse_in = 0.f;
+    constexpr bool F16 = DT == OM_DTYPE_F16;
+    float delta_part = 0.f, grad_part = 0.f, lse_in = 0.f;
     if (!KV && warp < W_LOAD) {
         const int w = warp / 4, r = r0 + (warp % 4) * 32 + lane;
         if (r < ql) {
@@ -862,6 +922,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                         const float2 f = Half16<DT>::unpack(a2[y]), g = Half16<DT>::unpack(b2[y]);
                         delta_part += f.x * g.x + f.y * g.y;
                     }
+                    if (F16) grad_part += squares<DT>(u[x]);
                 }
         }
     }
@@ -964,7 +1025,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
         const uint32_t s_addr = tmem + lanes + w * CW, dp_addr = s_addr + Cf::DP_COL;
         constexpr float LOG2E = 1.4426950408889634f;
         bool ok = true;
-        float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's -lse * log2(e) and -scale * delta
+        float lse2 = 0.f, ds0 = 0.f;          // dQ: the row's -lse * log2(e) and -delta (times its factor)
+        Factor range = {1.f, 1.f};
         int row_lo = 0, row_hi = 0;           // the streamed rows that this row meets
         if (KV) {
             if (r < kl) {
@@ -976,11 +1038,23 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             if (p.causal) row_hi = min(row_hi, r + kl - ql + 1);
             if (row_hi > 0) lse2 = -lse_in * LOG2E;
             stat[tid] = row_hi > 0 ? delta_part : 0.f;
+            if (F16) stat[Cf::WG * 128 + tid] = row_hi > 0 ? grad_part : 0.f;
             warp_arrive(out_ready);               // its first phase: the parts of delta
             ok = warp_wait(out_ready, 0, abort_flag);
-            float delta = 0.f;
-            for (int x = 0; x < Cf::WG; ++x) delta += stat[row + x * 128];
-            ds0 = -delta * p.scale;
+            float delta = 0.f, grad = 0.f;
+            for (int x = 0; x < Cf::WG; ++x) {
+                delta += stat[row + x * 128];
+                if (F16) grad += stat[(Cf::WG + x) * 128 + row];
+            }
+            if (F16) {
+                pdl_wait();                       // vmax
+                const int tiles = (p.Sk + 127) / 128;
+                const float* v = p.vmax + ((long long)b * p.Hkv + hy0) * tiles;
+                float most = 0.f;
+                for (int x = lane; x < tiles; x += 32) most = fmaxf(most, __ldcg(v + x));
+                range = range_factor(sqrtf(grad) * sqrtf(warp_max(most)) + fabsf(delta));
+            }
+            ds0 = -delta * range.f;
             if (ok && w == 0 && split == 0) {   // for the KV kernel
                 alignas(16) typename Half16<DT>::T v[8];
                 four_parts<DT>(row_hi > 0 ? -lse_in * p.inv_scale : 0.f, v);
@@ -988,7 +1062,29 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                 uint4* out = reinterpret_cast<uint4*>(stat_tile(p, b, hx, (r0 + row) / 64) + row % 64 / 8 * 256 + row % 8 * 16);
                 out[0] = *reinterpret_cast<const uint4*>(v);
                 out[8] = make_uint4(0, 0, 0, 0);
+                if (F16) {
+                    const float2 most = {warp_max(if_finite(grad)), warp_max(if_finite(fabsf(delta)))};
+                    if (lane == 0) p.qmax[((long long)b * p.H + hx) * stat_tiles(p.Sq) * 2 + (r0 + row) / 32] = most;
+                }
             }
+        }
+        if (KV && F16 && nblk > 0) {
+            pdl_wait();                           // qmax
+            float2 most = {0.f, 0.f};
+            for (int h = 0; h < rep; ++h) {
+                const float2* q = p.qmax + ((long long)b * p.H + hy0 + h) * stat_tiles(p.Sq) * 2;
+                for (int x = first * BN / 32 + lane; x < (first + per) * BN / 32; x += 32) {
+                    const float2 v = __ldcg(q + x);
+                    most = {fmaxf(most.x, v.x), fmaxf(most.y, v.y)};
+                }
+            }
+            most = {warp_max(most.x), warp_max(most.y)};
+            ok = warp_wait(x_full, 0, abort_flag);
+            float v2 = 0.f;                       // |V_j|^2 from the kept tile, its columns in any order
+#pragma unroll
+            for (int x = 0; x < DP / 8; ++x)
+                v2 += squares<DT>(*reinterpret_cast<const uint4*>(smem + Cf::TILE + x / 8 * PANEL + row * 128 + ((x ^ row) % 8 << 4)));
+            range = range_factor(sqrtf(most.x) * sqrtf(v2) + most.y);
         }
         int y0 = y_start * BN;
         for (int i = 0; ok && i < nblk; ++i) {
@@ -1045,8 +1141,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             float* dp = reinterpret_cast<float*>(dv);
 #pragma unroll
             for (int c = 0; c < CW; c += 2) {
-                const F2 v = {dp[c], dp[c + 1]}, k = {p.scale, p.scale};
-                const F2 e = mul2({pr[c], pr[c + 1]}, KV ? mul2(v, k) : fma2(v, k, {ds0, ds0}));
+                const F2 v = {dp[c], dp[c + 1]}, k = {range.f, range.f};
+                const F2 e = mul2({pr[c], pr[c + 1]}, KV ? (F16 ? mul2(v, k) : v) : F16 ? fma2(v, k, {ds0, ds0}) : add2(v, {ds0, ds0}));
                 dp[c] = e.x;
                 dp[c + 1] = e.y;
             }
@@ -1078,13 +1174,14 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                               ? p.part + ((((KV && w >= HALF ? p.splits : 0) + (long long)split) * bhs + bh) * rows + r) * p.D
                               : nullptr;
             const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w / HALF * DP : 0);
+            const float f = KV && w >= HALF ? 1.f : p.scale * range.inverse;
             for (int c = (KV ? w % HALF : w) * 32; c < p.D; c += (KV ? HALF : Cf::WG) * 32) {
                 uint32_t o[32];
                 if (nblk > 0) {
                     tmem_ld32_issue(acc + c, o);
                     tmem_ld_wait<32>(o);
                 }
-                store_chunk<DT>(o, nblk > 0, 1.f, p.splits > 1, tile, row, part, c, p.D);
+                store_chunk<DT>(o, nblk > 0, f, p.splits > 1, tile, row, part, c, p.D);
             }
             if (p.splits == 1) {
                 fence_async_smem();
@@ -1184,7 +1281,7 @@ static int parts(long long ctas, int blocks, int places, bool causal) {
 // The split of each kernel of a problem and the workspace it takes.
 struct Plan {
     int nt, fwd, dq, dkv;                 // query tiles of a forward CTA; parts
-    long long fwd_bytes, bwd_bytes, dq_at, dkv_at;
+    long long fwd_bytes, bwd_bytes, qmax_at, vmax_at, dq_at, dkv_at;
 };
 static Plan plan(int B, int H, int Hkv, int Sq, int Sk, int D, bool causal) {
     Plan n;
@@ -1195,7 +1292,9 @@ static Plan plan(int B, int H, int Hkv, int Sq, int Sk, int D, bool causal) {
     const int places = D <= 64 ? 296 : 148, bn = D <= 64 ? 64 : 128;
     n.dq = parts(qt * bh, (Sk + bn - 1) / bn, places, causal);
     n.dkv = parts(kt * bhk, (Sq + bn - 1) / bn * (H / Hkv), places, causal);
-    n.dq_at = bh * stat_tiles(Sq) * STAT_TILE;
+    n.qmax_at = bh * stat_tiles(Sq) * STAT_TILE;
+    n.vmax_at = n.qmax_at + bh * stat_tiles(Sq) * 2 * (long long)sizeof(float2);
+    n.dq_at = n.vmax_at + (bhk * kt * 4 + 15) / 16 * 16;
     n.dkv_at = n.dq_at + (n.dq > 1 ? n.dq * bh * Sq * D * 4 : 0);
     n.bwd_bytes = n.dkv_at + (n.dkv > 1 ? 2 * n.dkv * bhk * Sk * D * 4 : 0);
     return n;
@@ -1295,7 +1394,7 @@ static int forward(DeviceCtx* c, Params p, void* workspace) {
 // x1, x2: maps of the kept tiles (128 rows), y1, y2: of the streamed ones (BN rows)
 template <int DP, bool KV, int DT>
 static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2, const CUtensorMap& y1,
-                      const CUtensorMap& y2, const Params& p, bool after_dq = false) {
+                      const CUtensorMap& y2, const Params& p, bool overlap) {
     using Cf = BwdCfg<DP>;
     CUtensorMap o1 = {}, o2 = {};         // dQ, or dK and dV
     if (p.splits == 1) {
@@ -1321,7 +1420,7 @@ static int launch_bwd(DeviceCtx* c, const CUtensorMap& x1, const CUtensorMap& x2
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = at;
-    cfg.numAttrs = KV && after_dq ? 1 : 0;    // it may set up while the dQ kernel ends
+    cfg.numAttrs = overlap ? 1 : 0;           // it may set up while the launch before it ends
     OMB_CHECK(cudaLaunchKernelEx(&cfg, kern, x1, x2, y1, y2, o1, o2, p));
     return after_launch(c);
 }
@@ -1340,10 +1439,20 @@ static int backward(DeviceCtx* c, Params p) {
     }
     const Plan n = plan(p.B, p.H, p.Hkv, p.Sq, p.Sk, p.D, p.causal);
     int st = OM_OK;
+    const bool norms = DT == OM_DTYPE_F16 && p.Sq > 0 && p.Sk > 0;
+    p.qmax = reinterpret_cast<float2*>(p.stat + n.qmax_at);
+    p.vmax = reinterpret_cast<float*>(p.stat + n.vmax_at);
+    if (norms) {
+        const long long blocks = (long long)p.B * p.Hkv * ((p.Sk + 127) / 128);
+        if (blocks > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
+        value_norms_kernel<DT><<<(unsigned)blocks, 256, 0, c->compute>>>(p);
+        st = after_launch(c);
+        if (st != OM_OK) return st;
+    }
     if (p.Sq > 0) {                       // dQ first: it leaves the queries' statistics for dK and dV
         p.splits = n.dq;
         p.part = reinterpret_cast<float*>(p.stat + n.dq_at);
-        st = launch_bwd<DP, false, DT>(c, m[0][0], m[0][3], m[1][1], m[1][2], p);
+        st = launch_bwd<DP, false, DT>(c, m[0][0], m[0][3], m[1][1], m[1][2], p, norms);
         if (st == OM_OK && n.dq > 1) st = join<DT, false>(c, p, p.dq, p.Sq, p.H);
     }
     if (st == OM_OK && p.Sk > 0) {

@@ -88,3 +88,75 @@ def test_attention_one_query_beyond_range_leaves_dv_alone(gpu):
     size = p[0, 0].T @ np.abs(c.do[0, :, 0])
     es = 8 * 2.0 ** -24 * (float(c.scale) * np.sqrt((c.q ** 2).sum(-1).max() * (c.k ** 2).sum(-1).max()) + 8)
     assert (np.abs(dv[0, :, 0] - want) <= (2.0 ** -11 + es + 32 * 2.0 ** -24) * size + 2.0 ** -11 * np.abs(want) + 2.0 ** -24).all()
+
+
+# ---------------------------------------------------------------- score gradients in fp16
+@pytest.mark.parametrize("size", [1.0, 1e-2, 1e-3, 1e-5])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_small_gradients(gpu, size, d, dtype):
+    """Gradients of the size that long training has, over 4096 keys; the other operand is large enough
+    for results in the type's normal range, so that the score gradients' rounding shows."""
+    big = min(3000.0, 30 / size)
+    c = _Case(1, 1, 1, 140, 4096, d, dtype)
+    _set(c, k=c.k * big, q=c.q / big, do=c.do * size).check()
+    c = _Case(1, 2, 1, 4096, 70, d, dtype)
+    _set(c, q=c.q * big, k=c.k / big, do=c.do * size).check()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -19, 2.0 ** -16, -2.0 ** -12])
+def test_attention_small_scale(gpu, scale):
+    c = _Case(1, 2, 1, 197, 197, 64, F16, scale=scale)
+    _set(c, k=c.k * 2000).check()
+    c = _Case(1, 2, 1, 197, 197, 64, F16, scale=scale)
+    _set(c, q=c.q * 2000).check()
+
+
+@pytest.mark.parametrize("scale", [1.0, 3.0, 5.5])
+def test_attention_large_scale(gpu, scale):
+    c = _Case(1, 2, 1, 150, 197, 64, F16, scale=scale)
+    _set(c, q=0.2 * c.q, k=0.2 * c.k).check()
+
+
+def test_attention_gradients_of_unlike_sizes(gpu):
+    """Queries' gradients from 1e-4 to 1e4 side by side: each row of dQ at its own precision; heads and
+    batch entries whose gradients are zero or whose queries are not in use among them."""
+    c = _Case(2, 4, 2, 300, 500, 64, F16, qlens=[300, 129], klens=[500, 260])
+    size = 10.0 ** np.linspace(-4, 4, 300)[None, :, None, None]
+    do = c.do * size
+    do[:, :, 1], do[1, :40, 2], do[0, 250:, 3] = 0, 0, 0
+    _set(c, k=c.k / 8, q=c.q, v=c.v, do=do)
+    o, lse, p, es = c.check_forward()
+    dq, dk, dv = c.backward(rounded(o, F16), lse)
+    assert np.isfinite(dq).all() and np.isfinite(dk).all() and np.isfinite(dv).all()
+    assert (dq[:, :, 1] == 0).all() and (dq[1, 129:] == 0).all() and (dk[1, 260:] == 0).all()
+    u = 2.0 ** -11
+    for i in range(2):
+        m = ref.visible(300, 500, c.ql[i], c.kl[i], False)
+        for j in range(4):
+            g, terms, sizes = ref.attention_backward(c.q[i, :, j], c.k[i, :, j // 2], c.v[i, :, j // 2],
+                                                     rounded(o, F16)[i, :, j], c.do[i, :, j], p[i, j], float(c.scale), m)
+            tol = u * terms[0] + (es + 32 * 2.0 ** -24) * sizes[0] + u * np.abs(g[0]) + 2.0 ** -24
+            assert (np.abs(dq[i, :, j] - g[0]) <= tol).all()
+
+
+@pytest.mark.parametrize("grad,qsize,ksize", [("dq", 100, 0.01), ("dk", 0.01, 100)])
+def test_attention_large_gradients_stay_finite(gpu, grad, qsize, ksize):
+    """Score gradients far beyond the type's range (sharp scores, sum(dO v) of 1e6) whose products with
+    the small operand lie in it."""
+    c = _Case(1, 2, 1, 197, 260, 64, F16, scale=1.0)
+    _set(c, q=qsize * c.q, k=ksize * c.k, v=40 * c.v, do=5e3 * np.tanh(c.do))
+    o, lse, p, es = c.check_forward()
+    o = rounded(o, F16)
+    got = dict(zip(("dq", "dk", "dv"), c.backward(o, lse)))[grad]
+    want, tol, top, u = np.zeros_like(got), np.zeros_like(got), 0, 2.0 ** -11
+    for j in range(2):
+        g, terms, sizes = ref.attention_backward(c.q[0, :, j], c.k[0, :, 0], c.v[0, :, 0], o[0, :, j], c.do[0, :, j],
+                                                 p[0, j], float(c.scale), np.ones((197, 260), bool))
+        n, at = (0, j) if grad == "dq" else (1, 0)
+        want[0, :, at] += g[n]
+        tol[0, :, at] += u * terms[n] + (es + 32 * 2.0 ** -24) * sizes[n]
+        delta = (c.do[0, :, j] * o[0, :, j]).sum(1, keepdims=True)
+        top = max(top, np.abs(p[0, j] * (c.do[0, :, j] @ c.v[0, :, 0].T - delta)).max())
+    assert top > 2e5 and (np.abs(want) + tol).max() < 65504
+    assert (np.abs(got - want) <= tol + u * np.abs(want) + 2.0 ** -24).all()
