@@ -187,11 +187,11 @@ constexpr int PANEL = 128 * 128;
 // panels of 64 columns as far apart as they are long.
 __device__ __forceinline__ uint32_t desc_k(uint32_t tile) { return (tile >> 4) | (1u << 16); }
 __device__ __forceinline__ uint32_t desc_mn(uint32_t tile, int panel) { return (tile >> 4) | ((uint32_t)(panel >> 4) << 16); }
-// D = X Y^T over the head dimension, ks steps of 16 (X: a tile of 128 rows, Y: of ROWS)
-template <int DP, int ROWS>
+// D (+)= X Y^T over the head dimension, ks steps of 16 (X: a tile of 128 rows, Y: of ROWS)
+template <int DP, int ROWS, bool ACC = false>
 __device__ __forceinline__ void product_k(uint32_t leader, uint32_t d_tmem, uint32_t x, uint32_t y, uint32_t idesc, int ks) {
     const uint32_t a = desc_k(x), b = desc_k(y);
-    mma_ss<false>(leader, d_tmem, a, b, idesc);
+    mma_ss<ACC>(leader, d_tmem, a, b, idesc);
 #pragma unroll
     for (int k = 1; k < DP / 16; ++k)
         if (k < ks)
@@ -734,23 +734,26 @@ __device__ __forceinline__ uint8_t* stat_tile(const Params& p, int b, int h, int
 // low descriptor word of an unswizzled operand; the high word: rows of cores `rows` bytes apart
 __device__ __forceinline__ uint32_t desc_plain(uint32_t at, uint32_t cols) { return (at >> 4) | (cols >> 4 << 16); }
 __host__ __device__ constexpr uint32_t plain_hi(uint32_t rows) { return (rows >> 4) | (1u << 14); }
-// D += XE YE^T
+// D = XE YE^T
 __device__ __forceinline__ void product_plain(uint32_t leader, uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .b64 a, b;\n\t.reg .pred p, q;\n\t"
-        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %5};\n\tsetp.eq.b32 p, 0, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "mov.b64 a, {%1, %4};\n\tmov.b64 b, {%2, %5};\n\tsetp.ne.b32 p, 0, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n" ::"r"(d_tmem),
         "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(plain_hi(128)), "r"(plain_hi(256)), "r"(leader));
 }
-// the four parts of a value and their units: each part is what the ones before it left, rounded
+// the four parts of a value (v + more, whose sum is not rounded first) and their units: each part is
+// what the ones before it left, rounded
 __device__ __forceinline__ float part_unit(int i) { return i == 0 ? 0x1p15f : i == 1 ? 0x1p4f : i == 2 ? 0x1p-7f : 0x1p-18f; }
 template <int DT>
-__device__ __forceinline__ void four_parts(float v, typename Half16<DT>::T* out) {
+__device__ __forceinline__ void four_parts(float v, float more, typename Half16<DT>::T* out) {
     using H16 = Half16<DT>;
     constexpr float MOST = 65504.f * 0x1p15f;
     if (DT == OM_DTYPE_F16 && fabsf(v) > MOST) v = copysignf(MOST, v);
+    out[0] = H16::from_f((v + more) * (1.f / part_unit(0)));
+    v = (v - H16::to_f(out[0]) * part_unit(0)) + more;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 1; i < 4; ++i) {
         out[i] = H16::from_f(v * (1.f / part_unit(i)));
         v -= H16::to_f(out[i]) * part_unit(i);
     }
@@ -771,6 +774,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // fp16 the launch and the bounds cost 6 to 13 us: 32 x 12 heads of 197 tokens 71 -> 79 us, the ragged
 // causal batch 61 -> 67, 24 heads of 4096 tokens 403 -> 416 (bf16, by the multiply that went: 403 -> 386).
 struct Factor { float f, inverse; };
+// P for dV is 1 at most, and in fp16 below 2^-14 no normal number (1e-7 came out up to 30 % off, and
+// with it the dV of a key that every query gives so little): there the dK/dV kernel works with 2^14 P,
+// by 14 more in the exponent that its parts of -lse give (by a sum per score: 24 heads of 4096 tokens
+// 417 -> 423 us).
+template <int DT> constexpr int P_SHIFT = DT == OM_DTYPE_F16 ? 14 : 0;
 __device__ __forceinline__ Factor range_factor(float bound) {
     if (!(bound >= 0x1p-100f && bound <= 0x1p100f)) return {1.f, 1.f};   // no gradient, or not finite
     const int e = __float_as_int(bound) >> 23;
@@ -979,10 +987,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             auto wait_y = [&](int i) { return warp_wait(full + i % Cf::SLOTS, (i / Cf::SLOTS) & 1, abort_flag); };
             auto score = [&](uint32_t d, uint32_t x, int i, uint32_t id, uint64_t* bar) {
                 tc_fence_after();
-                product_k<DP, BN>(leader, tmem + d, x, tile(i), id, ks);
+                // first the statistics, so that the sum over the head dimension runs towards the small
+                // difference and not the other way (the sums drop bits below their largest term's)
                 if (KV)                   // d == 0: XE1, else XE2
                     product_plain(leader, tmem + d, desc_plain(xe + (d ? 0 : XE_REGION), d ? 2 * XE_REGION : XE_REGION),
                                   desc_plain(ye + i / 2 % (Cf::SLOTS / 2) * Cf::STAT, 128), id_dp);
+                product_k<DP, BN, KV>(leader, tmem + d, x, tile(i), id, ks);
                 commit(leader, bar);
             };
             bool ok = warp_wait(x_full, 0, abort_flag) && wait_y(0);
@@ -1057,8 +1067,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             ds0 = -delta * range.f;
             if (ok && w == 0 && split == 0) {   // for the KV kernel
                 alignas(16) typename Half16<DT>::T v[8];
-                four_parts<DT>(row_hi > 0 ? -lse_in * p.inv_scale : 0.f, v);
-                four_parts<DT>(-delta, v + 4);
+                four_parts<DT>(row_hi > 0 ? -lse_in * p.inv_scale : 0.f, P_SHIFT<DT> / p.scale2, v);
+                four_parts<DT>(-delta, 0.f, v + 4);
                 uint4* out = reinterpret_cast<uint4*>(stat_tile(p, b, hx, (r0 + row) / 64) + row % 64 / 8 * 256 + row % 8 * 16);
                 out[0] = *reinterpret_cast<const uint4*>(v);
                 out[8] = make_uint4(0, 0, 0, 0);
@@ -1085,6 +1095,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
             for (int x = 0; x < DP / 8; ++x)
                 v2 += squares<DT>(*reinterpret_cast<const uint4*>(smem + Cf::TILE + x / 8 * PANEL + row * 128 + ((x ^ row) % 8 << 4)));
             range = range_factor(sqrtf(most.x) * sqrtf(v2) + most.y);
+            range.f *= 1.f / (1 << P_SHIFT<DT>);
         }
         int y0 = y_start * BN;
         for (int i = 0; ok && i < nblk; ++i) {
@@ -1174,7 +1185,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap mx1, const __grid_constant__
                               ? p.part + ((((KV && w >= HALF ? p.splits : 0) + (long long)split) * bhs + bh) * rows + r) * p.D
                               : nullptr;
             const uint32_t acc = tmem + lanes + Cf::ACC + (KV ? w / HALF * DP : 0);
-            const float f = KV && w >= HALF ? 1.f : p.scale * range.inverse;
+            const float f = KV && w >= HALF ? 1.f / (1 << P_SHIFT<DT>) : p.scale * range.inverse;
             for (int c = (KV ? w % HALF : w) * 32; c < p.D; c += (KV ? HALF : Cf::WG) * 32) {
                 uint32_t o[32];
                 if (nblk > 0) {

@@ -160,3 +160,18 @@ def test_attention_large_gradients_stay_finite(gpu, grad, qsize, ksize):
         top = max(top, np.abs(p[0, j] * (c.do[0, :, j] @ c.v[0, :, 0].T - delta)).max())
     assert top > 2e5 and (np.abs(want) + tol).max() < 65504
     assert (np.abs(got - want) <= tol + u * np.abs(want) + 2.0 ** -24).all()
+
+
+# ---------------------------------------------------------------- probabilities in fp16
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_rarely_seen_keys(gpu, d, dtype):
+    """Keys that every query gives a probability of about 1e-7: their dV at the same relative precision."""
+    c = _Case(1, 2, 1, 300, 400, d, dtype)
+    q, k = c.q.copy(), c.k.copy()
+    q[..., 0] = 8
+    k[:, ::2, :, 0] = -10 / (8 * float(c.scale))
+    _set(c, q=q, k=k, do=500 * c.do)
+    _, _, p = c.reference()
+    assert p[0, 0][:, ::2].max() < 1e-5
+    c.check()
