@@ -16,6 +16,8 @@
 // 1979), so a mean far from zero costs no precision; every merge has a fixed order.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "om_common.cuh"
 #include "om_f2.cuh"
 
@@ -291,8 +293,9 @@ __device__ void block_stats(const Params& p, const Stats<GV>& st, float count, f
     __syncthreads();
 }
 
-// z = (x - mean) scale + shift of a thread's 8 channels; with 16-bit inputs the mean is folded
-// into the shift (its rounding, 2^-24 of mean * scale, is far below the output's). Padding: 0.
+// z = (x - mean) scale + shift of a thread's 8 channels; with 16-bit inputs the mean is folded into
+// the shift (its rounding, 2^-24 of mean * scale, is that of the mean itself). Padding: 0. Not for ReLU
+// and ReLU6, whose backward has to see the sign that the forward saw: see Normal.
 template <int DT>
 struct Affine {
     F2 minus_mean[DT == OM_DTYPE_F32 ? 4 : 1], scale[4], shift[4];
@@ -328,6 +331,74 @@ __device__ __forceinline__ Vec<DT> apply(const Vec<DT>& v, const Affine<DT>& f, 
                                  f.scale[i], f.shift[i]));
     return pack<DT>(x);
 }
+
+// The coefficients of z = ((x - mean) rstd) gamma + beta of a thread's 8 channels; statistics once per
+// entry of GV (channel i belongs to entry i * GV / 8).
+template <int GV>
+struct Normal {
+    float minus_mean[GV], rstd[GV];
+    F2 gamma[4], beta[4];
+};
+// the pair i of a vector from values per entry
+template <int GV>
+__device__ __forceinline__ F2 pair_of(const float (&v)[GV], int i) {
+    return {v[2 * i * GV / 8], v[(2 * i + 1) * GV / 8]};
+}
+template <int GV, class MeanOf, class RstdOf>
+__device__ __forceinline__ void normal_of(const Params& p, const Part& t, Normal<GV>& f, MeanOf mean_of, RstdOf rstd_of) {
+    int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const bool in = i < t.nval;
+        if (i % (8 / GV) == 0) {
+            f.minus_mean[i * GV / 8] = in ? -mean_of(g) : 0.f;
+            f.rstd[i * GV / 8] = in ? rstd_of(g) : 0.f;
+        }
+        half_of(f.gamma, i) = !in ? 0.f : p.gamma ? p.gamma[t.c0 + i] : 1.f;
+        half_of(f.beta, i) = in && p.beta ? p.beta[t.c0 + i] : 0.f;
+        if (--left == 0) { ++g; left = p.cpg; }
+    }
+}
+template <int ACT> constexpr bool HAS_KINK = ACT == OM_ACT_RELU || ACT == OM_ACT_RELU6;
+template <int GV>
+__device__ __forceinline__ F2 normalised(F2 x, const Normal<GV>& f, int i) {
+    return mul2(add2(x, pair_of<GV>(f.minus_mean, i)), pair_of<GV>(f.rstd, i));
+}
+// z of the pair i. Where its sign decides, product and sum are rounded apart, as the formula reads, in
+// both passes: fused (as the paired instructions can be), a z that rounds to 0 came out next to 0 and
+// let its gradient through; rounded otherwise in the forward than in the backward, constant maps gave
+// outputs above 0 that no gradient came back through
+template <int ACT, int GV>
+__device__ __forceinline__ F2 pre_activation(F2 xh, const Normal<GV>& f, int i) {
+    if (!HAS_KINK<ACT>) return fma2(xh, f.gamma[i], f.beta[i]);
+    return {__fadd_rn(__fmul_rn(xh.x, f.gamma[i].x), f.beta[i].x), __fadd_rn(__fmul_rn(xh.y, f.gamma[i].y), f.beta[i].y)};
+}
+template <int DT, int ACT, int GV>
+__device__ __forceinline__ Vec<DT> apply(const Vec<DT>& v, const Normal<GV>& f, int nval) {
+    F2 x[4];
+    unpack<DT>(v, x);
+    cut(x, nval);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = act_fwd<ACT>(pre_activation<ACT, GV>(normalised<GV>(x[i], f, i), f, i));
+    return pack<DT>(x);
+}
+// the forward's coefficients and what it does with them
+template <int DT, int ACT, int GV> struct Forward {
+    Affine<DT> f;
+    template <class M, class R> __device__ __forceinline__ Forward(const Params& p, const Part& t, M mean_of, R rstd_of) {
+        affine_of<DT>(p, t, f, mean_of, rstd_of);
+    }
+    __device__ __forceinline__ Vec<DT> operator()(const Vec<DT>& v, int nval) const { return apply<DT, ACT>(v, f, nval); }
+};
+template <int DT, int ACT, int GV> struct ForwardKink {
+    Normal<GV> f;
+    template <class M, class R> __device__ __forceinline__ ForwardKink(const Params& p, const Part& t, M mean_of, R rstd_of) {
+        normal_of<GV>(p, t, f, mean_of, rstd_of);
+    }
+    __device__ __forceinline__ Vec<DT> operator()(const Vec<DT>& v, int nval) const { return apply<DT, ACT, GV>(v, f, nval); }
+};
+template <int DT, int ACT, int GV>
+using ForwardOf = std::conditional_t<HAS_KINK<ACT>, ForwardKink<DT, ACT, GV>, Forward<DT, ACT, GV>>;
 
 // ---------------------------------------------------------------- one launch, unit in a cluster
 // GV: entries of a vector whose statistics are kept apart: 1 where a vector lies within a group
@@ -419,42 +490,19 @@ __global__ void __launch_bounds__(T, 4) gn_fwd_unit_kernel(const Params p) {
     }
     // also: no CTA of the cluster leaves while another reads its sums
     if (p.cluster > 1) cl.sync(); else __syncthreads();
-    Affine<DT> f;
-    affine_of<DT>(p, t, f, [&](int g) { return total[2 * (g - g_lo)]; }, [&](int g) { return total[2 * (g - g_lo) + 1]; });
+    const ForwardOf<DT, ACT, GV> f(p, t, [&](int g) { return total[2 * (g - g_lo)]; }, [&](int g) { return total[2 * (g - g_lo) + 1]; });
     long long e = at(p, t, t.first);
-    for (int s = 0; s < mine_rows; ++s, e += step) store<DT>(p.out, e, apply<DT, ACT>(own<DT>(sm, s), f, t.nval));
+    for (int s = 0; s < mine_rows; ++s, e += step) store<DT>(p.out, e, f(own<DT>(sm, s), t.nval));
 }
 
-// The backward's coefficients of a thread's 8 channels; statistics once per entry of GV (channel
-// i belongs to entry i * GV / 8).
 template <int GV>
-struct BwdAffine {
-    float minus_mean[GV], rstd[GV];
-    F2 gamma[4], beta[4];
-};
-// the pair i of a vector from values per entry
-template <int GV>
-__device__ __forceinline__ F2 pair_of(const float (&v)[GV], int i) {
-    return {v[2 * i * GV / 8], v[(2 * i + 1) * GV / 8]};
-}
-template <int GV>
-__device__ __forceinline__ void bwd_affine_of(const Params& p, const Part& t, BwdAffine<GV>& f) {
-    int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const bool in = i < t.nval;
-        if (i % (8 / GV) == 0) {
-            f.minus_mean[i * GV / 8] = in ? -p.mean[(long long)t.n * p.G + g] : 0.f;
-            f.rstd[i * GV / 8] = in ? p.rstd[(long long)t.n * p.G + g] : 0.f;
-        }
-        half_of(f.gamma, i) = !in ? 0.f : p.gamma ? p.gamma[t.c0 + i] : 1.f;
-        half_of(f.beta, i) = in && p.beta ? p.beta[t.c0 + i] : 0.f;
-        if (--left == 0) { ++g; left = p.cpg; }
-    }
+__device__ __forceinline__ void saved_normal_of(const Params& p, const Part& t, Normal<GV>& f) {
+    const long long at = (long long)t.n * p.G;
+    normal_of<GV>(p, t, f, [&](int g) { return p.mean[at + g]; }, [&](int g) { return p.rstd[at + g]; });
 }
 // minus rstd times the means of t and t xh, from pairs of means per group starting at group g0
 template <int GV>
-__device__ __forceinline__ void bwd_means_of(const Params& p, const Part& t, const BwdAffine<GV>& f, const float* pairs,
+__device__ __forceinline__ void bwd_means_of(const Params& p, const Part& t, const Normal<GV>& f, const float* pairs,
                                              int g0, float (&m1)[GV], float (&m2)[GV]) {
     int g = t.c0 / p.cpg, left = p.cpg - (t.c0 - g * p.cpg);
 #pragma unroll
@@ -468,7 +516,7 @@ __device__ __forceinline__ void bwd_means_of(const Params& p, const Part& t, con
 }
 // dz and xh of 8 channels of one pixel (0 for padding, whatever it holds)
 template <int DT, int ACT, int GV>
-__device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy, const BwdAffine<GV>& f, int nval,
+__device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy, const Normal<GV>& f, int nval,
                                           F2 (&dz)[4], F2 (&xh)[4]) {
     unpack<DT>(vx, xh);
     unpack<DT>(vdy, dz);
@@ -476,14 +524,8 @@ __device__ __forceinline__ void bwd_terms(const Vec<DT>& vx, const Vec<DT>& vdy,
     cut(dz, nval);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        xh[i] = mul2(add2(xh[i], pair_of<GV>(f.minus_mean, i)), pair_of<GV>(f.rstd, i));
-        // Where z's sign decides, product and sum are rounded apart, as the formula reads: fused (as the
-        // paired instructions can be), a z that rounds to 0 came out next to 0 and let its gradient through
-        const F2 z = ACT == OM_ACT_RELU || ACT == OM_ACT_RELU6
-                         ? F2{__fadd_rn(__fmul_rn(xh[i].x, f.gamma[i].x), f.beta[i].x),
-                              __fadd_rn(__fmul_rn(xh[i].y, f.gamma[i].y), f.beta[i].y)}
-                         : fma2(xh[i], f.gamma[i], f.beta[i]);
-        dz[i] = act_bwd<ACT>(dz[i], z);
+        xh[i] = normalised<GV>(xh[i], f, i);
+        dz[i] = act_bwd<ACT>(dz[i], pre_activation<ACT, GV>(xh[i], f, i));
     }
 }
 // the sums that a thread keeps of them: dz, and dz xh
@@ -500,7 +542,7 @@ __device__ __forceinline__ void flat(const F2 (&v)[4], float (&f)[8]) {
 }
 // dx = rstd (gamma dz - mean(t) - xh mean(t xh)); m1 and m2: minus the means, with their rstd
 template <int DT, int GV>
-__device__ __forceinline__ Vec<DT> bwd_out(const F2 (&dz)[4], const F2 (&xh)[4], const BwdAffine<GV>& f,
+__device__ __forceinline__ Vec<DT> bwd_out(const F2 (&dz)[4], const F2 (&xh)[4], const Normal<GV>& f,
                                            const float (&m1)[GV], const float (&m2)[GV]) {
     F2 d[4];
 #pragma unroll
@@ -533,8 +575,8 @@ __global__ void __launch_bounds__(T, GV == 8 ? 2 : 3) gn_bwd_unit_kernel(const P
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    BwdAffine<GV> f;
-    bwd_affine_of<GV>(p, t, f);
+    Normal<GV> f;
+    saved_normal_of<GV>(p, t, f);
     F2 a2[4] = {}, b2[4] = {};
     auto take = [&](int s, int end) {
         for (; s < end; ++s) {
@@ -613,8 +655,8 @@ __global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_partial_kernel(const Pa
     float* sums = red + T * 16;
     const Part t = part_of(p, blockIdx.z, blockIdx.y, blockIdx.x);
     if constexpr (BWD) {
-        BwdAffine<GV> f;
-        bwd_affine_of<GV>(p, t, f);
+        Normal<GV> f;
+        saved_normal_of<GV>(p, t, f);
         F2 a2[4] = {}, b2[4] = {};
 #pragma unroll 2
         for (int r = t.first; r < t.end; r += t.step) {
@@ -730,8 +772,8 @@ __global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_apply_kernel(const Para
     const Part t = part_of(p, gridDim.z - 1 - blockIdx.z, gridDim.y - 1 - blockIdx.y, gridDim.x - 1 - blockIdx.x);
     const float* s = stat + 2 * (long long)t.n * p.G;
     if constexpr (BWD) {
-        BwdAffine<GV> f;
-        bwd_affine_of<GV>(p, t, f);
+        Normal<GV> f;
+        saved_normal_of<GV>(p, t, f);
         float m1[GV], m2[GV];
         bwd_means_of<GV>(p, t, f, s, 0, m1, m2);
 #pragma unroll 2
@@ -741,11 +783,10 @@ __global__ void __launch_bounds__(T, GV == 8 ? 3 : 4) gn_apply_kernel(const Para
             store<DT>(p.out, at(p, t, r), bwd_out<DT, GV>(dz, xh, f, m1, m2));
         }
     } else {
-        Affine<DT> f;
-        affine_of<DT>(p, t, f, [&](int g) { return s[2 * g]; }, [&](int g) { return s[2 * g + 1]; });
+        const ForwardOf<DT, ACT, GV> f(p, t, [&](int g) { return s[2 * g]; }, [&](int g) { return s[2 * g + 1]; });
 #pragma unroll 4
         for (int r = t.first; r < t.end; r += t.step)
-            store<DT>(p.out, at(p, t, r), apply<DT, ACT>(load<DT>(p.x, at(p, t, r)), f, t.nval));
+            store<DT>(p.out, at(p, t, r), f(load<DT>(p.x, at(p, t, r)), t.nval));
     }
 }
 

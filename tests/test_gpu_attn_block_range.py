@@ -175,3 +175,46 @@ def test_attention_rarely_seen_keys(gpu, d, dtype):
     _, _, p = c.reference()
     assert p[0, 0][:, ::2].max() < 1e-5
     c.check()
+
+
+# ---------------------------------------------------------------- GroupNorm's two passes at the kink
+@pytest.mark.parametrize("shape", [(1, 49, 64, 64, 8), (2, 300, 48, 48, 12), (3, 130, 15, 16, 3), (1, 30011, 64, 64, 8),
+                                   (1, 30011, 32, 32, 8), (2, 9, 40, 40, 4)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_group_norm_passes_agree_at_the_kink(gpu, shape, dtype):
+    """The backward lets a gradient through where the forward's output is above 0, and nowhere else:
+    on constant maps (every pre-activation within rounding of 0), and where a map's values meet the
+    kink. dY is 1, so the gradient of beta counts the elements that let it through."""
+    from omnimatchdeeplearningtool_b200._lib import call
+    n, hw, c, cs, g = shape
+    elem, cpg = 4 if dtype == F32 else 2, c // g
+    rng = np.random.Generator(np.random.PCG64(sum(shape) + dtype))
+    for trial in range(6):
+        if trial % 2 == 0:                  # constant maps
+            x = np.repeat(rng.choice([-1, 1], (n, 1, g)) * 10.0 ** rng.uniform(0, 2, (n, 1, g)), cpg, 2) * np.ones((1, hw, 1))
+            beta = np.zeros(c)
+        elif dtype == F16:                  # (an output below 2^-25 would be 0 in f16)
+            continue
+        else:                               # a few values a map; beta puts one of them on the kink
+            x = rng.integers(-3, 4, (n, hw, c)) * 0.37 + rng.standard_normal((1, 1, c))
+            x = rounded(x, dtype)
+            _, mean, rstd, _, xh = ref.group_norm(x, 1.0, 0.0, g, 1e-5, 0)
+            beta = None
+        x = rounded(x, dtype)
+        gamma = rounded(rng.choice([-1, 1], c) * rng.uniform(0.5, 2, c), F32)
+        if beta is None:
+            beta = rounded(-xh[0, 0] * gamma, F32)
+        full = np.zeros((n, hw, cs))
+        full[..., :c] = x
+        xd, gd, bd = _dev(full, dtype), _dev(gamma.astype(np.float32)), _dev(beta.astype(np.float32))
+        y, m, r = _new(n * hw * cs * elem), _new(n * g * 4), _new(n * g * 4)
+        dy = _dev(np.ones((n, hw, cs)), dtype)
+        dx, dg, db = _new(n * hw * cs * elem), _new(c * 4), _new(c * 4)
+        for kind in (1, 2) if dtype == F32 else (1,):
+            call("omCudaGroupNormActNhwc", xd.ptr, y.ptr, gd.ptr, bd.ptr, m.ptr, r.ptr, _gn_ws(n, hw, c, cs, g, dtype, 0).ptr,
+                 n, hw, c, cs, g, 1e-5, kind, dtype)
+            call("omCudaGroupNormActNhwcBackward", dy.ptr, xd.ptr, m.ptr, r.ptr, gd.ptr, bd.ptr, dx.ptr, dg.ptr, db.ptr,
+                 _gn_ws(n, hw, c, cs, g, dtype, 1).ptr, n, hw, c, cs, g, kind, dtype)
+            out = _get(y, (n, hw, cs), dtype)[..., :c]
+            through = (out > 0) & ((kind == 1) | (out < 6))
+            assert (db.to_numpy((c,)) == through.sum((0, 1))).all(), (trial, kind)
