@@ -643,7 +643,8 @@ long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int nKvHeads, in
  * [0, nSk]); what tokens past them hold is not used, NaN and infinities included. bCausal: query i
  * sees keys j <= i + kvLen - qLen. A query that sees no key, or lies past its length, gets zeros.
  * pLse [nBatch, nHeads, nSq] fp32 (NULL when no backward follows): log(sum exp(score)) of each
- * query, minus infinity where it sees no key. nDtype BF16 or F16, nHeadDim a multiple of 8 up to
+ * query, minus infinity where it sees no key, NaN (as its output) where a score is NaN or plus
+ * infinity. nDtype BF16 or F16, nHeadDim a multiple of 8 up to
  * 128 (else OM_ERR_UNSUPPORTED); scores, sums and accumulators in fp32, probabilities rounded to
  * nDtype for their product with V. */
 int omCudaAttention(const void* pQ, const void* pK, const void* pV, void* pOut, float* pLse,

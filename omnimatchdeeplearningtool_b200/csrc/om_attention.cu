@@ -632,7 +632,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             asm volatile("" : "+r"(again));
             const FwdPlace w = fwd_place<NT>(p, again);
             const int i = w.q0 + t * 128 + row;
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+            const float inv = l == 0.f ? 0.f : 1.f / l;    // 0: no key seen; NaN stays NaN, also in lse
             const long long rows = (long long)p.B * p.H * p.Sq, to = ((long long)w.b * p.H + w.h) * p.Sq + i;
             float* part = i < p.Sq && p.splits > 1 ? p.part + (w.split * rows + to) * p.D : nullptr;
             for (int c = 0; c < p.D; c += 32) {
@@ -649,7 +649,7 @@ attn_fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ 
             }
             if (i < p.Sq) {
                 // l is relative to the rounded product, as `sub` had it: fused with the sum, it would not be
-                const float lse2 = l > 0.f ? __fadd_rn(__fmul_rn(m, p.scale2), log2f(l)) : -INFINITY;
+                const float lse2 = l == 0.f ? -INFINITY : __fadd_rn(__fmul_rn(m, p.scale2), log2f(l));
                 if (p.splits > 1)
                     p.part_lse[w.split * rows + to] = lse2;
                 else if (p.lse)
@@ -1259,11 +1259,11 @@ __global__ void __launch_bounds__(128) join_kernel(const Params p, const View ou
         acc.w += __shfl_xor_sync(~0u, acc.w, o);
         if (LSE) total += __shfl_xor_sync(~0u, total, o);
     }
-    const float f = !LSE ? 1.f : total > 0.f ? 1.f / total : 0.f;
+    const float f = !LSE ? 1.f : total == 0.f ? 0.f : 1.f / total;
     if (lane < cols)
         *reinterpret_cast<uint2*>(row_out<DT>(out, b, t, h) + lane * 4) =
             make_uint2(pack16<DT>(acc.x * f, acc.y * f), pack16<DT>(acc.z * f, acc.w * f));
-    if (LSE && lane == 0 && p.lse) p.lse[row] = total > 0.f ? (top + log2f(total)) * LN2 : -INFINITY;
+    if (LSE && lane == 0 && p.lse) p.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * LN2;
 }
 template <int DT, bool LSE>
 static int join(DeviceCtx* c, const Params& p, const View& out, int T, int H, const View* second = nullptr) {

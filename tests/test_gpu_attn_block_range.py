@@ -218,3 +218,28 @@ def test_group_norm_passes_agree_at_the_kink(gpu, shape, dtype):
             out = _get(y, (n, hw, cs), dtype)[..., :c]
             through = (out > 0) & ((kind == 1) | (out < 6))
             assert (db.to_numpy((c,)) == through.sum((0, 1))).all(), (trial, kind)
+
+
+# ---------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("dims", [(1, 2, 1, 5, 4096, 64), (1, 2, 2, 300, 200, 64), (2, 2, 1, 150, 300, 128)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attention_nan_scores_are_not_an_empty_row(gpu, dims, dtype):
+    """A query with a NaN has NaN as its output and its lse (minus infinity says that a query sees no
+    key); a NaN in one key reaches every query that sees it. Other queries are as without it."""
+    b, h, hkv, sq, sk, d = dims
+    c = _Case(*dims, dtype)
+    want, wl = c.forward()
+    q = c.q.copy()
+    q[0, 1, 0, 3] = np.nan
+    c.q, c.dq_ = q, c._put(q)
+    got, gl = c.forward()
+    hit = np.zeros((b, sq, h), bool)
+    hit[0, 1, 0] = True
+    assert np.isnan(got[hit]).all() and np.isnan(gl.transpose(0, 2, 1)[hit]).all()
+    assert (got[~hit] == want[~hit]).all() and (gl.transpose(0, 2, 1)[~hit] == wl.transpose(0, 2, 1)[~hit]).all()
+    c = _Case(*dims, dtype)
+    c.k[0, sk // 2, 0, 2] = np.nan
+    c.dk_ = c._put(c.k)
+    got, gl = c.forward()
+    assert np.isnan(got[0, :, :h // hkv]).all() and np.isnan(gl[0, :h // hkv]).all()
+    assert (got[1:] == want[1:]).all() and (gl[1:] == wl[1:]).all()
