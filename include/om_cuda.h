@@ -623,11 +623,19 @@ int omCudaGroupNormActNhwcBackward(const void* pGradOut, const void* pIn, const 
  * Philox4x32-10 (Salmon, Moraes, Dror, Shaw, 2011) at counter (i / 8, nOffset) and key nSeed,
  * each 64 bits, low word first. No mask is stored: the backward is the same call on dY with the
  * same nSeed and nOffset and no residual (the residual's gradient is dY itself). Give every
- * call of a training run its own nOffset. p in [0, 1]; a dropped NaN or infinity gives 0. pOut
- * may be pIn or pResidual. */
+ * call of a training run its own nOffset (or every layer its own nSeed, and every step its own
+ * nOffset). p in [0, 1]; a dropped NaN or infinity gives 0. pOut may be pIn or pResidual. A call
+ * captured into a CUDA graph keeps its nOffset, so that every replay drops the same elements: capture
+ * omCudaDropoutAddStep instead. */
 int omCudaDropoutAdd(const void* pIn, const void* pResidual, void* pOut, long long nCount,
                      float fProb, unsigned long long nSeed, unsigned long long nOffset,
                      int nDtype);
+/* The same at offset nOffset + *pStep, where pStep is device memory (8-byte aligned) that the kernel
+ * reads when it runs: a captured training step draws new masks when *pStep is another before each
+ * replay. Forward and backward of a step see the same *pStep. */
+int omCudaDropoutAddStep(const void* pIn, const void* pResidual, void* pOut, long long nCount,
+                         float fProb, unsigned long long nSeed, unsigned long long nOffset,
+                         const unsigned long long* pStep, int nDtype);
 /* Bytes of pWorkspace of omCudaAttention (bBackward = 0) and omCudaAttentionBackward (1); a
  * negative OM_ERR_* for arguments those calls refuse. */
 long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int nKvHeads, int nSq, int nSk,

@@ -174,6 +174,7 @@ _SIGS = {
     "omCudaGroupNormActNhwc": [P, P, P, P, P, P, P, I, I, I, I, I, F, I, I],
     "omCudaGroupNormActNhwcBackward": [P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, I],
     "omCudaDropoutAdd": [P, P, P, c_longlong, F, c_ulonglong, c_ulonglong, I],
+    "omCudaDropoutAddStep": [P, P, P, c_longlong, F, c_ulonglong, c_ulonglong, P, I],
     "omCudaAttention": [P, P, P, P, P, POINTER(c_longlong), P, P, P] + [I] * 6 + [F, I, I],
     "omCudaAttentionBackward": [P, P, P, P, P, P, P, P, P, POINTER(c_longlong), P, P, P] + [I] * 6 +
                                [F, I, I],

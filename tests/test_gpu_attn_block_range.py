@@ -243,3 +243,44 @@ def test_attention_nan_scores_are_not_an_empty_row(gpu, dims, dtype):
     got, gl = c.forward()
     assert np.isnan(got[0, :, :h // hkv]).all() and np.isnan(gl[0, :h // hkv]).all()
     assert (got[1:] == want[1:]).all() and (gl[1:] == wl[1:]).all()
+
+
+# ---------------------------------------------------------------- dropout in a captured step
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_dropout_replayed_with_another_step(gpu, dtype):
+    """A captured call draws the mask of the step that device memory holds when it is replayed, the same
+    as a call with that offset."""
+    from omnimatchdeeplearningtool_b200._lib import call, lib
+    n, seed, base = 5003, 9, (1 << 40) - 2
+    rng = np.random.Generator(np.random.PCG64(dtype))
+    x, r = _dev(rng.standard_normal(n), dtype), _dev(rng.standard_normal(n), dtype)
+    step, out, one = _dev(np.zeros(1, np.uint64)), _new(n * 4), _new(n * 4)
+    args = (x.ptr, r.ptr, out.ptr, n, 0.3, seed, base, step.ptr, dtype)
+    call("omCudaDropoutAddStep", *args)
+    call("omCudaSynchronize")
+    call("omCudaGraphBeginCapture")
+    st = lib.omCudaDropoutAddStep(*args)
+    graph = ctypes.c_void_p()
+    assert lib.omCudaGraphEndCapture(ctypes.byref(graph)) == 0 and st == 0
+    seen = []
+    for s in (0, 1, 2, 1 << 33, 1):
+        step.upload(np.array([s], np.uint64))
+        call("omCudaGraphLaunch", graph)
+        call("omCudaSynchronize")
+        got = out.to_numpy((n,), np_type(dtype))
+        call("omCudaDropoutAdd", x.ptr, r.ptr, one.ptr, n, 0.3, seed, base + s, dtype)
+        assert (got == one.to_numpy((n,), np_type(dtype))).all()
+        seen.append(got)
+    call("omCudaGraphDestroy", graph)
+    assert (seen[1] == seen[4]).all() and all((a != b).any() for i, a in enumerate(seen[:4]) for b in seen[:i])
+
+
+def test_dropout_step_refusals(gpu):
+    from omnimatchdeeplearningtool_b200._lib import lib
+    b, step = _new(4096), _new(16)
+
+    def f(p=step.ptr, prob=0.1, n=8):
+        return lib.omCudaDropoutAddStep(b.ptr, None, b.ptr, n, prob, 0, 0, p, BF16)
+
+    assert f() == 0 and f(n=0) == 0
+    assert f(p=None) == -2 and f(p=step.ptr + 4) == -2 and f(prob=1.5) == -2 and f(n=-1) == -2
