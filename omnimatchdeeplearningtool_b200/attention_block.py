@@ -19,7 +19,8 @@ All calls go to the library's compute stream; results are device buffers.
 from __future__ import annotations
 
 import ctypes
-from typing import Dict, List
+import itertools
+from typing import Dict, List, Optional
 
 import numpy as np
 
@@ -31,11 +32,17 @@ DTYPES = {"bf16": DTYPE_BF16, "fp16": DTYPE_F16}
 
 class AttentionBlock:
     """``params``: host arrays gamma, beta [C], w_qkv [3C, C], b_qkv [3C], w_out [C, C], b_out [C]
-    (rows are output channels, as conv weights [Cout, Cin, 1, 1])."""
+    (rows are output channels, as conv weights [Cout, Cin, 1, 1]).
+
+    The dropout mask is that of ``seed`` and the step that :meth:`forward` is given. A model's blocks
+    need seeds of their own, since two blocks with one seed drop the same elements in a step; a block
+    that is given none takes the next number of its process."""
+
+    _seeds = itertools.count()
 
     def __init__(self, n: int, h: int, w: int, c: int, heads: int, groups: int,
                  params: Dict[str, np.ndarray], dtype: str = "bf16", dropout: float = 0.0,
-                 seed: int = 0, eps: float = 1e-5, act: int = ACT_SILU):
+                 seed: Optional[int] = None, eps: float = 1e-5, act: int = ACT_SILU):
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}")
         if c % heads or (c // heads) % 8 or c // heads > 128 or c % groups:
@@ -45,7 +52,8 @@ class AttentionBlock:
             raise ValueError("channels must be stored without padding (a multiple of 8)")
         self.n, self.h, self.w, self.c = n, h, w, c
         self.heads, self.groups, self.d, self.tokens = heads, groups, c // heads, h * w
-        self.dt, self.p, self.seed, self.eps, self.act = DTYPES[dtype], dropout, seed, eps, act
+        self.dt, self.p, self.eps, self.act = DTYPES[dtype], dropout, eps, act
+        self.seed = next(AttentionBlock._seeds) if seed is None else seed
         self.scale = 1.0 / float(np.sqrt(self.d))
         self._keep: List[DeviceBuffer] = []
         self.params = {k: self._dev(v) for k, v in params.items()}
@@ -66,7 +74,7 @@ class AttentionBlock:
         self._bwd_strides = (ctypes.c_longlong * 24)(*third, *third, *third, *one, *one,
                                                      *third, *third, *third)
         self._grads: Dict[str, DeviceBuffer] = {}
-        self.step = 0
+        self.step, self.step_ptr = -1, None
 
     # ------------------------------------------------------------------ buffers
     def _dev(self, a: np.ndarray) -> DeviceBuffer:
@@ -110,11 +118,16 @@ class AttentionBlock:
         return [base + i * self.c * 2 for i in range(3)]
 
     # ------------------------------------------------------------------ passes
-    def forward(self, x: int, step: int = 0) -> int:
-        """``x``: device pointer of the [N, H, W, C] map; returns the output's. ``step`` selects
-        the dropout mask."""
+    def forward(self, x: int, step: Optional[int] = None, step_ptr: Optional[int] = None) -> int:
+        """``x``: device pointer of the [N, H, W, C] map, which stays until the backward; returns the
+        output's. ``step`` selects the dropout mask: without one, the step after the last call's, the
+        first call's being 0. ``step_ptr``: device pointer of a 64-bit number to be added to it (then 0
+        without one), read when the pass and its backward run; a captured pass needs it to draw new
+        masks on its replays."""
         n, t, c = self.n, self.tokens, self.c
-        self.x, self.step = x, step
+        if step is None:
+            step = 0 if step_ptr else self.step + 1
+        self.x, self.step, self.step_ptr = x, step, step_ptr
         call("omCudaGroupNormActNhwc", x, self.hid.ptr, self.params["gamma"].ptr,
              self.params["beta"].ptr, self.mean.ptr, self.rstd.ptr, self.ws.ptr, n, t, c, c,
              self.groups, self.eps, self.act, self.dt)
@@ -122,9 +135,15 @@ class AttentionBlock:
         call("omCudaAttention", *self._qkv_ptrs(self.qkv.ptr), self.att.ptr, self.lse.ptr,
              self._fwd_strides, None, None, self.ws.ptr, *self.dims, self.scale, 0, self.dt)
         self._project(self.att.ptr, self.pk_out, self.out.ptr, c, c)
-        call("omCudaDropoutAdd", self.out.ptr, x, self.out.ptr, n * t * c, self.p, self.seed, step,
-             self.dt)
+        self._dropout(self.out.ptr, x, self.out.ptr)
         return self.out.ptr
+
+    def _dropout(self, x: int, residual: Optional[int], out: int) -> None:
+        count = self.n * self.tokens * self.c
+        if self.step_ptr:
+            call("omCudaDropoutAddStep", x, residual, out, count, self.p, self.seed, self.step, self.step_ptr, self.dt)
+        else:
+            call("omCudaDropoutAdd", x, residual, out, count, self.p, self.seed, self.step, self.dt)
 
     def _weight_grad(self, x: DeviceBuffer, dy: DeviceBuffer, cin: int, cout: int, dw, db) -> None:
         """dW [cout, cin] and db from channels-last 16-bit tensors, in fp32."""
@@ -151,7 +170,7 @@ class AttentionBlock:
         grads = {"x": dx, "gamma": g("gamma", c * 4), "beta": g("beta", c * 4),
                  "w_qkv": g("w_qkv", 3 * c * c * 4), "b_qkv": g("b_qkv", 3 * c * 4),
                  "w_out": g("w_out", c * c * 4), "b_out": g("b_out", c * 4)}
-        call("omCudaDropoutAdd", dout, None, dy.ptr, m * c, self.p, self.seed, self.step, self.dt)
+        self._dropout(dout, None, dy.ptr)
         self._weight_grad(self.att, dy, c, c, grads["w_out"], grads["b_out"])
         self._project(dy.ptr, self.pk_out_t, datt.ptr, c, c)
         call("omCudaAttentionBackward", datt.ptr, *self._qkv_ptrs(self.qkv.ptr), self.att.ptr,
