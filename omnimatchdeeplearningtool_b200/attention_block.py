@@ -45,11 +45,17 @@ class AttentionBlock:
                  seed: Optional[int] = None, eps: float = 1e-5, act: int = ACT_SILU):
         if dtype not in DTYPES:
             raise ValueError(f"dtype must be one of {sorted(DTYPES)}")
+        if min(n, h, w, c, heads, groups) < 1:
+            raise ValueError("sizes must be positive")
         if c % heads or (c // heads) % 8 or c // heads > 128 or c % groups:
             raise ValueError("channels must split into groups, and into heads of 8 .. 128 channels "
                              "(a multiple of 8)")
         if lib.omCudaStoredChannels(c) != c:
             raise ValueError("channels must be stored without padding (a multiple of 8)")
+        for name, count in (("gamma", c), ("beta", c), ("w_qkv", 3 * c * c), ("b_qkv", 3 * c), ("w_out", c * c),
+                            ("b_out", c)):
+            if name not in params or np.size(params[name]) != count:
+                raise ValueError(f"parameter {name} must be there, with {count} values")
         self.n, self.h, self.w, self.c = n, h, w, c
         self.heads, self.groups, self.d, self.tokens = heads, groups, c // heads, h * w
         self.dt, self.p, self.eps, self.act = DTYPES[dtype], dropout, eps, act

@@ -87,3 +87,24 @@ def test_captured_step_draws_new_masks(gpu):
     assert all((a != b).any() for a, b in zip(seen[0], seen[1])) and all((a != b).any() for a, b in zip(seen[1], seen[2]))
     call("omCudaGraphDestroy", graph)
     blk.close()
+
+
+@pytest.mark.parametrize("name", ["gamma", "beta", "w_qkv", "b_qkv", "w_out", "b_out"])
+def test_block_refuses_parameters_of_another_size(name):
+    """Refused before anything reaches the device, where the kernels would read past the array."""
+    from omnimatchdeeplearningtool_b200.attention_block import AttentionBlock
+    prm = _params()
+    prm[name] = prm[name][:-1]
+    with pytest.raises(ValueError, match=name):
+        AttentionBlock(N, H, W, C, HEADS, GROUPS, prm)
+    del prm[name]
+    with pytest.raises(ValueError, match=name):
+        AttentionBlock(N, H, W, C, HEADS, GROUPS, prm)
+
+
+@pytest.mark.parametrize("sizes", [(0, H, W, C, HEADS, GROUPS), (N, -1, W, C, HEADS, GROUPS), (N, H, 0, C, HEADS, GROUPS),
+                                   (N, H, W, 0, HEADS, GROUPS), (N, H, W, C, 0, GROUPS), (N, H, W, C, HEADS, -8)])
+def test_block_refuses_empty_sizes(sizes):
+    from omnimatchdeeplearningtool_b200.attention_block import AttentionBlock
+    with pytest.raises(ValueError):
+        AttentionBlock(*sizes, _params())
