@@ -284,3 +284,43 @@ def test_dropout_step_refusals(gpu):
 
     assert f() == 0 and f(n=0) == 0
     assert f(p=None) == -2 and f(p=step.ptr + 4) == -2 and f(prob=1.5) == -2 and f(n=-1) == -2
+
+
+# ---------------------------------------------------------------- dropout past 32 bits of elements and of groups
+@pytest.mark.parametrize("shift", [32, 35])
+def test_dropout_long_tensors(gpu, shift):
+    """The last elements of an in-place call of 2^32 + 24 (2^35 + 24) elements are those of their own
+    index: past 2^32 the element offset, past 2^35 the group index needs its high word."""
+    import torch
+    from omnimatchdeeplearningtool_b200._lib import call
+    from omnimatchdeeplearningtool_b200.backend import DeviceBuffer
+    n = (1 << shift) + 24
+    if torch.cuda.mem_get_info(0)[0] < 2 * n + (8 << 30):
+        pytest.skip("not enough free device memory")
+    buf = DeviceBuffer(2 * n)
+    try:
+        call("omCudaMemset", buf.ptr, 0x3F, buf.nbytes)       # 0x3F3F, 0.74609375
+        call("omCudaDropoutAdd", buf.ptr, None, buf.ptr, n, 0.5, 77, 5, BF16)
+        last = np.zeros(4096 + 24, np.uint16)
+        call("omCudaCopyD2H", last.ctypes.data, buf.ptr + 2 * (n - last.size), last.nbytes)
+        first = np.zeros(4096, np.uint16)
+        call("omCudaCopyD2H", first.ctypes.data, buf.ptr, first.nbytes)
+    finally:
+        buf.free()
+    keep, _ = ref.keep_mask(last.size, 0.5, 77, 5, first=n - last.size)
+    assert ((last != 0) == keep).all() and (last[keep] == 0x3FBF).all()
+    keep, _ = ref.keep_mask(4096, 0.5, 77, 5)
+    assert ((first != 0) == keep).all()
+
+
+def test_attention_backward_scale_limits(gpu):
+    from omnimatchdeeplearningtool_b200._lib import lib
+    b, ws, g = _new(1 << 16), _new(1 << 20), _new(1 << 16)
+    st = (ctypes.c_longlong * 24)(*[256, 64, 64] * 8)
+
+    def f(scale):
+        return lib.omCudaAttentionBackward(b.ptr, b.ptr, b.ptr, b.ptr, b.ptr, b.ptr, g.ptr, g.ptr + 8192, g.ptr + 16384, st,
+                                           None, None, ws.ptr, 1, 1, 1, 4, 4, 64, scale, 0, BF16)
+
+    assert f(2.0 ** -20) == 0 and f(-2.0 ** -20) == 0 and f(4.0) == 0
+    assert f(2.0 ** -21) == -3 and f(0.0) == -3 and f(float("inf")) == -2 and f(float("nan")) == -2
