@@ -771,8 +771,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 // delta_i, and the largest |V_j| of the head from a launch before (vmax, per 128 keys); dK's rows take
 // their own |V_j|, and from the dQ kernel the largest |dO_i| and |delta_i| of the queries that the
 // CTA streams (qmax, squared and not, per 32 queries). bf16 has fp32's range and needs none of it. In
-// fp16 the launch and the bounds cost 6 to 13 us: 32 x 12 heads of 197 tokens 71 -> 79 us, the ragged
-// causal batch 61 -> 67, 24 heads of 4096 tokens 403 -> 416 (bf16, by the multiply that went: 403 -> 386).
+// fp16 the launch and the bounds cost 6 to 8 us of a short call: 32 x 12 heads of 197 tokens 71 -> 79 us,
+// the ragged causal batch 61 -> 67, 24 heads of 4096 tokens 403 -> 413 (bf16, by the multiply that went
+// and the order of the products: 403 -> 385).
 struct Factor { float f, inverse; };
 // P for dV is 1 at most, and in fp16 below 2^-14 no normal number (1e-7 came out up to 30 % off, and
 // with it the dV of a key that every query gives so little): there the dK/dV kernel works with 2^14 P,
@@ -799,28 +800,36 @@ __device__ __forceinline__ float squares(const uint4& u) {
     return s;
 }
 // vmax: the largest sum of squares of a value row of 128 keys, rows that are not finite left out. 8 or
-// 16 lanes a row, one 16-byte load each
+// 16 lanes a row, one 16-byte load each, 32 rows at a time; all of a thread's loads go out before anything waits (one after
+// another, behind the length, they took 8 us of an idle GPU's time instead of 5)
 template <int DT>
-__global__ void __launch_bounds__(256) value_norms_kernel(const Params p) {
-    __shared__ float sh[8];
+__global__ void __launch_bounds__(512) value_norms_kernel(const Params p) {
+    __shared__ float sh[16];
     pdl_launch_dependents();
     const int tiles = (p.Sk + 127) / 128, t0 = blockIdx.x % tiles * 128, bh = blockIdx.x / tiles;
-    const int b = bh / p.Hkv, h = bh - b * p.Hkv, end = min(len_of(p.kvlens, b, p.Sk), t0 + 128);
-    const int wide = p.D <= 64 ? 8 : 16, col = threadIdx.x % wide * 8;
+    const int b = bh / p.Hkv, h = bh - b * p.Hkv, end = len_of(p.kvlens, b, p.Sk);
+    const int wide = blockDim.x / 32, col = threadIdx.x % wide * 8, r = threadIdx.x / wide;
+    uint4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int t = r + i * 32;
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (t0 + t < p.Sk && col < p.D)
+            v[i] = __ldg(reinterpret_cast<const uint4*>(row<DT>(p.v, b, t0 + t, h) + col));
+    }
     float most = 0.f;
-#pragma unroll 4
-    for (int r = threadIdx.x / wide; r < 128; r += 256 / wide) {
-        float s = 0.f;
-        if (t0 + r < end && col < p.D) s = squares<DT>(__ldg(reinterpret_cast<const uint4*>(row<DT>(p.v, b, t0 + r, h) + col)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float s = squares<DT>(v[i]);
         for (int o = wide / 2; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
-        most = fmaxf(most, if_finite(s));
+        if (t0 + r + i * 32 < end) most = fmaxf(most, if_finite(s));
     }
     most = warp_max(most);
     if (threadIdx.x % 32 == 0) sh[threadIdx.x / 32] = most;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; ++i) most = fmaxf(most, sh[i]);
-        p.vmax[blockIdx.x] = most;
+    if (threadIdx.x < 32) {
+        most = warp_max(threadIdx.x < wide ? sh[threadIdx.x] : 0.f);
+        if (threadIdx.x == 0) p.vmax[blockIdx.x] = most;
     }
 }
 constexpr int max_of(int a, int b) { return a > b ? a : b; }
@@ -1456,7 +1465,7 @@ static int backward(DeviceCtx* c, Params p) {
     if (norms) {
         const long long blocks = (long long)p.B * p.Hkv * ((p.Sk + 127) / 128);
         if (blocks > 0x7FFFFFFF) return OM_ERR_UNSUPPORTED;
-        value_norms_kernel<DT><<<(unsigned)blocks, 256, 0, c->compute>>>(p);
+        value_norms_kernel<DT><<<(unsigned)blocks, p.D <= 64 ? 256 : 512, 0, c->compute>>>(p);
         st = after_launch(c);
         if (st != OM_OK) return st;
     }
