@@ -49,7 +49,8 @@ extern "C" {
 #define OM_ACT_NONE 0
 #define OM_ACT_RELU 1
 #define OM_ACT_RELU6 2
-/* x * sigmoid(x): only in the GroupNorm entry points (omCudaGroupNormActNhwc and its backward) */
+/* x * sigmoid(x): only in the GroupNorm entry points (omCudaGroupNormActNhwc and its backward);
+ * OM_ERR_UNSUPPORTED elsewhere */
 #define OM_ACT_SILU 3
 
 /* ---------------- device, memory, streams ---------------- */

@@ -1362,6 +1362,7 @@ extern "C" int omCudaConv2dBnAct(const void* pInput, const void* pPacked, const 
         return OM_ERR_INVALID;
     if (nDtype != OM_DTYPE_BF16 && nDtype != OM_DTYPE_F16) return OM_ERR_UNSUPPORTED;
     if (nOutDtype != nDtype && nOutDtype != OM_DTYPE_F32) return OM_ERR_UNSUPPORTED;
+    if (nAct == OM_ACT_SILU) return OM_ERR_UNSUPPORTED;   // GroupNorm's only
     if (nCs % 8 != 0 || nCout % 8 != 0) return OM_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(pInput) | reinterpret_cast<uintptr_t>(pPacked) |
          reinterpret_cast<uintptr_t>(pOutput) | reinterpret_cast<uintptr_t>(pResidual) |
@@ -2370,7 +2371,7 @@ static int stem_conv(const void* pInput, int nInDtype, void* pWorkspace, const v
         nStride <= 0 || nPad < 0)
         return OM_ERR_INVALID;
     if (nDtype != OM_DTYPE_BF16 && nDtype != OM_DTYPE_F16) return OM_ERR_UNSUPPORTED;
-    if (nCout % 8 != 0) return OM_ERR_UNSUPPORTED;
+    if (nCout % 8 != 0 || nAct == OM_ACT_SILU) return OM_ERR_UNSUPPORTED;
     StemGeom g;
     if (!stem_geom(nCin, nH, nW, nKH, nKW, nStride, nPad, &g)) {
         const int P = (nH + 2 * nPad - nKH) / nStride + 1;
@@ -3040,6 +3041,7 @@ extern "C" int omCudaConvPairBnAct(const void* pInput, const void* pPacked1, con
     if (nBatch <= 0 || nH <= 0 || nW <= 0 || nKH <= 0 || nKW <= 0 || nStride <= 0 || nPad < 0)
         return OM_ERR_INVALID;
     if (!omCudaConvPairSupported(nCs, nMid, nCout, nDtype)) return OM_ERR_UNSUPPORTED;
+    if (nAct1 == OM_ACT_SILU || nAct2 == OM_ACT_SILU) return OM_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(pInput) | reinterpret_cast<uintptr_t>(pPacked1) |
          reinterpret_cast<uintptr_t>(pPacked2) | reinterpret_cast<uintptr_t>(pOutput) |
          reinterpret_cast<uintptr_t>(pResidual) | reinterpret_cast<uintptr_t>(pBias1) |

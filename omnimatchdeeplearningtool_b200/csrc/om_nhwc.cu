@@ -650,6 +650,7 @@ extern "C" int omCudaDepthwiseConv2dNhwc(const void* pIn, const float* pPacked, 
     if (!pIn || !pOut || !pPacked || !pBias || nCs % 8 || !aligned16(pIn) || !aligned16(pOut) ||
         !aligned16(pPacked) || !aligned16(pBias))
         return OM_ERR_INVALID;
+    if (nAct == OM_ACT_SILU) return OM_ERR_UNSUPPORTED;   // GroupNorm's only
     int P = (nH + 2 * nPad - nKH) / nStride + 1, Q = (nW + 2 * nPad - nKW) / nStride + 1;
     if (P <= 0 || Q <= 0) return OM_ERR_INVALID;
     const long long rows = (long long)nN * P;
@@ -692,6 +693,7 @@ extern "C" int omCudaAddActNhwc(const void* pA, const void* pB, void* pOut, long
     OMB_CTX_OR_FAIL(c);
     if (!pA || !pB || !pOut || nCount % 8 || !aligned16(pA) || !aligned16(pB) || !aligned16(pOut))
         return OM_ERR_INVALID;
+    if (nAct == OM_ACT_SILU) return OM_ERR_UNSUPPORTED;   // GroupNorm's only
     long long n8 = nCount / 8;
     int grid = ew_grid(c, n8, 256);
     if (nDtype == OM_DTYPE_BF16)
