@@ -650,7 +650,8 @@ long long omCudaAttentionWorkspaceBytes(int nBatch, int nHeads, int nKvHeads, in
  * are positive; strides are multiples of 8 and pointers 16-byte aligned.
  * pQLens, pKvLens: optional device arrays [nBatch] of the tokens in use (clamped to [0, nSq] and
  * [0, nSk]); what tokens past them hold is not used, NaN and infinities included. bCausal: query i
- * sees keys j <= i + kvLen - qLen. A query that sees no key, or lies past its length, gets zeros.
+ * sees keys j <= i + kvLen - qLen (of a key within the lengths that it does not see, a NaN or an
+ * infinity in V may reach it all the same, as zero times that). A query that sees no key, or lies past its length, gets zeros.
  * pLse [nBatch, nHeads, nSq] fp32 (NULL when no backward follows): log(sum exp(score)) of each
  * query, minus infinity where it sees no key, NaN (as its output) where a score is NaN or plus
  * infinity. nDtype BF16 or F16, nHeadDim a multiple of 8 up to

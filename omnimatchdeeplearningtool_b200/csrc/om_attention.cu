@@ -270,8 +270,9 @@ constexpr float LN2 = 0.6931471805599453f;
 // Per tile and block:
 //   S = Q K^T (TMEM, fp32) -> running maximum, P = exp(S - m), row sums -> P (TMEM, 16-bit, over
 //   S's columns) -> O += P V (TMEM, fp32).
-// O is rescaled only when a row's maximum has grown by more than 2^8 since its last reference
-// maximum: P stays below 2^8, in range of both types, and the factor cancels in O / l.
+// The running maximum and sum are those of Milakov and Gimelshein (2018). O is rescaled only when a
+// row's maximum has grown by more than 2^8 since its last reference maximum (a known refinement): P
+// stays below 2^8, in range of both types, and the factor cancels in O / l.
 // Score tile n = NT j + t (block j, query tile t) lies in TMEM buffer n % NB, counted over all items.
 // There are more buffers than query tiles, so that a tile's next scores are there when its
 // probabilities are done (without, a softmax warp waited about 900 of 2900 clocks a block for them):
@@ -296,7 +297,8 @@ struct FwdCfg {
     static constexpr bool MORE_REGS = KB == 128;
     static constexpr int THREADS = NT * 128 + (MORE_REGS ? 128 : 64), OCC = NT == 1 ? 2 : 1;
     static constexpr int MATH_REGS = 208, OTHER_REGS = 80;
-    // registers a thread that the launch must have for that split, else the softmax warps would wait
+    // Registers a thread that the launch must have for that split, else the softmax warps would wait.
+    // The compiler gives such a kernel all that its launch bounds allow (168); the host checks it
     static constexpr int LAUNCH_REGS = MORE_REGS ? (NT * 128 * MATH_REGS + 128 * OTHER_REGS + THREADS - 1) / THREADS : 0;
     static constexpr int TMEM_COLS = NT * 256;
     static constexpr int NB = KB == 64 ? 2 * NT : 3;
@@ -1287,7 +1289,9 @@ static int join(DeviceCtx* c, const Params& p, const View& out, int T, int H, co
 // estimated time, in blocks: the longest part or the even share of all of them, each part with about
 // 4 blocks' time for its start and end; joining costs about 3 (another launch) and grows with the
 // parts. Parts of two blocks at least. (84 tiles of 28 causal blocks: 3 parts, 62 -> 32 us; 16 tiles
-// of 32 blocks: 16 parts, 55 -> 18 us.)
+// of 32 blocks: 16 parts, 55 -> 18 us: the constants come from these two.) The forward's blocks count
+// as 128 keys, also where it takes two of 64; lengths are on the device and count as full. The number
+// of SMs is a constant, as the workspace's size has to be the same without a device to ask.
 static int parts(long long ctas, int blocks, int places, bool causal) {
     int best = 1;
     float least = INFINITY;

@@ -63,7 +63,7 @@ __device__ __forceinline__ void dropout_group(const Params& p, uint32_t o0, uint
     }
 }
 
-// One thread per 8 elements, four groups in flight: the loads of all four go out before the first
+// One thread per 8 elements, four groups in flight (fp32: two): the loads of all go out before the first
 // group's generator rounds (with one, 56 us for 50 M f16 elements whose copy takes 31 us; the
 // rounds alone are about half of that in issue slots). VEC: all pointers 16-byte aligned, so full
 // groups move in 16-byte accesses; the last group, and every group otherwise, goes element by

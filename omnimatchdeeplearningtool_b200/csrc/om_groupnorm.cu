@@ -801,7 +801,8 @@ static int check_shape(int nN, int nHW, int nC, int nCs, int nGroups, int nDtype
 }
 static bool aligned(const void* p, int a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-// GV of a number of channels per group
+// GV of a number of channels per group. Other multiples of 4 than these could keep two entries as well;
+// only 4 and multiples of 8, the usual ones, were measured so, and the rest take the general form
 static int entries(int cpg) { return cpg % 8 == 0 ? 1 : cpg == 4 ? 2 : 8; }
 
 // Fills in the split of the work: p->cluster > 0 for the one-launch form with `smem` bytes,
